@@ -50,6 +50,73 @@ def dequantize_fp8b16(
     return (g * scales.to(torch.float32).unsqueeze(-1)).reshape(payload.shape).to(dtype)
 
 
+# -- the 4-bit format ---------------------------------------------------------------
+#
+# fp4b16 (oracle of ``ops/csrc/fp4.cuh``): groups of 16 consecutive ``dim`` elements share one scale.  A value is e2m1 (0, 0.5, 1,
+# 1.5, 2, 3, 4, 6 with a sign, two to a byte, the even element in the low half); a scale is 8 bits, the upper 8 of the 15
+# magnitude bits of an f16 (five exponent and three mantissa bits).  ``s = round4(f16(absmax * fl(1/6)))``, four significant bits,
+# at most 10240; the payload is ``rne_e2m1(fl(x / s))``, saturating at 6.  A group with an infinity or a NaN has
+# scale byte 255 and reads back as NaN.
+
+_E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+FP4_MAX_SCALE = 10240.0
+
+
+def fp4_scale_values(scales: torch.Tensor) -> torch.Tensor:
+    """uint8 scale bytes -> the fp32 values they stand for."""
+    return (scales.to(torch.int32) << 7).to(torch.int16).view(torch.float16).to(torch.float32)
+
+
+def quantize_fp4b16(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``x[..., D]`` (any float dtype) -> (uint8 codes ``[..., D/2]``, uint8 scales ``[..., D/16]``)."""
+    if x.shape[-1] % FP8_GROUP:
+        raise ValueError("last dimension must be a multiple of 16")
+    xf = x.detach().to(torch.float32)
+    g = xf.reshape(*xf.shape[:-1], xf.shape[-1] // FP8_GROUP, FP8_GROUP)
+    absmax = g.abs().amax(dim=-1)  # propagates NaN
+    t = (absmax * torch.tensor(1.0 / 6.0, dtype=torch.float32)).clamp(max=FP4_MAX_SCALE)
+    bits = t.to(torch.float16).view(torch.int16).to(torch.int32)
+    byte = (bits + 63 + ((bits >> 7) & 1)) >> 7
+    byte = torch.where(torch.isfinite(absmax), byte, torch.full_like(byte, 255)).to(torch.uint8)
+    s = fp4_scale_values(byte).unsqueeze(-1)
+    ok = s > 0  # false for a group that rounds to nothing and for one that is not finite
+    y = torch.where(ok, torch.div(g, torch.where(ok, s, torch.ones_like(s))), torch.copysign(torch.zeros_like(g), g))
+    borders = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    a = y.abs()
+    code = torch.bucketize(a, borders)  # borders below a: a tie goes down ...
+    for i in (1, 3, 5):  # ... except where the code above is the even one
+        code = torch.where(a == borders[i], torch.full_like(code, i + 1), code)
+    code = (code.to(torch.uint8) | (torch.signbit(y).to(torch.uint8) << 3)).reshape(x.shape)
+    return code[..., 0::2] | (code[..., 1::2] << 4), byte
+
+
+def dequantize_fp4b16(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values that (codes ``[..., D/2]``, scales ``[..., D/16]``) stand for (exact in bf16 and fp32)."""
+    table = torch.tensor(_E2M1 + tuple(-v for v in _E2M1))
+    v = torch.stack([table[(codes & 15).long()], table[(codes >> 4).long()]], -1).reshape(*codes.shape[:-1], -1)
+    g = v.reshape(*scales.shape, FP8_GROUP)
+    return (g * fp4_scale_values(scales).unsqueeze(-1)).reshape(v.shape).to(dtype)
+
+
+def pack_kv4_records(k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+    """``k, v [..., 16, 128]`` of one page -> its record ``[..., 2304]`` (uint8), the layout of ``ops/csrc/kv4.h``."""
+    lead = k.shape[:-2]
+    (kc, ks), (vc, vs) = quantize_fp4b16(k), quantize_fp4b16(v)
+    vc = vc.reshape(*lead, 2, 8, 8, 8).transpose(-3, -2)  # [token / 8][group][token % 8][8]
+    vs = vs.reshape(*lead, 2, 8, 8).transpose(-2, -1)
+    return torch.cat([t.reshape(*lead, -1) for t in (kc, vc, ks, vs)], dim=-1)
+
+
+def unpack_kv4_records(records: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Inverse of :func:`pack_kv4_records`: fp32 ``k, v [..., 16, 128]``."""
+    lead = records.shape[:-1]
+    kc, vc, ks, vs = records.split([1024, 1024, 128, 128], dim=-1)
+    k = dequantize_fp4b16(kc.reshape(*lead, 16, 64), ks.reshape(*lead, 16, 8))
+    vc = vc.reshape(*lead, 2, 8, 8, 8).transpose(-3, -2).reshape(*lead, 16, 64)
+    vs = vs.reshape(*lead, 2, 8, 8).transpose(-2, -1).reshape(*lead, 16, 8)
+    return k, dequantize_fp4b16(vc, vs)
+
+
 # -- RoPE ---------------------------------------------------------------------------
 
 

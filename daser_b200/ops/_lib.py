@@ -37,6 +37,21 @@ class KVPool(C.Structure):
     ]
 
 
+class KV4Pool(C.Structure):
+    """Mirror of ``DaserKV4Pool`` (``ops/csrc/kv4.h``)."""
+
+    _fields_ = [
+        ("records", C.c_void_p * MAX_RANKS),
+        ("stride_layer", C.c_int64),
+        ("stride_block", C.c_int64),
+        ("stride_head", C.c_int64),
+        ("num_layers", C.c_int32),
+        ("num_blocks", C.c_int32),
+        ("n_ranks", C.c_int32),
+        ("heads_per_rank", C.c_int32),
+    ]
+
+
 class KVJob(C.Structure):
     """Mirror of ``DaserKVJob``."""
 
@@ -142,6 +157,59 @@ def check(code: int, what: str) -> None:
     if code < 0:
         raise KernelError(f"{what}: {_ERRORS.get(code, code)}")
     raise KernelError(f"{what}: CUDA error {code}")
+
+
+# Entry points of the 4-bit pool, with their argument types: declared once, so that a call converts plain
+# ints (a decode step makes these calls per layer).
+_P, _I, _L, _F = C.c_void_p, C.c_int, C.c_int64, C.c_float
+_KV4_ARGS = {
+    "daser_rope_kv4_write": [_P, _I, _L, _P, _P, _P, _I, _P, _I, _I, _I, _P, _I, _I, _I, _P, _P, _F, _P],
+    "daser_kv4_read": [_P, _I, _I, _P, _P, _P, _I, _P],
+    "daser_kv4_restore": [_P, _P, _P],
+    "daser_kv4_save": [_P, _P, _P],
+    "daser_kv4_page_bounds": [_P, _I, _I, _P, _P, _P, _I, _P, _P, _I, _I, _P],
+    "daser_quant_fp4b16": [_P, _P, _P, _L, _P],
+    "daser_dequant_fp4b16": [_P, _P, _P, _L, _P],
+    "daser_paged_attention_kv4": [_P, _P, _P, _P, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P],
+    "daser_sparse_attention_kv4": [_P, _P, _P, _P, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _P, _I, _I, _I, _F, _P],
+    "daser_select_pages_kv4": [_P, _P, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _P, _I, _P, _I, _I, _I, _P],
+}
+_kv4_fns: dict = {}
+
+
+def kv4_fn(name: str):
+    """The C function ``name`` of the 4-bit pool with its argument types set."""
+    fn = _kv4_fns.get(name)
+    if fn is None:
+        fn = getattr(lib(), name)
+        fn.argtypes, fn.restype = _KV4_ARGS[name], C.c_int
+        _kv4_fns[name] = fn
+    return fn
+
+
+def require(cond: bool, what: str) -> None:
+    """Argument checks of the 4-bit pool's operators."""
+    if not cond:
+        raise ValueError(what)
+
+
+def check_tensor(t, name: str, dtype, device) -> None:
+    """``t`` is a contiguous tensor of ``dtype`` on the CUDA device ``device``."""
+    if t.dtype != dtype or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name}: needs a contiguous {dtype} tensor on {device}, got {t.dtype} on {t.device}, strides {tuple(t.stride())}")
+
+
+def call_on(device, fn, what: str, *args, stream=None) -> None:
+    """``fn(*args, stream)`` with ``device`` current: its current stream unless one is given."""
+    import torch
+
+    if device.index is not None and device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            s = stream if stream is not None else torch.cuda.current_stream()
+            check(fn(*args, s.cuda_stream), what)
+        return
+    s = stream if stream is not None else torch.cuda.current_stream()
+    check(fn(*args, s.cuda_stream), what)
 
 
 def stream_ptr(stream=None) -> C.c_void_p:

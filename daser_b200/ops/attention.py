@@ -1,4 +1,6 @@
-"""Paged attention over the block-scaled fp8 pool (``ops/csrc/attention.cu``)."""
+"""Paged attention over the block-scaled fp8 pool (``ops/csrc/attention.cu``) and over the 4-bit pool
+(``ops/csrc/attention4.cu``, ``attention4_tc.cu``), there also over pages selected per query
+(``ops/csrc/attention4_select.cu``)."""
 
 from __future__ import annotations
 
@@ -9,7 +11,7 @@ from typing import Optional
 import torch
 
 from daser_b200.ops import _lib
-from daser_b200.ops.kv_ops import PagedKVPool
+from daser_b200.ops.kv_ops import KV4_DIM, KV4_TOKENS, PageBounds, PagedKV4Pool, PagedKVPool
 
 NUM_SMS = 148
 MAX_ROW_SPLITS = 262144  # (query rows x KV splits) the split-KV scratch is sized for (135 MB)
@@ -70,25 +72,70 @@ def plan_splits(num_seqs: int, kv_heads: int, max_q_len: int, group: int, max_ct
     return nsplit, split_tokens
 
 
+def kv4_status() -> int:
+    """Non-zero if a CTA of the 4-bit attention kernels ever gave up on a bounded wait (synchronises): bit 0 decode,
+    bit 1 prefill."""
+    out, bits = C.c_uint32(0), 0
+    for bit, name in enumerate(("daser_attention4_status", "daser_attention4_tc_status")):
+        _lib.check(getattr(_lib.lib(), name)(C.byref(out)), name)
+        bits |= int(out.value != 0) << bit
+    return bits
+
+
+def plan_splits_kv4(num_seqs: int, kv_heads: int, max_q_len: int, group: int, max_pages: int, rows: int = 0) -> tuple[int, int]:
+    """(nsplit, pages per split) of attention over the 4-bit pool (``max_pages``: of the longest context, or of a page list)."""
+    max_pages = max(1, max_pages)
+    if max_q_len * group >= TC_MIN_ROWS:
+        # tcgen05 kernel: a CTA of 128 query rows, two per SM, tiles of four pages; splits of two tiles at the shortest
+        items = num_seqs * kv_heads * -(-max_q_len // (128 // group))
+        nsplit = max(1, min((NUM_SMS * 2) // max(items, 1), -(-max_pages // 8), 64))
+        if rows > 0:
+            nsplit = max(1, min(nsplit, MAX_ROW_SPLITS // rows))
+        per = -(--(-max_pages // nsplit) // 4) * 4
+        return -(-max_pages // per), per
+    tiles = 1 if max_q_len * group <= 8 else -(-max_q_len * group // 16)
+    items = max(1, num_seqs * kv_heads * tiles)
+    slots = NUM_SMS * (4 if max_q_len * group <= 8 else 3)  # resident CTAs
+    # one wave of CTAs when the batch is small, 128 pages (2048 keys) a CTA when it is large, never less than four pages a warp
+    nsplit = max(slots // items, -(-max_pages // 128), 1)
+    nsplit = max(1, min(nsplit, max_pages // 16, 256))
+    if rows > 0:
+        nsplit = max(1, min(nsplit, MAX_ROW_SPLITS // rows))
+    per = -(-max_pages // nsplit)
+    return -(-max_pages // per), per
+
+
 class AttentionWorkspace:
-    """Scratch for split-KV partials, grown on demand and reused."""
+    """Scratch for split-KV partials, grown on demand and reused.
+
+    Calls that use one workspace have to be ordered (one stream, or events between streams), graph replays included.  When it
+    grows it keeps the smaller buffers, whose addresses captured graphs may hold."""
 
     def __init__(self, device) -> None:
         self.device = device
         self.part_o: Optional[torch.Tensor] = None
         self.part_lse: Optional[torch.Tensor] = None
+        self.scores: Optional[torch.Tensor] = None  # of select_pages
+        self._outgrown: list = []
 
     def ensure(self, rows: int, nsplit: int, head_dim: int) -> None:
         need = rows * nsplit
         if self.part_lse is None or self.part_lse.numel() < need:
+            self._outgrown += [self.part_o, self.part_lse]
             self.part_o = torch.empty(need * head_dim, dtype=torch.float32, device=self.device)
             self.part_lse = torch.empty(need, dtype=torch.float32, device=self.device)
+
+    def ensure_scores(self, need: int) -> torch.Tensor:
+        if self.scores is None or self.scores.numel() < need:
+            self._outgrown.append(self.scores)
+            self.scores = torch.empty(need, dtype=torch.float32, device=self.device)
+        return self.scores
 
 
 def paged_attention(
     q: torch.Tensor,
     out: torch.Tensor,
-    pool: PagedKVPool,
+    pool: PagedKVPool | PagedKV4Pool,
     layer: int,
     block_tables: torch.Tensor,
     q_start: torch.Tensor,
@@ -97,7 +144,7 @@ def paged_attention(
     max_ctx: int,
     num_kv_heads: int,
     softmax_scale: float,
-    workspace: AttentionWorkspace,
+    workspace: Optional[AttentionWorkspace],
     rank: int = 0,
     block_tokens: int = 16,
     nsplit: Optional[int] = None,
@@ -106,8 +153,17 @@ def paged_attention(
     """``q, out``: bf16 ``[Tq, Hq, D]``; sequences given by ``q_start`` (prefix sums) and ``ctx_lens``.
 
     The K/V of the new tokens must already be in the pool; row ``t`` of a sequence attends
-    keys ``0 .. ctx_len - q_len + t``.
+    keys ``0 .. ctx_len - q_len + t`` (a row with none gets zeros); rows behind the last sequence are left as they were.
+
+    Over a :class:`~daser_b200.ops.kv_ops.PagedKV4Pool` any group of up to 16 query heads per KV head is taken,
+    ``max_ctx`` has to be at least the longest context, and ``workspace`` may be ``None`` (scratch of the call's own).
     """
+    if isinstance(pool, PagedKV4Pool):
+        _lib.require(block_tokens == KV4_TOKENS and num_kv_heads == pool.heads_per_rank, "block_tokens or num_kv_heads are not the pool's")
+        _lib.require((nsplit is None) == (split_tokens is None) and (split_tokens is None or split_tokens % KV4_TOKENS == 0),
+                     "nsplit and split_tokens (a multiple of 16) go together")
+        return _attention_kv4(q, out, pool, layer, block_tables, q_start, ctx_lens, max_q_len, max_ctx, softmax_scale, workspace, rank,
+                              None, nsplit, split_tokens // KV4_TOKENS if split_tokens is not None else None)
     Tq, Hq, D = q.shape
     num_seqs = ctx_lens.numel()
     assert block_tables.dtype == torch.int32 and q_start.dtype == torch.int32 and ctx_lens.dtype == torch.int32
@@ -131,3 +187,122 @@ def paged_attention(
     if nsplit > 1:
         _lib.launch_count += 1  # the merge kernel
     return out
+
+
+def _check_step(q, out, pool_device, kv_heads, block_tables, q_start, ctx_lens, max_q_len) -> tuple[int, int, int]:
+    """The arguments every 4-bit attention call shares; (query rows, query heads, sequences)."""
+    need = _lib.require
+    need(q.dim() == 3 and q.shape[2] == KV4_DIM, "q: [rows, heads, 128]")
+    Tq, Hq, _ = q.shape
+    need(Hq > 0 and Hq % kv_heads == 0 and Hq // kv_heads <= 16, "1 to 16 query heads per KV head")
+    _lib.check_tensor(q, "q", torch.bfloat16, pool_device)
+    if out is not None:
+        _lib.check_tensor(out, "out", torch.bfloat16, pool_device)
+        need(out.numel() >= q.numel(), "out is smaller than q")
+    _lib.check_tensor(block_tables, "block_tables", torch.int32, pool_device)
+    _lib.check_tensor(q_start, "q_start", torch.int32, pool_device)
+    _lib.check_tensor(ctx_lens, "ctx_lens", torch.int32, pool_device)
+    n = ctx_lens.numel()
+    need(block_tables.dim() == 2 and block_tables.shape[0] >= n and q_start.numel() == n + 1, "one table row per sequence, one q_start more")
+    need(max_q_len >= 0, "max_q_len")
+    return Tq, Hq, n
+
+
+def _attention_kv4(q, out, pool, layer, block_tables, q_start, ctx_lens, max_q_len, max_ctx, softmax_scale, workspace, rank, pages,
+                   nsplit, split_pages) -> torch.Tensor:
+    pool.check(layer, rank)
+    Tq, Hq, n = _check_step(q, out, pool.device, pool.heads_per_rank, block_tables, q_start, ctx_lens, max_q_len)
+    Hkv = pool.heads_per_rank
+    max_pages = pages.shape[2] if pages is not None else -(-max_ctx // KV4_TOKENS)
+    if nsplit is None:
+        if pages is not None:  # every query row is an item of its own
+            nsplit, split_pages = plan_splits_kv4(Tq, Hkv, 1, Hq // Hkv, max_pages, rows=Tq * Hq)
+        else:
+            nsplit, split_pages = plan_splits_kv4(n, Hkv, max_q_len, Hq // Hkv, max_pages, rows=Tq * Hq)
+    _lib.require(nsplit >= 1 and split_pages >= 1 and nsplit * split_pages >= max_pages, "the splits do not cover max_ctx")
+    po = pl = None
+    if nsplit > 1:
+        if workspace is None:
+            workspace = AttentionWorkspace(q.device)
+        workspace.ensure(Tq * Hq, nsplit, KV4_DIM)
+        _lib.require(workspace.part_o.device == q.device, "the workspace is on another device")
+        po, pl = workspace.part_o.data_ptr(), workspace.part_lse.data_ptr()
+    head = (q.data_ptr(), out.data_ptr(), po, pl, pool.c_ptr, layer, rank, block_tables.data_ptr(), block_tables.shape[1],
+            q_start.data_ptr(), ctx_lens.data_ptr(), n, Tq, max_q_len, Hq)
+    if pages is None:
+        _lib.call_on(pool.device, _lib.kv4_fn("daser_paged_attention_kv4"), "paged_attention_kv4", *head, nsplit, split_pages,
+                     softmax_scale)
+    else:
+        _lib.call_on(pool.device, _lib.kv4_fn("daser_sparse_attention_kv4"), "sparse_attention_kv4", *head, pages.data_ptr(), max_pages,
+                     nsplit, split_pages, softmax_scale)
+    if nsplit > 1:
+        _lib.launch_count += 1  # the merge kernel
+    return out
+
+
+def select_pages(
+    q: torch.Tensor,
+    bounds: PageBounds,
+    layer: int,
+    block_tables: torch.Tensor,
+    q_start: torch.Tensor,
+    ctx_lens: torch.Tensor,
+    max_q_len: int,
+    max_ctx: int,
+    num_pages: int,
+    sink_pages: int = 1,
+    recent_pages: int = 4,
+    workspace: Optional[AttentionWorkspace] = None,
+) -> torch.Tensor:
+    """The pages every query row reads per KV head: int32 ``[Tq, Hkv, num_pages]``, logical pages in ascending order, -1
+    behind the last.
+
+    Always the first ``sink_pages`` and the last ``recent_pages`` (at least one: the page of the newest key, whose bounds need not be
+    up to date) of the pages a row sees; the other places go to the highest bounds on the sum of the group's scores, the lower
+    page first among equals.  A row that sees at most ``num_pages`` pages gets them all.  ``bounds`` have to cover the context
+    (:func:`~daser_b200.ops.kv_ops.update_page_bounds`); other arguments as in :func:`paged_attention`.
+    """
+    Hkv, dev = bounds.exps.shape[2], bounds.exps.device
+    _lib.require(dev.type == "cuda" and 0 <= layer < bounds.exps.shape[0], "bounds on a CUDA device, layer inside them")
+    Tq, Hq, n = _check_step(q, None, dev, Hkv, block_tables, q_start, ctx_lens, max_q_len)
+    _lib.require(sink_pages >= 0 and recent_pages >= 1 and sink_pages + recent_pages <= num_pages, "sink_pages + recent_pages (at least 1) <= num_pages")
+    pages = torch.empty((Tq, Hkv, num_pages), dtype=torch.int32, device=dev)
+    stride = max(1, -(-max_ctx // KV4_TOKENS))
+    scores = None
+    if stride > num_pages:
+        need = Tq * Hkv * stride
+        scores = workspace.ensure_scores(need) if workspace is not None else torch.empty(need, dtype=torch.float32, device=dev)
+        _lib.require(scores.device == dev, "the workspace is on another device")
+    _lib.call_on(dev, _lib.kv4_fn("daser_select_pages_kv4"), "select_pages_kv4", q.data_ptr(), bounds.codes.data_ptr(),
+                 bounds.exps.data_ptr(), layer, bounds.exps.shape[1], block_tables.data_ptr(), block_tables.shape[1], q_start.data_ptr(),
+                 ctx_lens.data_ptr(), n, Tq, max_q_len, Hq, Hkv, scores.data_ptr() if scores is not None else pages.data_ptr(), stride,
+                 pages.data_ptr(), num_pages, sink_pages, recent_pages)
+    if stride > num_pages:
+        _lib.launch_count += 1  # the score kernel
+    return pages
+
+
+def sparse_paged_attention(
+    q: torch.Tensor,
+    out: torch.Tensor,
+    pool: PagedKV4Pool,
+    layer: int,
+    block_tables: torch.Tensor,
+    q_start: torch.Tensor,
+    ctx_lens: torch.Tensor,
+    pages: torch.Tensor,
+    max_q_len: int,
+    softmax_scale: float,
+    workspace: Optional[AttentionWorkspace] = None,
+    rank: int = 0,
+) -> torch.Tensor:
+    """:func:`paged_attention` over the pages of ``pages`` (int32 ``[Tq, Hkv, n]``, as :func:`select_pages` gives them): row ``t``
+    of a sequence attends the keys of its listed pages up to ``ctx_len - q_len + t``.  Every query row reads its own list: a
+    decode operator, for one or a few query tokens per sequence.  Pages have to be distinct within a list (one listed
+    twice counts twice); entries outside the context are skipped."""
+    _lib.require(isinstance(pool, PagedKV4Pool), "sparse attention works on a PagedKV4Pool")
+    _lib.require(pages.dim() == 3 and pages.shape[2] >= 1 and tuple(pages.shape[:2]) == (q.shape[0], pool.heads_per_rank),
+                 "pages: int32 [rows, KV heads, pages]")
+    _lib.check_tensor(pages, "pages", torch.int32, pool.device)
+    return _attention_kv4(q, out, pool, layer, block_tables, q_start, ctx_lens, max_q_len, 0, softmax_scale, workspace, rank, pages,
+                          None, None)

@@ -8,7 +8,7 @@ from typing import Optional, Sequence
 import torch
 
 from daser_b200.ops import _lib
-from daser_b200.ops.kv_ops import PagedKVPool
+from daser_b200.ops.kv_ops import KV4_DIM, KV4_TOKENS, PagedKV4Pool, PagedKVPool
 
 
 class TpSync(C.Structure):
@@ -132,7 +132,7 @@ def rope_kv_write(
     num_kv_heads: int,
     head_dim: int,
     block_tokens: int,
-    pool: PagedKVPool,
+    pool: PagedKVPool | PagedKV4Pool,
     layer: int,
     rank: int = 0,
     zero_after: bool = False,
@@ -141,7 +141,13 @@ def rope_kv_write(
     """RoPE on q and k of ``qkv[T, (Hq + 2 Hkv) * D]``; q -> ``q_out``, k/v -> the paged pool.
 
     ``qk_norm = (q_weight[D], k_weight[D], eps)``: RMSNorm over head_dim on every query and key
-    head before the rotation (Qwen3 family)."""
+    head before the rotation (Qwen3 family).
+
+    Into a :class:`~daser_b200.ops.kv_ops.PagedKV4Pool` keys and values are quantised to 4 bits as they are written."""
+    if isinstance(pool, PagedKV4Pool):
+        _rope_kv4_write(qkv, positions, slot_mapping, cos_sin, q_out, num_q_heads, num_kv_heads, head_dim, block_tokens, pool, layer,
+                        rank, zero_after, qk_norm)
+        return
     assert positions.dtype == torch.int32 and slot_mapping.dtype == torch.int64
     pool_c = pool.c_struct()
     if qk_norm is not None:
@@ -169,6 +175,34 @@ def rope_kv_write(
         ),
         "rope_kv_write",
     )
+
+
+def _rope_kv4_write(qkv, positions, slot_mapping, cos_sin, q_out, hq, hkv, head_dim, block_tokens, pool, layer, rank, zero_after,
+                    qk_norm) -> None:
+    need, dev = _lib.require, pool.device
+    pool.check(layer, rank)
+    need(head_dim == KV4_DIM and block_tokens == KV4_TOKENS, "a 4-bit pool has head_dim 128 and 16 tokens per block")
+    need(hkv == pool.heads_per_rank, f"the pool keeps {pool.heads_per_rank} KV heads, not {hkv}")
+    need(qkv.dim() == 2 and qkv.device == dev and qkv.dtype in (torch.float32, torch.bfloat16), "qkv: float32 or bfloat16 [T, heads * 128] on the pool's device")
+    T = qkv.shape[0]
+    need(qkv.shape[1] >= (hq + 2 * hkv) * head_dim and qkv.stride(1) == 1, "qkv: too few columns, or columns with a stride")
+    _lib.check_tensor(positions, "positions", torch.int32, dev)
+    _lib.check_tensor(slot_mapping, "slot_mapping", torch.int64, dev)
+    _lib.check_tensor(cos_sin, "cos_sin", torch.float32, dev)
+    _lib.check_tensor(q_out, "q_out", torch.bfloat16, dev)
+    need(positions.numel() >= T and slot_mapping.numel() >= T, "positions, slot_mapping: one entry per token")
+    need(cos_sin.dim() == 2 and cos_sin.shape[1] == head_dim and q_out.numel() >= T * hq * head_dim, "cos_sin [positions, 128], q_out [T, heads, 128]")
+    qw = kw = None
+    eps = 0.0
+    if qk_norm is not None:
+        qw, kw, eps = qk_norm
+        for w, name in ((qw, "q weight"), (kw, "k weight")):
+            _lib.check_tensor(w, name, torch.bfloat16, dev)
+            need(w.numel() == head_dim, f"{name}: one value per dim")
+        qw, kw = qw.data_ptr(), kw.data_ptr()
+    _lib.call_on(dev, _lib.kv4_fn("daser_rope_kv4_write"), "rope_kv4_write", qkv.data_ptr(), int(qkv.dtype == torch.float32),
+                 qkv.stride(0), positions.data_ptr(), slot_mapping.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], q_out.data_ptr(), T,
+                 hq, hkv, pool.c_ptr, layer, rank, int(zero_after), qw, kw, eps)
 
 
 def swiglu(x: torch.Tensor, out: Optional[torch.Tensor] = None, zero_after: bool = False,

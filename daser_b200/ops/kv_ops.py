@@ -1,4 +1,4 @@
-"""Python entry points of the KV kernels: codec, fused restore, fused save.
+"""Python entry points of the KV kernels: codecs, fused restore, fused save, read-back, key bounds of pages.
 
 ``PagedKVPool`` describes a paged pool (one per tensor-parallel rank) with explicit
 strides, so the kernels never assume an attention backend's layout; the reference
@@ -121,6 +121,150 @@ class PagedKVPool:
         )
 
 
+def quantize_fp4b16(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """bf16 CUDA tensor ``[..., D]`` -> (uint8 codes ``[..., D/2]``, uint8 scales ``[..., D/16]``); the format is
+    described in :mod:`daser_b200.kv.codec`."""
+    _lib.require(x.is_cuda and x.shape[-1] % 16 == 0, "quantize_fp4b16: needs a CUDA tensor whose last dimension is a multiple of 16")
+    _lib.check_tensor(x, "x", torch.bfloat16, x.device)
+    codes = torch.empty((*x.shape[:-1], x.shape[-1] // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((*x.shape[:-1], x.shape[-1] // 16), dtype=torch.uint8, device=x.device)
+    _lib.call_on(x.device, _lib.kv4_fn("daser_quant_fp4b16"), "quant_fp4b16", x.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+                 x.numel())
+    return codes, scales
+
+
+def dequantize_fp4b16(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """The values that :func:`quantize_fp4b16`'s result stands for, in bf16 (exact)."""
+    _lib.require(codes.is_cuda and tuple(scales.shape) == (*codes.shape[:-1], codes.shape[-1] // 8) and codes.shape[-1] % 8 == 0,
+                 "dequantize_fp4b16: codes [..., D/2] and scales [..., D/16] on a CUDA device")
+    _lib.check_tensor(codes, "codes", torch.uint8, codes.device)
+    _lib.check_tensor(scales, "scales", torch.uint8, codes.device)
+    out = torch.empty((*codes.shape[:-1], codes.shape[-1] * 2), dtype=torch.bfloat16, device=codes.device)
+    _lib.call_on(codes.device, _lib.kv4_fn("daser_dequant_fp4b16"), "dequant_fp4b16", codes.data_ptr(), scales.data_ptr(),
+                 out.data_ptr(), out.numel())
+    return out
+
+
+KV4_RECORD = 2304  # bytes of one page (16 tokens) of one KV head: ``ops/csrc/kv4.h``
+KV4_TOKENS, KV4_DIM = 16, 128
+
+
+class PagedKV4Pool:
+    """A paged pool in the 4-bit format: one 2304-byte record per (layer, block, KV head), 0.5625 bytes per element
+    (:class:`PagedKVPool` holds 1.25 in fp8 and 2 in bf16).
+
+    It takes the place of a :class:`PagedKVPool` in ``rope_kv_write``, :func:`kv_restore`, :func:`kv_save` and
+    ``paged_attention``, and is what :func:`kv_read`, :func:`update_page_bounds` and
+    ``sparse_paged_attention`` work on.  16 tokens per block, head_dim 128.  ``record_ptrs[r]`` is rank ``r``'s base
+    address as mapped into this process; the pool's kernels run on ``device``.
+
+    Slots written by one call have to be distinct: of two tokens with the same slot, one wins group by group.
+    """
+
+    def __init__(self, record_ptrs: Sequence[int], stride_layer: int, stride_block: int, stride_head: int, num_layers: int,
+                 num_blocks: int, heads_per_rank: int, device: torch.device, keepalive: Optional[list] = None) -> None:
+        _lib.require(1 <= len(record_ptrs) <= _lib.MAX_RANKS, f"1 to {_lib.MAX_RANKS} ranks")
+        _lib.require(all(int(p) % 16 == 0 for p in record_ptrs) and all(x % 16 == 0 for x in (stride_layer, stride_block, stride_head)),
+                     "records have to start on 16-byte boundaries")
+        _lib.require(min(num_layers, num_blocks, heads_per_rank) > 0, "a 4-bit pool needs layers, blocks and heads")
+        self.record_ptrs = [int(p) for p in record_ptrs]
+        self.stride_layer, self.stride_block, self.stride_head = stride_layer, stride_block, stride_head
+        self.num_layers, self.num_blocks, self.heads_per_rank = num_layers, num_blocks, heads_per_rank
+        self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.keepalive = keepalive
+        c = _lib.KV4Pool()
+        for r, ptr in enumerate(self.record_ptrs):
+            c.records[r] = ptr
+        c.stride_layer, c.stride_block, c.stride_head = stride_layer, stride_block, stride_head
+        c.num_layers, c.num_blocks, c.n_ranks, c.heads_per_rank = num_layers, num_blocks, len(self.record_ptrs), heads_per_rank
+        self._c = c
+        self.c_ptr = C.addressof(c)  # entry points copy the block before they return
+
+    @property
+    def n_ranks(self) -> int:
+        return len(self.record_ptrs)
+
+    @classmethod
+    def from_tensors(cls, records: Sequence[torch.Tensor]) -> "PagedKV4Pool":
+        """From one uint8 tensor ``[layers, blocks, heads, 2304]`` per rank; records are contiguous, the other
+        strides are free (multiples of 16)."""
+        t = records[0]
+        for r in records:
+            _lib.require(r.dtype == torch.uint8 and r.dim() == 4 and r.shape[3] == KV4_RECORD and r.stride(3) == 1,
+                         "records: uint8 [layers, blocks, heads, 2304] with contiguous records")
+            _lib.require(r.shape == t.shape and r.stride() == t.stride(), "every rank's records need the same shape and strides")
+        return cls([r.data_ptr() for r in records], t.stride(0), t.stride(1), t.stride(2), t.shape[0], t.shape[1], t.shape[2],
+                   t.device, [list(records)])
+
+    @classmethod
+    def zeros(cls, num_layers: int, num_blocks: int, num_heads: int, device) -> "PagedKV4Pool":
+        return cls.from_tensors([torch.zeros(num_layers, num_blocks, num_heads, KV4_RECORD, dtype=torch.uint8, device=device)])
+
+    def check(self, layer: int, rank: int) -> None:
+        _lib.require(self.device.type == "cuda", "the pool's kernels need a CUDA device")
+        _lib.require(0 <= layer < self.num_layers and 0 <= rank < self.n_ranks, f"layer {layer} or rank {rank} outside the pool")
+
+
+def kv_read(pool: PagedKV4Pool, layer: int, slot_mapping: torch.Tensor, rank: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values bf16 ``[T, heads, 128]`` of the tokens at ``slot_mapping`` (int64 ``[T]``, block * 16 + offset,
+    as ``rope_kv_write`` takes it), as the pool holds them; a negative slot reads as zeros."""
+    pool.check(layer, rank)
+    _lib.check_tensor(slot_mapping, "slot_mapping", torch.int64, pool.device)
+    T = slot_mapping.numel()
+    k = torch.empty((T, pool.heads_per_rank, KV4_DIM), dtype=torch.bfloat16, device=pool.device)
+    v = torch.empty_like(k)
+    _lib.call_on(pool.device, _lib.kv4_fn("daser_kv4_read"), "kv4_read", pool.c_ptr, layer, rank, slot_mapping.data_ptr(),
+                 k.data_ptr(), v.data_ptr(), T)
+    return k, v
+
+
+class PageBounds:
+    """Bounds of the keys of every page of a 4-bit pool: what ``select_pages`` scores.
+
+    ``codes`` int8 ``[layers, blocks, heads, 2, 128]`` (high, low) and ``exps`` int8 ``[layers, blocks, heads]``: the keys of a
+    page lie between ``codes[..., 1, :] * 2^exp`` and ``codes[..., 0, :] * 2^exp``, 257 bytes per page and head.
+    """
+
+    def __init__(self, codes: torch.Tensor, exps: torch.Tensor) -> None:
+        _lib.require(codes.dim() == 5 and tuple(codes.shape[3:]) == (2, KV4_DIM) and tuple(exps.shape) == tuple(codes.shape[:3]),
+                     "codes [layers, blocks, heads, 2, 128], exps [layers, blocks, heads]")
+        _lib.check_tensor(codes, "codes", torch.int8, codes.device)
+        _lib.check_tensor(exps, "exps", torch.int8, codes.device)
+        _lib.require(codes.data_ptr() % 16 == 0, "codes have to start on a 16-byte boundary")
+        self.codes, self.exps = codes, exps
+
+    @classmethod
+    def for_pool(cls, pool: PagedKV4Pool) -> "PageBounds":
+        shape = (pool.num_layers, pool.num_blocks, pool.heads_per_rank)
+        return cls(torch.zeros(*shape, 2, KV4_DIM, dtype=torch.int8, device=pool.device),
+                   torch.zeros(shape, dtype=torch.int8, device=pool.device))
+
+    def read(self, layer: int, blocks: torch.Tensor) -> torch.Tensor:
+        """The bounds of ``blocks`` as float32 ``[n, heads, 2, 128]`` (high, low)."""
+        at = blocks.long()
+        return torch.ldexp(self.codes[layer, at].float(), self.exps[layer, at].int()[..., None, None])
+
+
+def update_page_bounds(pool: PagedKV4Pool, bounds: PageBounds, layer: int, block_tables: torch.Tensor, q_start: torch.Tensor,
+                       ctx_lens: torch.Tensor, max_q_len: int, rank: int = 0) -> None:
+    """Recompute the bounds of every page that holds one of a sequence's last ``q_start[s+1] - q_start[s]`` tokens (the step's
+    new ones; after a restore, the restored ones).  Arguments as ``paged_attention`` takes them; call it behind the step's
+    ``rope_kv_write``."""
+    pool.check(layer, rank)
+    _lib.require(tuple(bounds.exps.shape) == (pool.num_layers, pool.num_blocks, pool.heads_per_rank) and bounds.exps.device == pool.device,
+                 "the bounds belong to a pool of another shape or device")
+    n = ctx_lens.numel()
+    _lib.check_tensor(block_tables, "block_tables", torch.int32, pool.device)
+    _lib.check_tensor(q_start, "q_start", torch.int32, pool.device)
+    _lib.check_tensor(ctx_lens, "ctx_lens", torch.int32, pool.device)
+    _lib.require(block_tables.dim() == 2 and block_tables.shape[0] >= n and q_start.numel() >= n + 1, "one table row and one q_start per sequence")
+    _lib.call_on(pool.device, _lib.kv4_fn("daser_kv4_page_bounds"), "kv4_page_bounds", pool.c_ptr, layer, rank, bounds.codes.data_ptr(),
+                 bounds.exps.data_ptr(), block_tables.data_ptr(), block_tables.shape[1], q_start.data_ptr(), ctx_lens.data_ptr(), n,
+                 max_q_len)
+
+
 @dataclass
 class KVWorkList:
     """Device-side work list of one restore/save launch."""
@@ -150,24 +294,37 @@ def _job(work, geo, image_is_fp8, cos_sin, status, rank=0) -> KVJob:
     return j
 
 
-def kv_restore(work: KVWorkList, geo, pool: PagedKVPool, cos_sin: Optional[torch.Tensor],
+def kv_restore(work: KVWorkList, geo, pool: PagedKVPool | PagedKV4Pool, cos_sin: Optional[torch.Tensor],
                status: Optional[torch.Tensor] = None, stream=None, layer_begin: int = 0,
                layer_count: int = 0) -> None:
     """Slot images -> paged pools of every rank: dequantise, rotate keys by ``deltas``, scatter.
 
     ``layer_begin`` / ``layer_count`` restrict the launch to a range of layers (0 = through the
     last one): a restore can then run group by group while the storage reads of later layers
-    are still in flight and the model already computes on the earlier ones."""
+    are still in flight and the model already computes on the earlier ones.
+
+    Into a :class:`PagedKV4Pool` the (rotated) values are quantised to 4 bits on the way."""
     job = _job(work, geo, geo.codec == "fp8b16", cos_sin, status)
     job.layer_begin, job.layer_count = int(layer_begin), int(layer_count)
+    if isinstance(pool, PagedKV4Pool):
+        pool.check(0, 0)
+        _lib.call_on(pool.device, _lib.kv4_fn("daser_kv4_restore"), "kv4_restore", C.addressof(job), pool.c_ptr, stream=stream)
+        return
     pool_c = pool.c_struct()
     _lib.check(_lib.lib().daser_kv_restore(C.byref(job), C.byref(pool_c), _lib.stream_ptr(stream)), "kv_restore")
 
 
-def kv_save(work: KVWorkList, geo, pool: PagedKVPool, rank: int = 0,
+def kv_save(work: KVWorkList, geo, pool: PagedKVPool | PagedKV4Pool, rank: int = 0,
             status: Optional[torch.Tensor] = None, stream=None) -> None:
-    """Rank ``rank``'s blocks -> its head slice of each slot image (compressing for fp8b16)."""
+    """Rank ``rank``'s blocks -> its head slice of each slot image (compressing for fp8b16).
+
+    Out of a :class:`PagedKV4Pool` a raw image gets the 4-bit values as they stand (exact in bf16), an fp8b16 image the
+    same values quantised once more."""
     job = _job(work, geo, geo.codec == "fp8b16", None, status, rank)
+    if isinstance(pool, PagedKV4Pool):
+        pool.check(0, rank)
+        _lib.call_on(pool.device, _lib.kv4_fn("daser_kv4_save"), "kv4_save", C.addressof(job), pool.c_ptr, stream=stream)
+        return
     pool_c = pool.c_struct()
     _lib.check(_lib.lib().daser_kv_save(C.byref(job), C.byref(pool_c), _lib.stream_ptr(stream)), "kv_save")
 
