@@ -168,6 +168,7 @@ _KV4_ARGS = {
     "daser_kv4_restore": [_P, _P, _P],
     "daser_kv4_save": [_P, _P, _P],
     "daser_kv4_page_bounds": [_P, _I, _I, _P, _P, _P, _I, _P, _P, _I, _I, _P],
+    "daser_kv4_bounds_read": [_P, _P, _I, _I, _I, _P, _P, _I, _P],
     "daser_quant_fp4b16": [_P, _P, _P, _L, _P],
     "daser_dequant_fp4b16": [_P, _P, _P, _L, _P],
     "daser_paged_attention_kv4": [_P, _P, _P, _P, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P],
@@ -194,22 +195,31 @@ def require(cond: bool, what: str) -> None:
 
 
 def check_tensor(t, name: str, dtype, device) -> None:
-    """``t`` is a contiguous tensor of ``dtype`` on the CUDA device ``device``."""
-    if t.dtype != dtype or t.device != device or not t.is_contiguous():
+    """``t`` is a contiguous tensor of ``dtype`` on ``device`` (a CUDA device with its index, or the CPU)."""
+    if t.dtype != dtype or t.get_device() != (-1 if device.index is None else device.index) or not t.is_contiguous():
         raise ValueError(f"{name}: needs a contiguous {dtype} tensor on {device}, got {t.dtype} on {t.device}, strides {tuple(t.stride())}")
+
+
+_torch_c = None
 
 
 def call_on(device, fn, what: str, *args, stream=None) -> None:
     """``fn(*args, stream)`` with ``device`` current: its current stream unless one is given."""
-    import torch
+    global _torch_c
+    if _torch_c is None:
+        import torch
 
-    if device.index is not None and device.index != torch.cuda.current_device():
+        torch.cuda.init()
+        _torch_c = torch._C
+    # the raw accessors: torch.cuda.current_stream() builds an object and costs as much as a launch
+    index = device.index
+    if index != _torch_c._cuda_getDevice():
+        import torch
+
         with torch.cuda.device(device):
-            s = stream if stream is not None else torch.cuda.current_stream()
-            check(fn(*args, s.cuda_stream), what)
+            check(fn(*args, stream.cuda_stream if stream is not None else _torch_c._cuda_getCurrentRawStream(index)), what)
         return
-    s = stream if stream is not None else torch.cuda.current_stream()
-    check(fn(*args, s.cuda_stream), what)
+    check(fn(*args, stream.cuda_stream if stream is not None else _torch_c._cuda_getCurrentRawStream(index)), what)
 
 
 def stream_ptr(stream=None) -> C.c_void_p:

@@ -93,39 +93,6 @@ attn4_kernel(const Attn4Params p) {
   const int page_end = min(page_begin + p.split_pages, n_all);
   const int mine = page_end - page_begin > warp ? (page_end - page_begin - warp + A4_WARPS - 1) / A4_WARPS : 0;  // pages of this warp
 
-  // ---- queries: B fragments, scaled, f16.  Column g of n-tile nt is row row0 + 8 nt + g ----
-  uint32_t qf[NT][16];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = row0 + 8 * nt + g;
-    const bool ok = r < n_rows;
-    const int tq = SPARSE ? tok0 : r / G, h = SPARSE ? r : r % G;
-    const __nv_bfloat16* qp = p.q + ((int64_t)(q0 + tq) * p.Hq + kvh * G + h) * ATT_D + 32 * t;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint4 w = make_uint4(0u, 0u, 0u, 0u);
-      if (ok) w = *reinterpret_cast<const uint4*>(qp + 8 * i);
-      const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) qf[nt][4 * i + e] = pack_half2(bf16_lo(ww[e]) * p.scale_log2, bf16_hi(ww[e]) * p.scale_log2);
-    }
-  }
-  // last visible key of this lane's columns 2t, 2t + 1 of every n-tile
-  int pos[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) pos[nt][e] = SPARSE ? first_pos : first_pos + (row0 + 8 * nt + 2 * t + e) / G - tok0;
-
-  float o[NT][8][4], m[NT][2], l[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    m[nt][0] = m[nt][1] = -INFINITY;
-    l[nt][0] = l[nt][1] = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
-  }
-
   // ---- page fetch ----
   // Logical pages of the next 32 fetches sit one per lane (page_of), read a window ahead of their use.
   uint8_t* ring = a4_smem + warp * A4_RING;
@@ -163,6 +130,39 @@ attn4_kernel(const Attn4Params p) {
   };
   int fetched = 0;
   for (; fetched < A4_STAGES - 1 && fetched < mine; ++fetched) fetch(fetched);
+
+  // ---- queries: B fragments, scaled, f16.  Column g of n-tile nt is row row0 + 8 nt + g ----
+  uint32_t qf[NT][16];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = row0 + 8 * nt + g;
+    const bool ok = r < n_rows;
+    const int tq = SPARSE ? tok0 : r / G, h = SPARSE ? r : r % G;
+    const __nv_bfloat16* qp = p.q + ((int64_t)(q0 + tq) * p.Hq + kvh * G + h) * ATT_D + 32 * t;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint4 w = make_uint4(0u, 0u, 0u, 0u);
+      if (ok) w = *reinterpret_cast<const uint4*>(qp + 8 * i);
+      const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) qf[nt][4 * i + e] = pack_half2(bf16_lo(ww[e]) * p.scale_log2, bf16_hi(ww[e]) * p.scale_log2);
+    }
+  }
+  // last visible key of this lane's columns 2t, 2t + 1 of every n-tile
+  int pos[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) pos[nt][e] = SPARSE ? first_pos : first_pos + (row0 + 8 * nt + 2 * t + e) / G - tok0;
+
+  float o[NT][8][4], m[NT][2], l[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    m[nt][0] = m[nt][1] = -INFINITY;
+    l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
+  }
 
   int used = 0;
   bool fail = false;
@@ -359,45 +359,62 @@ attn4_kernel(const Attn4Params p) {
   }
 }
 
-// out = sum_s w_s O_s / sum_s w_s, w_s = 2^(lse_s - max): one CTA per output row, its warps take the splits in turn, so that a few
-// rows with many splits (one long sequence) are not a serial loop of one warp.  The order of the sums is fixed.
-__global__ void __launch_bounds__(128)
+// out = sum_s w_s O_s / sum_s w_s, w_s = 2^(lse_s - max): one CTA per output row.  The weights are made once, then its warps
+// take the splits in turn, eight loads in flight each: a few rows with many splits (one long sequence on one KV head) are
+// a matter of latency.  The order of the sums is fixed.
+constexpr int MERGE_WARPS = 8;
+constexpr int MERGE_MAX_SPLITS = 256;
+__global__ void __launch_bounds__(MERGE_WARPS * 32)
 attn4_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_lse, __nv_bfloat16* __restrict__ out,
                    const int32_t* __restrict__ q_start, int num_seqs, int Hq, int nsplit) {
-  __shared__ float s_w[4];
-  __shared__ __align__(16) float s_o[4][ATT_D];
+  __shared__ float s_w[MERGE_MAX_SPLITS];
+  __shared__ float s_max[MERGE_WARPS], s_sum[MERGE_WARPS];
+  __shared__ __align__(16) float s_o[MERGE_WARPS][ATT_D];
   const int64_t row = blockIdx.x;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_enter();
   if (row >= (int64_t)q_start[num_seqs] * Hq) return;  // a row behind the last sequence: nobody wrote its partials
-  const float* lse = part_lse + row * nsplit;
-  float mx = -INFINITY;
-  bool nan = false;
-  for (int s = lane; s < nsplit; s += 32) {
-    const float v = lse[s];
-    nan |= v != v;
-    mx = fmaxf(mx, v);
-  }
-  mx = warp_max(mx);
-  nan = __any_sync(0xffffffffu, nan);
-  const float base = mx == -INFINITY ? 0.f : mx;
+  const float lse = tid < nsplit ? part_lse[row * nsplit + tid] : -INFINITY;
+  const float* src = part_o + row * nsplit * ATT_D + 4 * lane;
+  // NaN marks a row that saw one: it has to survive the maximum
+  const bool nan = lse != lse;
+  const float wm = warp_max(nan ? INFINITY : lse);
+  if (lane == 0) s_max[warp] = wm;
+  __syncthreads();
+  float mx = s_max[0];
+#pragma unroll
+  for (int w = 1; w < MERGE_WARPS; ++w) mx = fmaxf(mx, s_max[w]);
+  const float wt = nan ? NAN : (lse == -INFINITY ? 0.f : ex2f(lse - mx));
+  s_w[tid] = wt;
+  const float ws = warp_sum(wt);
+  if (lane == 0) s_sum[warp] = ws;
+  __syncthreads();
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float wsum = 0.f;
-  for (int s = warp; s < nsplit; s += 4) {
-    const float v = lse[s];
-    if (v == -INFINITY) continue;
-    const float w = ex2f(v - base);
-    const float4 x = *reinterpret_cast<const float4*>(part_o + (row * nsplit + s) * ATT_D + 4 * lane);
-    acc.x += w * x.x; acc.y += w * x.y; acc.z += w * x.z; acc.w += w * x.w;
-    wsum += w;
+  for (int s0 = warp; s0 < nsplit; s0 += 8 * MERGE_WARPS) {
+    float4 x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int s = s0 + u * MERGE_WARPS;
+      x[u] = s < nsplit ? *reinterpret_cast<const float4*>(src + (int64_t)s * ATT_D) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int s = s0 + u * MERGE_WARPS;
+      const float w = s < nsplit ? s_w[s] : 0.f;
+      acc.x += w * x[u].x; acc.y += w * x[u].y; acc.z += w * x[u].z; acc.w += w * x[u].w;
+    }
   }
-  if (lane == 0) s_w[warp] = wsum;
   *reinterpret_cast<float4*>(&s_o[warp][4 * lane]) = acc;
   __syncthreads();
-  const float total = s_w[0] + s_w[1] + s_w[2] + s_w[3];
-  const float v = s_o[0][threadIdx.x] + s_o[1][threadIdx.x] + s_o[2][threadIdx.x] + s_o[3][threadIdx.x];
-  const float r = nan ? NAN : (total > 0.f ? v / total : 0.f);
-  out[row * ATT_D + threadIdx.x] = __float2bfloat16(r);
+  if (tid < ATT_D) {
+    float total = 0.f, v = 0.f;
+#pragma unroll
+    for (int w = 0; w < MERGE_WARPS; ++w) {
+      total += s_sum[w];
+      v += s_o[w][tid];
+    }
+    out[row * ATT_D + tid] = __float2bfloat16(total == 0.f ? 0.f : v / total);  // no key: zeros
+  }
 }
 
 template <int NT, bool SPARSE>
@@ -421,6 +438,7 @@ static int fill_attn4(Attn4Params& p, const void* q, void* out, float* part_o, f
   const int Hkv = pool->heads_per_rank;
   if (Hq <= 0 || Hq % Hkv || num_seqs < 0 || total_q < 0 || max_q_len < 0 || max_blocks <= 0) return DASER_ERR_BAD_ARG;
   if (nsplit < 1 || split_pages < 1 || (nsplit > 1 && (!part_o || !part_lse))) return DASER_ERR_BAD_ARG;
+  if (nsplit > MERGE_MAX_SPLITS) return DASER_ERR_TOO_LARGE;
   if (max_blocks > 0x7fffffff / DASER_KV4_TOKENS || total_q > 0x7fffffff / Hq) return DASER_ERR_TOO_LARGE;
   if (Hq / Hkv > 16) return DASER_ERR_UNSUPPORTED;
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)part_o) % 16) return DASER_ERR_UNSUPPORTED;
@@ -451,7 +469,7 @@ static int fill_attn4(Attn4Params& p, const void* q, void* out, float* part_o, f
 
 static int merge_attn4(const Attn4Params& p, cudaStream_t stream) {
   if (p.nsplit == 1) return 0;
-  return (int)launch_pdl(attn4_merge_kernel, dim3((unsigned)(p.total_q * p.Hq)), dim3(128), 0, stream, (const float*)p.part_o,
+  return (int)launch_pdl(attn4_merge_kernel, dim3((unsigned)(p.total_q * p.Hq)), dim3(MERGE_WARPS * 32), 0, stream, (const float*)p.part_o,
                          (const float*)p.part_lse, p.out, p.q_start, p.num_seqs, p.Hq, p.nsplit);
 }
 

@@ -12,9 +12,10 @@
 
 namespace daser {
 
-constexpr int SCORE_PAGES = 256;    // pages per CTA of the score kernel
-constexpr int SELECT_THREADS = 512;
+constexpr int SCORE_PAGES = 128;    // pages per CTA of the score kernel: 8 per half-warp
+constexpr int SELECT_THREADS = 1024;
 constexpr int SELECT_BINS = 2048;
+static_assert(SELECT_THREADS == 32 * 32, "one warp can hold a value of every warp");
 constexpr int SELECT_SMEM_KEYS = 40960;  // longer lists are read from global memory in every pass
 
 struct Select4Params {
@@ -58,56 +59,68 @@ attn4_score_kernel(const Select4Params p) {
   const int hi_page = min(count - p.recent, ((int)blockIdx.x + 1) * SCORE_PAGES);
   if (count <= p.n_pages || lo_page >= hi_page) return;  // everything is chosen, or nothing here needs a score
 
+  // Sixteen lanes a page, 16 bytes a lane, eight pages a half-warp.  All loads are issued before the query is prepared: the block
+  // id is a dependent load in front of them, and nothing else hides either.
+  const int lane = threadIdx.x & 31, sub = lane & 15;
+  const int page0 = blockIdx.x * SCORE_PAGES + (threadIdx.x >> 4) * 8;
+  const int my_page = page0 + (sub >> 1);  // whose score this lane ends up with
+  int blk = p.block_tables[(int64_t)seq * p.max_blocks + min(my_page, count - 1)];
+  blk = blk < 0 ? 0 : (blk >= p.num_blocks ? p.num_blocks - 1 : blk);
+  int4 c[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int b = __shfl_sync(0xffffffffu, blk, (lane & 16) + 2 * i);
+    c[i] = *reinterpret_cast<const int4*>(p.codes + ((int64_t)b * p.Hkv + kvh) * (2 * ATT_D) + 16 * sub);
+  }
+  const int e = p.exps[(int64_t)blk * p.Hkv + kvh];
+
   double up = 0.0, down = 0.0;  // sums of at most 16 bf16 values: exact
   if (threadIdx.x < ATT_D) {
     const __nv_bfloat16* qp = p.q + ((int64_t)row * p.Hq + kvh * p.G) * ATT_D + threadIdx.x;
-    for (int h = 0; h < p.G; ++h) {
-      const float x = __bfloat162float(qp[h * ATT_D]);
-      up += (double)fmaxf(x, 0.f);
-      down += (double)fminf(x, 0.f);
+    float x[16];
+#pragma unroll
+    for (int h = 0; h < 16; ++h) x[h] = h < p.G ? __bfloat162float(qp[h * ATT_D]) : 0.f;
+#pragma unroll
+    for (int h = 0; h < 16; ++h) {
+      if (h >= p.G) break;
+      up += (double)fmaxf(x[h], 0.f);
+      down += (double)fminf(x[h], 0.f);
     }
     const double mx = warp_max_f64(fmax(up, -down));
-    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = mx;
+    if (lane == 0) s_max[threadIdx.x >> 5] = mx;
   }
   __syncthreads();
   if (threadIdx.x < ATT_D) {
     const double a = fmax(fmax(s_max[0], s_max[1]), fmax(s_max[2], s_max[3]));
-    double f = 1.0;  // 2^-e, e the smallest with a <= 127 * 2^e
+    double f = 1.0;  // 2^-x, x the smallest with a <= 127 * 2^x
     if (a > 0.0) {
       const uint64_t b = (uint64_t)__double_as_longlong(a);
-      const int e = (int)(b >> 52) - 1022 - 7 + ((b & 0xfffffffffffffull) > (63ull << 46) ? 1 : 0);
-      f = __longlong_as_double((long long)(uint64_t)(1023 - e) << 52);
+      const int x = (int)(b >> 52) - 1022 - 7 + ((b & 0xfffffffffffffull) > (63ull << 46) ? 1 : 0);
+      f = __longlong_as_double((long long)(uint64_t)(1023 - x) << 52);
     }
     s_q[threadIdx.x] = (int8_t)__double2int_rn(up * f);
     s_q[ATT_D + threadIdx.x] = (int8_t)__double2int_rn(down * f);
   }
   __syncthreads();
-  // sixteen lanes a page, 16 bytes a lane
-  const int sub = threadIdx.x & 15, hw = threadIdx.x >> 4;
   const int4 qv = *reinterpret_cast<const int4*>(s_q + 16 * sub);
-  const int32_t* table = p.block_tables + (int64_t)seq * p.max_blocks;
-  float* dst = p.scores + ((int64_t)row * p.Hkv + kvh) * p.stride;
-#pragma unroll 4
-  for (int i = 0; i < SCORE_PAGES / 16; ++i) {
-    const int page = blockIdx.x * SCORE_PAGES + 16 * i + hw;
-    const bool in = page >= lo_page && page < hi_page;
-    int dot = 0, e = 0;
-    if (in) {
-      int blk = table[page];
-      blk = blk < 0 ? 0 : (blk >= p.num_blocks ? p.num_blocks - 1 : blk);
-      const int64_t at = (int64_t)blk * p.Hkv + kvh;
-      const int4 c = *reinterpret_cast<const int4*>(p.codes + at * 256 + 16 * sub);
-      e = p.exps[at];
-      dot = __dp4a(c.x, qv.x, dot);
-      dot = __dp4a(c.y, qv.y, dot);
-      dot = __dp4a(c.z, qv.z, dot);
-      dot = __dp4a(c.w, qv.w, dot);
-    }
+  int dot[8];
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    // exponent 127: a key of the page is not finite; such a page is always read
-    if (in && sub == 0) dst[page] = e == 127 ? INFINITY : (float)dot * __uint_as_float((uint32_t)(max(e, -126) + 127) << 23);
+  for (int i = 0; i < 8; ++i) dot[i] = __dp4a(c[i].x, qv.x, __dp4a(c[i].y, qv.y, __dp4a(c[i].z, qv.z, __dp4a(c[i].w, qv.w, 0))));
+  // sum over the sixteen lanes and transpose: a lane keeps half of its pages at each step, in the end page sub / 2
+#pragma unroll
+  for (int n = 4, o = 8; n > 0; n >>= 1, o >>= 1) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const bool high = (sub & o) != 0;
+      const int keep = high ? dot[n + i] : dot[i], give = high ? dot[i] : dot[n + i];
+      dot[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
   }
+  dot[0] += __shfl_xor_sync(0xffffffffu, dot[0], 1);
+  // exponent 127: a key of the page is not finite; such a page is always read
+  if ((sub & 1) == 0 && my_page >= lo_page && my_page < hi_page)
+    p.scores[((int64_t)row * p.Hkv + kvh) * p.stride + my_page] =
+        e == 127 ? INFINITY : (float)dot[0] * __uint_as_float((uint32_t)(max(e, -126) + 127) << 23);
 }
 
 // Floats in the order of unsigned integers.
@@ -128,8 +141,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* s_warp) {
   __syncthreads();
   if (lane == 31) s_warp[warp] = x;
   __syncthreads();
-  uint32_t before = 0;
-  for (int w = 0; w < warp; ++w) before += s_warp[w];
+  const uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? s_warp[lane] : 0u);
   return before + x - v;
 }
 
@@ -167,8 +179,9 @@ attn4_select_kernel(const Select4Params p) {
   hi = __reduce_max_sync(0xffffffffu, hi);
   if ((tid & 31) == 0) { s_lo[tid >> 5] = lo; s_hi[tid >> 5] = hi; }
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < SELECT_THREADS / 32; ++w) { lo = min(lo, s_lo[w]); hi = max(hi, s_hi[w]); }
+  lo = __reduce_min_sync(0xffffffffu, s_lo[tid & 31]);
+  hi = __reduce_max_sync(0xffffffffu, s_hi[tid & 31]);
+  __syncthreads();  // s_lo and s_hi are used again below
   auto key = [&](int i) { return cached ? s_keys[i] : ordered(src[i]); };
 
   // The need-th largest key, by digits of up to 11 bits from the first bit in which the keys differ.
@@ -187,7 +200,7 @@ attn4_select_kernel(const Select4Params p) {
       if (shift >= 32 || (k >> shift) == prefix) atomicAdd(&s_bins[(k >> at) & mask], 1u);
     }
     __syncthreads();
-    // bins from the top: thread t has bins [top - 4t - 3, top - 4t]
+    // bins from the top: two a thread
     constexpr int PER = SELECT_BINS / SELECT_THREADS;
     uint32_t c[PER], sum = 0;
 #pragma unroll
@@ -218,23 +231,30 @@ attn4_select_kernel(const Select4Params p) {
   // (prefix is not zero then: some key is not chosen)
   const uint32_t thr = whole ? (prefix << shift) - 1u : prefix;
   const int eq_need = whole ? 0 : need;
-  const int per = (n + SELECT_THREADS - 1) / SELECT_THREADS;
-  const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
+  // In ascending order: a warp owns a run of keys and takes 32 at a time (contiguous in shared memory), ballots count them.
+  const int lane = tid & 31, warp = tid >> 5;
+  const uint32_t below = (1u << lane) - 1u;
+  const int run = ((n + SELECT_THREADS - 1) / SELECT_THREADS) * 32;
+  const int i0 = min(warp * run, n), i1 = min(i0 + run, n);
   uint32_t gt = 0, eq = 0;
-  for (int i = i0; i < i1; ++i) {
-    const uint32_t k = key(i);
-    gt += k > thr;
-    eq += k == thr;
+  for (int i = i0; i < i1; i += 32) {
+    const bool in = i + lane < i1;
+    const uint32_t k = in ? key(i + lane) : 0u;
+    gt += __popc(__ballot_sync(0xffffffffu, in && k > thr));
+    eq += __popc(__ballot_sync(0xffffffffu, in && k == thr));
   }
-  const uint32_t gt0 = block_scan(gt, s_warp);
-  const uint32_t eq0 = block_scan(eq, s_warp);
-  int g = (int)gt0, e = (int)eq0;
-  for (int i = i0; i < i1; ++i) {
-    const uint32_t k = key(i);
-    const bool is_eq = k == thr;
-    if (k > thr || (is_eq && e < eq_need)) list[p.sink + g + min(e, eq_need)] = p.sink + i;
-    g += k > thr;
-    e += is_eq;
+  if (lane == 0) { s_lo[warp] = gt; s_hi[warp] = eq; }
+  __syncthreads();
+  int g = 0, e = 0;
+  for (int w = 0; w < warp; ++w) { g += (int)s_lo[w]; e += (int)s_hi[w]; }
+  for (int i = i0; i < i1; i += 32) {
+    const bool in = i + lane < i1;
+    const uint32_t k = in ? key(i + lane) : 0u;
+    const uint32_t mg = __ballot_sync(0xffffffffu, in && k > thr), me = __ballot_sync(0xffffffffu, in && k == thr);
+    const int my_e = e + __popc(me & below);
+    if (in && (k > thr || (k == thr && my_e < eq_need))) list[p.sink + g + __popc(mg & below) + min(my_e, eq_need)] = p.sink + i + lane;
+    g += __popc(mg);
+    e += __popc(me);
   }
 }
 

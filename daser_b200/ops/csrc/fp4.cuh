@@ -47,40 +47,77 @@ __device__ __forceinline__ uint32_t floats_to_e2m1x8(const float* x) {
   return w;
 }
 
-// The largest magnitude as bits: integer order is float order, and puts infinities and NaNs on top.
+// Two floats a register pair: one instruction for both, each rounded as the scalar one would be.
+__device__ __forceinline__ uint64_t pair2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// (a, b) rotated: a' = a c - b s, b' = b c + a s, every product and sum rounded (the CPU oracle's bits).  The sums are scalar: a packed
+// sum of packed products comes out of the compiler as one fused operation.
+__device__ __forceinline__ void rotate2(uint64_t& a, uint64_t& b, uint64_t c, uint64_t s) {
+  float ac0, ac1, bs0, bs1, bc0, bc1, as0, as1;
+  unpair2(mul2(a, c), ac0, ac1);
+  unpair2(mul2(b, s), bs0, bs1);
+  unpair2(mul2(b, c), bc0, bc1);
+  unpair2(mul2(a, s), as0, as1);
+  a = pair2(__fsub_rn(ac0, bs0), __fsub_rn(ac1, bs1));
+  b = pair2(__fadd_rn(bc0, as0), __fadd_rn(bc1, as1));
+}
+
+// The largest magnitude, NaN if there is one.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 template <int N>
-__device__ __forceinline__ uint32_t fp4_absmax_bits(const float (&x)[N]) {
-  uint32_t m = 0;
+__device__ __forceinline__ float fp4_absmax(const uint64_t (&x)[N]) {
+  float m = 0.f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+  for (int i = 0; i < N; ++i) {
+    float a, b;
+    unpair2(x[i], a, b);
+    m = max3_nan(m, fabsf(a), fabsf(b));
+  }
   return m;
 }
 
-__device__ __forceinline__ uint32_t fp4_scale_byte(uint32_t absmax_bits) {
-  if (absmax_bits >= 0x7f800000u) return 255u;
-  const float t = fminf(__fmul_rn(__uint_as_float(absmax_bits), 1.0f / 6.0f), 10240.f);
+__device__ __forceinline__ uint32_t fp4_scale_byte(float absmax) {
+  if (!(absmax < INFINITY)) return 255u;
+  const float t = fminf(__fmul_rn(absmax, 1.0f / 6.0f), 10240.f);
   const uint32_t b = __half_as_ushort(__float2half_rn(t));
   return (b + 63u + ((b >> 7) & 1u)) >> 7;
 }
 
-// x / s, correctly rounded, as two fused corrections of x * (1 / s): with inv the correctly rounded
-// reciprocal and q within one unit of the quotient, q + r * inv rounds correctly (P. Markstein, "Computation of elementary functions
-// on the IBM RISC System/6000 processor", 1990).  x * inv alone is not enough: 3.5 * 1.875 / 1.875 would come out
-// above the border between 3 and 4.
-__device__ __forceinline__ float fp4_quotient(float x, float s, float inv) {
-  const float q = __fmul_rn(x, inv);
-  return __fmaf_rn(__fmaf_rn(-q, s, x), inv, q);
-}
-
+// Pairs of values -> codes.  The quotient x / s is correctly rounded, as two fused corrections of x * (1 / s): with inv the
+// correctly rounded reciprocal and q within one unit of the quotient, q + (x - q s) * inv rounds correctly (P. Markstein,
+// "Computation of elementary functions on the IBM RISC System/6000 processor", 1990).  x * inv alone is not enough:
+// 3.5 * 1.875 / 1.875 would come out above the border between 3 and 4.
 template <int N>
-__device__ __forceinline__ void fp4_encode(const float (&x)[N], uint32_t scale_byte, uint32_t (&codes)[N / 8]) {
+__device__ __forceinline__ void fp4_encode(const uint64_t (&x)[N], uint32_t scale_byte, uint32_t (&codes)[N / 4]) {
   const float s = fp4_scale(scale_byte);
   const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
-  float y[N];
+  const uint64_t inv2 = pair2(inv, inv), ns2 = pair2(-s, -s);
+  float y[2 * N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) y[i] = fp4_quotient(x[i], s, inv);
+  for (int i = 0; i < N; ++i) {
+    const uint64_t q = mul2(x[i], inv2);
+    unpair2(fma2(fma2(q, ns2, x[i]), inv2, q), y[2 * i], y[2 * i + 1]);
+  }
 #pragma unroll
-  for (int i = 0; i < N / 8; ++i) codes[i] = floats_to_e2m1x8(y + 8 * i);
+  for (int i = 0; i < N / 4; ++i) codes[i] = floats_to_e2m1x8(y + 8 * i);
 }
 
 // 8 codes and their scale byte -> floats (exact).

@@ -16,30 +16,36 @@ __device__ __forceinline__ void kv4_report(uint32_t* status, uint32_t code, uint
 }
 
 template <typename T>
-__device__ __forceinline__ void load8(T* p, float (&x)[8], bool zero);
+__device__ __forceinline__ void load8(T* p, uint64_t (&x)[4], bool zero);
 template <>
-__device__ __forceinline__ void load8<float>(float* p, float (&x)[8], bool zero) {
-  float4* v = reinterpret_cast<float4*>(p);
-  const float4 a = v[0], b = v[1];
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  if (zero) v[0] = v[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+__device__ __forceinline__ void load8<float>(float* p, uint64_t (&x)[4], bool zero) {
+  ulonglong2* v = reinterpret_cast<ulonglong2*>(p);
+  const ulonglong2 a = v[0], b = v[1];
+  x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+  if (zero) v[0] = v[1] = make_ulonglong2(0ull, 0ull);
 }
 template <>
-__device__ __forceinline__ void load8<__nv_bfloat16>(__nv_bfloat16* p, float (&x)[8], bool zero) {
+__device__ __forceinline__ void load8<__nv_bfloat16>(__nv_bfloat16* p, uint64_t (&x)[4], bool zero) {
   const uint4 a = *reinterpret_cast<const uint4*>(p);
   const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) { x[2 * i] = bf16_lo(w[i]); x[2 * i + 1] = bf16_hi(w[i]); }
+  for (int i = 0; i < 4; ++i) x[i] = pair2(bf16_lo(w[i]), bf16_hi(w[i]));
   if (zero) *reinterpret_cast<uint4*>(p) = make_uint4(0u, 0u, 0u, 0u);
 }
 __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
 }
-__device__ __forceinline__ void load_f8(const float* p, float (&x)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+__device__ __forceinline__ uint32_t bf16_pair(uint64_t v) {
+  float a, b;
+  unpair2(v, a, b);
+  return pack_bf16x2(a, b);
+}
+__device__ __forceinline__ uint4 pack8(const uint64_t (&x)[4]) {
+  return make_uint4(bf16_pair(x[0]), bf16_pair(x[1]), bf16_pair(x[2]), bf16_pair(x[3]));
+}
+__device__ __forceinline__ void load_pairs4(const float* p, uint64_t (&x)[4]) {
+  const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(p), b = *reinterpret_cast<const ulonglong2*>(p + 4);
+  x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
 }
 
 // ---- RoPE + cache write of a step -----------------------------------------------------------------------------
@@ -67,9 +73,9 @@ kv4_write_kernel(TIn* __restrict__ qkv, int64_t qkv_stride, const int32_t* __res
   const int64_t block = slot / DASER_KV4_TOKENS;
   const int tok = (int)(slot % DASER_KV4_TOKENS);
   const bool live = slot >= 0 && block < num_blocks;
-  float cs[8], sn[8];
-  load_f8(cos_sin + (int64_t)pos * D + 8 * c, cs);
-  load_f8(cos_sin + (int64_t)pos * D + 64 + 8 * c, sn);
+  uint64_t cs[4], sn[4];
+  load_pairs4(cos_sin + (int64_t)pos * D + 8 * c, cs);
+  load_pairs4(cos_sin + (int64_t)pos * D + 64 + 8 * c, sn);
   TIn* row = qkv + (int64_t)t * qkv_stride;
   // every lane of a warp runs the same trips (the shuffles below are warp-wide): heads beyond the last are clamped
   for (int h0 = blockIdx.y * 16; h0 < heads; h0 += gridDim.y * 16) {
@@ -77,33 +83,37 @@ kv4_write_kernel(TIn* __restrict__ qkv, int64_t qkv_stride, const int32_t* __res
     const bool in = hd_raw < heads;
     const int hd = in ? hd_raw : heads - 1;
     const bool is_q = hd < Hq, is_v = hd >= Hq + Hkv;
-    float a[8], b[8];
+    uint64_t a[4], b[4];
     load8<TIn>(row + (int64_t)hd * D + 8 * c, a, in && zero_after != 0);
     load8<TIn>(row + (int64_t)hd * D + 64 + 8 * c, b, in && zero_after != 0);
     if (QKNORM) {
       float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
+      for (int i = 0; i < 4; ++i) {
+        float x0, x1, y0, y1;
+        unpair2(a[i], x0, x1);
+        unpair2(b[i], y0, y1);
+        ss += x0 * x0 + y0 * y0 + (x1 * x1 + y1 * y1);
+      }
 #pragma unroll
       for (int m = 4; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
       if (!is_v) {
         const float inv = rsqrtf(ss / (float)D + norm_eps);
         const __nv_bfloat16* w = (is_q ? q_norm_w : k_norm_w) + 8 * c;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
           // the normalised head is a bf16 tensor in the models this follows: round before rotating
-          a[i] = __bfloat162float(__float2bfloat16(a[i] * inv * __bfloat162float(w[i])));
-          b[i] = __bfloat162float(__float2bfloat16(b[i] * inv * __bfloat162float(w[64 + i])));
+          const uint64_t wa = pair2(__bfloat162float(w[2 * i]), __bfloat162float(w[2 * i + 1]));
+          const uint64_t wb = pair2(__bfloat162float(w[64 + 2 * i]), __bfloat162float(w[64 + 2 * i + 1]));
+          const uint32_t ra = bf16_pair(mul2(mul2(a[i], pair2(inv, inv)), wa)), rb = bf16_pair(mul2(mul2(b[i], pair2(inv, inv)), wb));
+          a[i] = pair2(bf16_lo(ra), bf16_hi(ra));
+          b[i] = pair2(bf16_lo(rb), bf16_hi(rb));
         }
       }
     }
     if (!is_v) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x = a[i], y = b[i];
-        a[i] = __fsub_rn(__fmul_rn(x, cs[i]), __fmul_rn(y, sn[i]));
-        b[i] = __fadd_rn(__fmul_rn(y, cs[i]), __fmul_rn(x, sn[i]));
-      }
+      for (int i = 0; i < 4; ++i) rotate2(a[i], b[i], cs[i], sn[i]);
     }
     if (in && is_q) {
       __nv_bfloat16* dst = q_out + ((int64_t)t * Hq + hd) * D + 8 * c;
@@ -112,17 +122,18 @@ kv4_write_kernel(TIn* __restrict__ qkv, int64_t qkv_stride, const int32_t* __res
     }
     if (h0 + 16 > Hq) {  // some lane of the block holds a key or value head: uniform over the block
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        a[i] = __bfloat162float(__float2bfloat16(a[i]));
-        b[i] = __bfloat162float(__float2bfloat16(b[i]));
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t ra = bf16_pair(a[i]), rb = bf16_pair(b[i]);
+        a[i] = pair2(bf16_lo(ra), bf16_hi(ra));
+        b[i] = pair2(bf16_lo(rb), bf16_hi(rb));
       }
-      uint32_t ma = fp4_absmax_bits<8>(a), mb = fp4_absmax_bits<8>(b);
-      ma = max(ma, __shfl_xor_sync(0xffffffffu, ma, 1));
-      mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
+      float ma = fp4_absmax<4>(a), mb = fp4_absmax<4>(b);
+      ma = max3_nan(ma, __shfl_xor_sync(0xffffffffu, ma, 1), 0.f);
+      mb = max3_nan(mb, __shfl_xor_sync(0xffffffffu, mb, 1), 0.f);
       const uint32_t sa = fp4_scale_byte(ma), sb = fp4_scale_byte(mb);
       uint32_t ca[1], cb[1];
-      fp4_encode<8>(a, sa, ca);
-      fp4_encode<8>(b, sb, cb);
+      fp4_encode<4>(a, sa, ca);
+      fp4_encode<4>(b, sb, cb);
       if (in && !is_q && live) {
         const int kv = is_v ? 1 : 0;
         uint8_t* rec = pool + block * stride_block + (int64_t)(hd - Hq - kv * Hkv) * stride_head;
@@ -171,6 +182,23 @@ kv4_read_kernel(const uint8_t* __restrict__ pool, int64_t stride_block, int64_t 
 // then leave as 16-byte stores.  Stored directly, the 8-byte pieces of V would each be a quarter of a 32-byte sector.
 constexpr int KV4_HEADS = 8;
 
+__device__ __forceinline__ void load_fp8_group(const uint8_t* p, float scale, uint64_t (&x)[8]) {
+  const uint4 q = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  const uint64_t s = pair2(scale, scale);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 f = e4m3x2_to_float2((uint16_t)(w[i >> 1] >> (16 * (i & 1))));
+    x[i] = mul2(pair2(f.x, f.y), s);
+  }
+}
+__device__ __forceinline__ void load_bf16_group(const __nv_bfloat16* p, uint64_t (&x)[8]) {
+  const uint4 a = *reinterpret_cast<const uint4*>(p), b = *reinterpret_cast<const uint4*>(p + 8);
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = pair2(bf16_lo(w[i]), bf16_hi(w[i]));
+}
+
 template <bool IMG_FP8>
 __global__ void __launch_bounds__(256)
 kv4_restore_kernel(const DaserKVJob job, const DaserKV4Pool pool) {
@@ -203,35 +231,37 @@ kv4_restore_kernel(const DaserKVJob job, const DaserKV4Pool pool) {
   const uint8_t* base = reinterpret_cast<const uint8_t*>(img) + (int64_t)layer * layer_bytes;
   const float* img_scales = reinterpret_cast<const float*>(base + elems);
   const int items = 2 * B * nh * 4;
+  const int lg = (nh & (nh - 1)) == 0 ? __ffs(nh) - 1 : -1;
   for (int item = threadIdx.x; item < items; item += 256) {
     const int j = item & 3;
     const int r = item >> 2;
-    const int hl = r % nh;
-    const int tok = (r / nh) % B, kv = r / (nh * B);
-    const int64_t e1 = (((int64_t)kv * B + tok) * H + head0 + hl) * D + j * FP8_GROUP, e2 = e1 + D / 2;
-    float x1[16], x2[16];
+    const int rr = lg >= 0 ? r >> lg : r / nh;  // kv * B + token
+    const int hl = r - rr * nh;
+    const int tok = rr & (B - 1), kv = rr / B;
+    const int64_t e1 = ((int64_t)rr * H + head0 + hl) * D + j * FP8_GROUP, e2 = e1 + D / 2;
+    uint64_t x1[8], x2[8];
     if (IMG_FP8) {
-      dequant_group16(*reinterpret_cast<const uint4*>(base + e1), img_scales[e1 / FP8_GROUP], x1);
-      dequant_group16(*reinterpret_cast<const uint4*>(base + e2), img_scales[e2 / FP8_GROUP], x2);
+      load_fp8_group(base + e1, img_scales[e1 / FP8_GROUP], x1);
+      load_fp8_group(base + e2, img_scales[e2 / FP8_GROUP], x2);
     } else {
-      load_bf16x16(reinterpret_cast<const __nv_bfloat16*>(base) + e1, x1);
-      load_bf16x16(reinterpret_cast<const __nv_bfloat16*>(base) + e2, x2);
+      load_bf16_group(reinterpret_cast<const __nv_bfloat16*>(base) + e1, x1);
+      load_bf16_group(reinterpret_cast<const __nv_bfloat16*>(base) + e2, x2);
     }
     if (kv == 0 && delta != 0) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float c = s_cs[j * FP8_GROUP + i], s = s_cs[D / 2 + j * FP8_GROUP + i];
-        const float a = x1[i], b = x2[i];
-        x1[i] = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
-        x2[i] = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
+      for (int i = 0; i < 4; ++i) {
+        const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(&s_cs[j * FP8_GROUP + 4 * i]);
+        const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(&s_cs[D / 2 + j * FP8_GROUP + 4 * i]);
+        rotate2(x1[2 * i], x2[2 * i], c.x, s.x);
+        rotate2(x1[2 * i + 1], x2[2 * i + 1], c.y, s.y);
       }
     }
     uint8_t* rec = s_rec + hl * DASER_KV4_RECORD;
     uint32_t codes[2];
-    const uint32_t s1 = fp4_scale_byte(fp4_absmax_bits<16>(x1)), s2 = fp4_scale_byte(fp4_absmax_bits<16>(x2));
-    fp4_encode<16>(x1, s1, codes);
+    const uint32_t s1 = fp4_scale_byte(fp4_absmax<8>(x1)), s2 = fp4_scale_byte(fp4_absmax<8>(x2));
+    fp4_encode<8>(x1, s1, codes);
     *reinterpret_cast<uint2*>(rec + kv4_code_at(kv, tok, 2 * j)) = make_uint2(codes[0], codes[1]);
-    fp4_encode<16>(x2, s2, codes);
+    fp4_encode<8>(x2, s2, codes);
     *reinterpret_cast<uint2*>(rec + kv4_code_at(kv, tok, 8 + 2 * j)) = make_uint2(codes[0], codes[1]);
     rec[kv4_scale_at(kv, tok, j)] = (uint8_t)s1;
     rec[kv4_scale_at(kv, tok, 4 + j)] = (uint8_t)s2;
@@ -294,13 +324,15 @@ kv4_save_kernel(const DaserKVJob job, const DaserKV4Pool pool) {
   uint8_t* base = reinterpret_cast<uint8_t*>(img) + (int64_t)layer * layer_bytes;
   float* img_scales = reinterpret_cast<float*>(base + elems);
   constexpr int PIECES = IMG_FP8 ? 8 : 16;  // of a row: a scale group, or 16 bytes of bf16
+  const int lg = (nh & (nh - 1)) == 0 ? __ffs(nh) - 1 : -1;
   for (int item = threadIdx.x; item < 2 * B * nh * PIECES; item += 256) {
     const int p = item % PIECES;
     const int r = item / PIECES;
-    const int hl = r % nh;
-    const int tok = (r / nh) % B, kv = r / (nh * B);
+    const int rr = lg >= 0 ? r >> lg : r / nh;  // kv * B + token
+    const int hl = r - rr * nh;
+    const int tok = rr & (B - 1), kv = rr / B;
     const uint8_t* rec = s_rec + hl * DASER_KV4_RECORD;
-    const int64_t row = ((int64_t)kv * B + tok) * H + first + l0 + hl;
+    const int64_t row = (int64_t)rr * H + first + l0 + hl;
     if (IMG_FP8) {
       float x[16];
       const uint2 w = *reinterpret_cast<const uint2*>(rec + kv4_code_at(kv, tok, 2 * p));
@@ -391,15 +423,36 @@ kv4_page_bounds_kernel(const uint8_t* __restrict__ pool, int64_t stride_block, i
   if (lane == 0) exps[at] = (int8_t)e;
 }
 
+// The bounds of listed blocks as floats [n][H][2][128]; a block outside the pool reads as zeros.
+__global__ void __launch_bounds__(256)
+kv4_bounds_read_kernel(const int8_t* __restrict__ codes, const int8_t* __restrict__ exps, const int32_t* __restrict__ blocks,
+                       float* __restrict__ out, int64_t items, int num_blocks, int H) {
+  pdl_enter();
+  for (int64_t it = blockIdx.x * (int64_t)256 + threadIdx.x; it < items; it += (int64_t)gridDim.x * 256) {
+    const int64_t nh = it >> 6;  // 64 pieces of four values a head
+    const int64_t n = nh / H;
+    const int blk = blocks[n];
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (blk >= 0 && blk < num_blocks) {
+      const int64_t at = (int64_t)blk * H + (nh - n * H);
+      const char4 c = *reinterpret_cast<const char4*>(codes + at * 256 + (it & 63) * 4);
+      const int e = exps[at];
+      const float f = e == 127 ? INFINITY : pow2f(max(e, -126));
+      v = make_float4(c.x * f, c.y * f, c.z * f, c.w * f);
+    }
+    *reinterpret_cast<float4*>(out + it * 4) = v;
+  }
+}
+
 // ---- the codec on its own ----------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(256)
 quant_fp4b16_kernel(const __nv_bfloat16* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t groups) {
   for (int64_t g = blockIdx.x * (int64_t)256 + threadIdx.x; g < groups; g += (int64_t)gridDim.x * 256) {
-    float v[16];
-    load_bf16x16(x + g * 16, v);
-    const uint32_t s = fp4_scale_byte(fp4_absmax_bits<16>(v));
+    uint64_t v[8];
+    load_bf16_group(x + g * 16, v);
+    const uint32_t s = fp4_scale_byte(fp4_absmax<8>(v));
     uint32_t c[2];
-    fp4_encode<16>(v, s, c);
+    fp4_encode<8>(v, s, c);
     *reinterpret_cast<uint2*>(codes + g * 8) = make_uint2(c[0], c[1]);
     scales[g] = (uint8_t)s;
   }
@@ -523,6 +576,19 @@ DASER_API int daser_kv4_page_bounds(const DaserKV4Pool* pool, int layer, int ran
                          (const uint8_t*)pool->records[rank] + (int64_t)layer * pool->stride_layer, pool->stride_block,
                          pool->stride_head, pool->num_blocks, codes + rows * 256, exps + rows, block_tables, max_blocks, q_start,
                          ctx_lens, (int)H);
+}
+
+// Bounds of `n` listed blocks as floats [n][heads][2][128].
+DASER_API int daser_kv4_bounds_read(const int8_t* codes, const int8_t* exps, int layer, int num_blocks, int heads, const int32_t* blocks,
+                                    float* out, int n, cudaStream_t stream) {
+  using namespace daser;
+  if (layer < 0 || num_blocks <= 0 || heads <= 0 || n < 0) return DASER_ERR_BAD_ARG;
+  if (n == 0) return 0;
+  if (!codes || !exps || !blocks || !out) return DASER_ERR_BAD_ARG;
+  if ((uintptr_t)codes % 4 || (uintptr_t)out % 16) return DASER_ERR_UNSUPPORTED;
+  const int64_t rows = (int64_t)layer * num_blocks * heads, items = (int64_t)n * heads * 64, grid = (items + 255) / 256;
+  return (int)launch_pdl(kv4_bounds_read_kernel, dim3((unsigned)(grid < 148 * 8 ? grid : 148 * 8)), dim3(256), 0, stream, codes + rows * 256,
+                         exps + rows, blocks, out, items, num_blocks, heads);
 }
 
 DASER_API int daser_quant_fp4b16(const void* x, void* codes, void* scales, int64_t n_elems, cudaStream_t stream) {

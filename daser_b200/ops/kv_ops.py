@@ -242,9 +242,15 @@ class PageBounds:
                    torch.zeros(shape, dtype=torch.int8, device=pool.device))
 
     def read(self, layer: int, blocks: torch.Tensor) -> torch.Tensor:
-        """The bounds of ``blocks`` as float32 ``[n, heads, 2, 128]`` (high, low)."""
-        at = blocks.long()
-        return torch.ldexp(self.codes[layer, at].float(), self.exps[layer, at].int()[..., None, None])
+        """The bounds of ``blocks`` (int32, any shape) as float32 ``[..., heads, 2, 128]`` (high, low); of a page with a key that is not
+        finite, infinities."""
+        dev = self.exps.device
+        _lib.require(dev.type == "cuda" and 0 <= layer < self.exps.shape[0], "bounds on a CUDA device, layer inside them")
+        _lib.check_tensor(blocks, "blocks", torch.int32, dev)
+        out = torch.empty((*blocks.shape, self.exps.shape[2], 2, KV4_DIM), dtype=torch.float32, device=dev)
+        _lib.call_on(dev, _lib.kv4_fn("daser_kv4_bounds_read"), "kv4_bounds_read", self.codes.data_ptr(), self.exps.data_ptr(), layer,
+                     self.exps.shape[1], self.exps.shape[2], blocks.data_ptr(), out.data_ptr(), blocks.numel())
+        return out
 
 
 def update_page_bounds(pool: PagedKV4Pool, bounds: PageBounds, layer: int, block_tables: torch.Tensor, q_start: torch.Tensor,

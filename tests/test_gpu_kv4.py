@@ -478,10 +478,27 @@ def test_page_bounds_are_exact_and_only_of_the_pages_touched(ctx, q_lens):
             else:
                 assert (codes[1, blk, h] == 55).all() and exps[1, blk, h] == 33
     assert (codes[0] == 55).all()
-    read = bounds.read(1, torch.tensor(sorted(touched), device="cuda")).cpu().double()
+    read = bounds.read(1, torch.tensor(sorted(touched), dtype=torch.int32, device="cuda")).cpu().double()
     for i, blk in enumerate(sorted(touched)):
         kk = k[blk, :, : touched[blk]].double()
         assert (read[i, :, 0] >= kk.max(1).values).all() and (read[i, :, 1] <= kk.min(1).values).all()
+        assert torch.equal(read[i], codes[1, blk].double() * torch.exp2(exps[1, blk].double())[:, None, None])
+
+
+def test_page_bounds_of_a_key_that_is_not_finite():
+    """Such a page has infinite bounds, so that it is always among the selected ones; one behind the context does not count."""
+    _, _, kv_ops = _ops()
+    rec = _records(3, 1, 13)
+    rec[0, 1, 0, 2048 + 8 * 5 + 3] = 0xFF  # token 5
+    rec[0, 2, 0, 2048 + 8 * 5 + 3] = 0xFF
+    pool = kv_ops.PagedKV4Pool.from_tensors([rec.cuda()])
+    bounds = kv_ops.PageBounds.for_pool(pool)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    kv_ops.update_page_bounds(pool, bounds, 0, torch.tensor([[0, 1, 2]], **i32), torch.tensor([0, 36], **i32), torch.tensor([36], **i32), 36)
+    read = bounds.read(0, torch.tensor([[0, 1], [2, 3]], **i32))
+    assert read.shape == (2, 2, 1, 2, 128) and torch.isfinite(read[0, 0]).all() and torch.isfinite(read[1, 0]).all()
+    assert (read[0, 1, 0, 0] == float("inf")).all() and (read[0, 1, 0, 1] == -float("inf")).all()
+    assert (read[1, 1] == 0).all()  # a block outside the pool
 
 
 def _select_oracle(q, codes, exps, tables, q_lens, ctx_lens, n_pages, sink, recent):
