@@ -172,7 +172,7 @@ _KV4_ARGS = {
     "daser_quant_fp4b16": [_P, _P, _P, _L, _P],
     "daser_dequant_fp4b16": [_P, _P, _P, _L, _P],
     "daser_paged_attention_kv4": [_P, _P, _P, _P, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P],
-    "daser_sparse_attention_kv4": [_P, _P, _P, _P, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _P, _I, _I, _I, _F, _P],
+    "daser_sparse_attention_kv4": [_P, _P, _P, _P, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _P, _I, _I, _F, _P],
     "daser_select_pages_kv4": [_P, _P, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _P, _I, _P, _I, _I, _I, _P],
 }
 _kv4_fns: dict = {}
@@ -194,32 +194,35 @@ def require(cond: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def check_tensor(t, name: str, dtype, device) -> None:
-    """``t`` is a contiguous tensor of ``dtype`` on ``device`` (a CUDA device with its index, or the CPU)."""
-    if t.dtype != dtype or t.get_device() != (-1 if device.index is None else device.index) or not t.is_contiguous():
-        raise ValueError(f"{name}: needs a contiguous {dtype} tensor on {device}, got {t.dtype} on {t.device}, strides {tuple(t.stride())}")
+def check_tensor(t, name: str, dtype, index: int) -> None:
+    """``t`` is a contiguous tensor of ``dtype`` on CUDA device ``index`` (-1: the CPU)."""
+    if t.dtype != dtype or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name}: needs a contiguous {dtype} tensor on CUDA device {index}, got {t.dtype} on {t.device}, strides {tuple(t.stride())}")
 
 
 _torch_c = None
 
 
-def call_on(device, fn, what: str, *args, stream=None) -> None:
-    """``fn(*args, stream)`` with ``device`` current: its current stream unless one is given."""
-    global _torch_c
+def call_on(index: int, fn, what: str, *args, stream=None) -> None:
+    """``fn(*args, stream)`` with CUDA device ``index`` current: its current stream unless one is given."""
+    global _torch_c, launch_count
     if _torch_c is None:
         import torch
 
         torch.cuda.init()
         _torch_c = torch._C
     # the raw accessors: torch.cuda.current_stream() builds an object and costs as much as a launch
-    index = device.index
-    if index != _torch_c._cuda_getDevice():
+    if index == _torch_c._cuda_getDevice():
+        code = fn(*args, stream.cuda_stream if stream is not None else _torch_c._cuda_getCurrentRawStream(index))
+    else:
         import torch
 
-        with torch.cuda.device(device):
-            check(fn(*args, stream.cuda_stream if stream is not None else _torch_c._cuda_getCurrentRawStream(index)), what)
-        return
-    check(fn(*args, stream.cuda_stream if stream is not None else _torch_c._cuda_getCurrentRawStream(index)), what)
+        with torch.cuda.device(index):
+            code = fn(*args, stream.cuda_stream if stream is not None else _torch_c._cuda_getCurrentRawStream(index))
+    if code == 0:
+        launch_count += 1
+    else:
+        check(code, what)
 
 
 def stream_ptr(stream=None) -> C.c_void_p:

@@ -5,13 +5,14 @@
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 from typing import Optional
 
 import torch
 
 from daser_b200.ops import _lib
-from daser_b200.ops.kv_ops import KV4_DIM, KV4_TOKENS, PageBounds, PagedKV4Pool, PagedKVPool
+from daser_b200.ops.kv_ops import KV4_DIM, KV4_TOKENS, PageBounds, PagedKV4Pool, PagedKVPool, check_sequences
 
 NUM_SMS = 148
 MAX_ROW_SPLITS = 262144  # (query rows x KV splits) the split-KV scratch is sized for (135 MB)
@@ -82,27 +83,28 @@ def kv4_status() -> int:
     return bits
 
 
-def plan_splits_kv4(num_seqs: int, kv_heads: int, max_q_len: int, group: int, max_pages: int, rows: int = 0) -> tuple[int, int]:
-    """(nsplit, pages per split) of attention over the 4-bit pool (``max_pages``: of the longest context, or of a page list)."""
+@functools.lru_cache(maxsize=4096)
+def plan_kv4(num_seqs: int, kv_heads: int, max_q_len: int, group: int, max_pages: int, rows: int = 0) -> tuple[int, int]:
+    """(parts, pages per split) of attention over the 4-bit pool; ``max_pages``: of the longest context, or of a page list.
+
+    From 64 query rows per KV head on (the tcgen05 kernel) parts are splits per context.  Below, they are the CTAs that share all
+    pages evenly, 0 for one CTA per (sequence, row tile, KV head) and no merge."""
     max_pages = max(1, max_pages)
     if max_q_len * group >= TC_MIN_ROWS:
-        # tcgen05 kernel: a CTA of 128 query rows, two per SM, tiles of four pages; splits of two tiles at the shortest
+        # a CTA of 128 query rows, two per SM, tiles of four pages; splits of two tiles at the shortest
         items = num_seqs * kv_heads * -(-max_q_len // (128 // group))
         nsplit = max(1, min((NUM_SMS * 2) // max(items, 1), -(-max_pages // 8), 64))
         if rows > 0:
             nsplit = max(1, min(nsplit, MAX_ROW_SPLITS // rows))
         per = -(--(-max_pages // nsplit) // 4) * 4
         return -(-max_pages // per), per
-    tiles = 1 if max_q_len * group <= 8 else -(-max_q_len * group // 16)
-    items = max(1, num_seqs * kv_heads * tiles)
-    slots = NUM_SMS * (4 if max_q_len * group <= 8 else 3)  # resident CTAs
-    # one wave of CTAs when the batch is small, 128 pages (2048 keys) a CTA when it is large, never less than four pages a warp
-    nsplit = max(slots // items, -(-max_pages // 128), 1)
-    nsplit = max(1, min(nsplit, max_pages // 16, 256))
-    if rows > 0:
-        nsplit = max(1, min(nsplit, MAX_ROW_SPLITS // rows))
-    per = -(-max_pages // nsplit)
-    return -(-max_pages // per), per
+    # up to 12 pages a warp, one CTA per item takes less than the merge kernel that sharing needs
+    if max_pages <= 96:
+        return 0, 0
+    # two CTAs a SM (one with two column tiles), and four pages a warp at least
+    resident = NUM_SMS * (2 if max_q_len * group <= 8 else 1)
+    pages = max(1, num_seqs) * kv_heads * -(-max_q_len * group // (8 if max_q_len * group <= 8 else 16)) * max_pages
+    return max(2, min(resident, pages // 32)), 0
 
 
 class AttentionWorkspace:
@@ -157,13 +159,13 @@ def paged_attention(
 
     Over a :class:`~daser_b200.ops.kv_ops.PagedKV4Pool` any group of up to 16 query heads per KV head is taken,
     ``max_ctx`` has to be at least the longest context, and ``workspace`` may be ``None`` (scratch of the call's own).
+    ``nsplit`` then is the first value of :func:`plan_kv4`.
     """
     if isinstance(pool, PagedKV4Pool):
         _lib.require(block_tokens == KV4_TOKENS and num_kv_heads == pool.heads_per_rank, "block_tokens or num_kv_heads are not the pool's")
-        _lib.require((nsplit is None) == (split_tokens is None) and (split_tokens is None or split_tokens % KV4_TOKENS == 0),
-                     "nsplit and split_tokens (a multiple of 16) go together")
+        _lib.require(split_tokens is None, "a 4-bit pool takes nsplit alone")
         return _attention_kv4(q, out, pool, layer, block_tables, q_start, ctx_lens, max_q_len, max_ctx, softmax_scale, workspace, rank,
-                              None, nsplit, split_tokens // KV4_TOKENS if split_tokens is not None else None)
+                              None, nsplit)
     Tq, Hq, D = q.shape
     num_seqs = ctx_lens.numel()
     assert block_tables.dtype == torch.int32 and q_start.dtype == torch.int32 and ctx_lens.dtype == torch.int32
@@ -189,54 +191,62 @@ def paged_attention(
     return out
 
 
-def _check_step(q, out, pool_device, kv_heads, block_tables, q_start, ctx_lens, max_q_len) -> tuple[int, int, int]:
+def _check_step(q, out, index, kv_heads, block_tables, q_start, ctx_lens, max_q_len) -> tuple[int, int, int]:
     """The arguments every 4-bit attention call shares; (query rows, query heads, sequences)."""
-    need = _lib.require
-    need(q.dim() == 3 and q.shape[2] == KV4_DIM, "q: [rows, heads, 128]")
+    bf16 = torch.bfloat16
+    if not (q.dtype is bf16 and q.get_device() == index and q.is_contiguous()):
+        _lib.check_tensor(q, "q", bf16, index)
+    if q.dim() != 3 or q.shape[2] != KV4_DIM:
+        raise ValueError("q: [rows, heads, 128]")
     Tq, Hq, _ = q.shape
-    need(Hq > 0 and Hq % kv_heads == 0 and Hq // kv_heads <= 16, "1 to 16 query heads per KV head")
-    _lib.check_tensor(q, "q", torch.bfloat16, pool_device)
+    if not (Hq > 0 and Hq % kv_heads == 0 and Hq // kv_heads <= 16 and max_q_len >= 0):
+        raise ValueError("1 to 16 query heads per KV head; max_q_len is not negative")
     if out is not None:
-        _lib.check_tensor(out, "out", torch.bfloat16, pool_device)
-        need(out.numel() >= q.numel(), "out is smaller than q")
-    _lib.check_tensor(block_tables, "block_tables", torch.int32, pool_device)
-    _lib.check_tensor(q_start, "q_start", torch.int32, pool_device)
-    _lib.check_tensor(ctx_lens, "ctx_lens", torch.int32, pool_device)
-    n = ctx_lens.numel()
-    need(block_tables.dim() == 2 and block_tables.shape[0] >= n and q_start.numel() == n + 1, "one table row per sequence, one q_start more")
-    need(max_q_len >= 0, "max_q_len")
-    return Tq, Hq, n
+        if not (out.dtype is bf16 and out.get_device() == index and out.is_contiguous()):
+            _lib.check_tensor(out, "out", bf16, index)
+        if out.numel() < q.numel():
+            raise ValueError("out is smaller than q")
+    return Tq, Hq, check_sequences(index, block_tables, q_start, ctx_lens)
 
 
 def _attention_kv4(q, out, pool, layer, block_tables, q_start, ctx_lens, max_q_len, max_ctx, softmax_scale, workspace, rank, pages,
-                   nsplit, split_pages) -> torch.Tensor:
+                   parts) -> torch.Tensor:
     pool.check(layer, rank)
-    Tq, Hq, n = _check_step(q, out, pool.device, pool.heads_per_rank, block_tables, q_start, ctx_lens, max_q_len)
     Hkv = pool.heads_per_rank
-    max_pages = pages.shape[2] if pages is not None else -(-max_ctx // KV4_TOKENS)
-    if nsplit is None:
-        if pages is not None:  # every query row is an item of its own
-            nsplit, split_pages = plan_splits_kv4(Tq, Hkv, 1, Hq // Hkv, max_pages, rows=Tq * Hq)
-        else:
-            nsplit, split_pages = plan_splits_kv4(n, Hkv, max_q_len, Hq // Hkv, max_pages, rows=Tq * Hq)
-    _lib.require(nsplit >= 1 and split_pages >= 1 and nsplit * split_pages >= max_pages, "the splits do not cover max_ctx")
+    Tq, Hq, n = _check_step(q, out, pool.index, Hkv, block_tables, q_start, ctx_lens, max_q_len)
+    group = Hq // Hkv
+    if pages is not None:  # every query row is an item of its own
+        max_pages, rows, prefill = pages.shape[2], group, False
+        planned, split_pages = plan_kv4(Tq, Hkv, 1, group, max_pages)
+    else:
+        max_pages, rows, prefill = -(-max_ctx // KV4_TOKENS), max_q_len * group, max_q_len * group >= TC_MIN_ROWS
+        planned, split_pages = plan_kv4(n, Hkv, max_q_len, group, max_pages, Tq * Hq if prefill else 0)
+    if parts is None:
+        parts = planned
+    elif prefill:
+        _lib.require(parts >= 1, "nsplit")
+        split_pages = -(--(-max_pages // parts) // 4) * 4
+    else:
+        _lib.require(parts >= 0 and parts != 1, "nsplit: 0, or two CTAs at least")
     po = pl = None
-    if nsplit > 1:
+    if parts > 1:
         if workspace is None:
             workspace = AttentionWorkspace(q.device)
-        workspace.ensure(Tq * Hq, nsplit, KV4_DIM)
-        _lib.require(workspace.part_o.device == q.device, "the workspace is on another device")
+        if prefill:
+            workspace.ensure(Tq * Hq, parts, KV4_DIM)
+        else:
+            workspace.ensure(16 if rows <= 8 else 32, parts, KV4_DIM)
+        _lib.require(workspace.part_o.get_device() == pool.index, "the workspace is on another device")
         po, pl = workspace.part_o.data_ptr(), workspace.part_lse.data_ptr()
-    head = (q.data_ptr(), out.data_ptr(), po, pl, pool.c_ptr, layer, rank, block_tables.data_ptr(), block_tables.shape[1],
-            q_start.data_ptr(), ctx_lens.data_ptr(), n, Tq, max_q_len, Hq)
-    if pages is None:
-        _lib.call_on(pool.device, _lib.kv4_fn("daser_paged_attention_kv4"), "paged_attention_kv4", *head, nsplit, split_pages,
-                     softmax_scale)
-    else:
-        _lib.call_on(pool.device, _lib.kv4_fn("daser_sparse_attention_kv4"), "sparse_attention_kv4", *head, pages.data_ptr(), max_pages,
-                     nsplit, split_pages, softmax_scale)
-    if nsplit > 1:
         _lib.launch_count += 1  # the merge kernel
+    if pages is None:
+        _lib.call_on(pool.index, _lib.kv4_fn("daser_paged_attention_kv4"), "paged_attention_kv4", q.data_ptr(), out.data_ptr(), po, pl,
+                     pool.c_ptr, layer, rank, block_tables.data_ptr(), block_tables.shape[1], q_start.data_ptr(), ctx_lens.data_ptr(), n,
+                     Tq, max_q_len, Hq, parts, split_pages, softmax_scale)
+    else:
+        _lib.call_on(pool.index, _lib.kv4_fn("daser_sparse_attention_kv4"), "sparse_attention_kv4", q.data_ptr(), out.data_ptr(), po, pl,
+                     pool.c_ptr, layer, rank, block_tables.data_ptr(), block_tables.shape[1], q_start.data_ptr(), ctx_lens.data_ptr(), n,
+                     Tq, max_q_len, Hq, pages.data_ptr(), max_pages, parts, softmax_scale)
     return out
 
 
@@ -262,19 +272,19 @@ def select_pages(
     page first among equals.  A row that sees at most ``num_pages`` pages gets them all.  ``bounds`` have to cover the context
     (:func:`~daser_b200.ops.kv_ops.update_page_bounds`); other arguments as in :func:`paged_attention`.
     """
-    Hkv, dev = bounds.exps.shape[2], bounds.exps.device
-    _lib.require(dev.type == "cuda" and 0 <= layer < bounds.exps.shape[0], "bounds on a CUDA device, layer inside them")
+    (layers, nb, Hkv), dev = bounds.shape, bounds.index
+    _lib.require(dev >= 0 and 0 <= layer < layers, "bounds on a CUDA device, layer inside them")
     Tq, Hq, n = _check_step(q, None, dev, Hkv, block_tables, q_start, ctx_lens, max_q_len)
     _lib.require(sink_pages >= 0 and recent_pages >= 1 and sink_pages + recent_pages <= num_pages, "sink_pages + recent_pages (at least 1) <= num_pages")
-    pages = torch.empty((Tq, Hkv, num_pages), dtype=torch.int32, device=dev)
+    pages = torch.empty((Tq, Hkv, num_pages), dtype=torch.int32, device=q.device)
     stride = max(1, -(-max_ctx // KV4_TOKENS))
     scores = None
     if stride > num_pages:
         need = Tq * Hkv * stride
-        scores = workspace.ensure_scores(need) if workspace is not None else torch.empty(need, dtype=torch.float32, device=dev)
-        _lib.require(scores.device == dev, "the workspace is on another device")
+        scores = workspace.ensure_scores(need) if workspace is not None else torch.empty(need, dtype=torch.float32, device=q.device)
+        _lib.require(scores.get_device() == dev, "the workspace is on another device")
     _lib.call_on(dev, _lib.kv4_fn("daser_select_pages_kv4"), "select_pages_kv4", q.data_ptr(), bounds.codes.data_ptr(),
-                 bounds.exps.data_ptr(), layer, bounds.exps.shape[1], block_tables.data_ptr(), block_tables.shape[1], q_start.data_ptr(),
+                 bounds.exps.data_ptr(), layer, nb, block_tables.data_ptr(), block_tables.shape[1], q_start.data_ptr(),
                  ctx_lens.data_ptr(), n, Tq, max_q_len, Hq, Hkv, scores.data_ptr() if scores is not None else pages.data_ptr(), stride,
                  pages.data_ptr(), num_pages, sink_pages, recent_pages)
     if stride > num_pages:
@@ -303,6 +313,6 @@ def sparse_paged_attention(
     _lib.require(isinstance(pool, PagedKV4Pool), "sparse attention works on a PagedKV4Pool")
     _lib.require(pages.dim() == 3 and pages.shape[2] >= 1 and tuple(pages.shape[:2]) == (q.shape[0], pool.heads_per_rank),
                  "pages: int32 [rows, KV heads, pages]")
-    _lib.check_tensor(pages, "pages", torch.int32, pool.device)
+    _lib.check_tensor(pages, "pages", torch.int32, pool.index)
     return _attention_kv4(q, out, pool, layer, block_tables, q_start, ctx_lens, max_q_len, 0, softmax_scale, workspace, rank, pages,
-                          None, None)
+                          None)

@@ -9,8 +9,8 @@ namespace daser {
 struct Attn4Params {
   const __nv_bfloat16* q;       // [Tq, Hq, 128]
   __nv_bfloat16* out;           // [Tq, Hq, 128]
-  float* part_o;                // [Tq * Hq, nsplit, 128] (nsplit > 1)
-  float* part_lse;              // [Tq * Hq, nsplit], base-2
+  float* part_o;                // partial outputs, 128 floats each, normalised ...
+  float* part_lse;              // ... and their log2-sum-exp (where they lie: attention4.cu)
   const uint8_t* records;       // the layer's records
   int64_t stride_block, stride_head;
   const int32_t* block_tables;  // [num_seqs, max_blocks]
@@ -19,7 +19,8 @@ struct Attn4Params {
   const int32_t* pages;         // sparse: [Tq, Hkv, n_pages] logical pages, ascending, -1 behind the last
   int max_blocks, num_blocks, num_seqs, Hq, Hkv, G;
   int n_pages;                  // sparse: pages listed per (query row, KV head)
-  int nsplit, split_pages;      // a split is split_pages pages (of the context, or of the list)
+  int workers;                  // decode: CTAs that share all pages evenly, 0 = one CTA per item
+  int nsplit, split_pages;      // prefill: splits of a context, of split_pages pages each
   float scale_log2;             // softmax scale * log2(e)
   int total_q;
 };

@@ -179,13 +179,15 @@ def rope_kv_write(
 
 def _rope_kv4_write(qkv, positions, slot_mapping, cos_sin, q_out, hq, hkv, head_dim, block_tokens, pool, layer, rank, zero_after,
                     qk_norm) -> None:
-    need, dev = _lib.require, pool.device
+    need, dev = _lib.require, pool.index
     pool.check(layer, rank)
     need(head_dim == KV4_DIM and block_tokens == KV4_TOKENS, "a 4-bit pool has head_dim 128 and 16 tokens per block")
-    need(hkv == pool.heads_per_rank, f"the pool keeps {pool.heads_per_rank} KV heads, not {hkv}")
-    need(qkv.dim() == 2 and qkv.device == dev and qkv.dtype in (torch.float32, torch.bfloat16), "qkv: float32 or bfloat16 [T, heads * 128] on the pool's device")
-    T = qkv.shape[0]
-    need(qkv.shape[1] >= (hq + 2 * hkv) * head_dim and qkv.stride(1) == 1, "qkv: too few columns, or columns with a stride")
+    need(hkv == pool.heads_per_rank, "num_kv_heads is not the pool's")
+    need(qkv.dim() == 2 and qkv.get_device() == dev and qkv.dtype in (torch.float32, torch.bfloat16),
+         "qkv: float32 or bfloat16 [T, heads * 128] on the pool's device")
+    T, cols = qkv.shape
+    step, unit = qkv.stride()
+    need(cols >= (hq + 2 * hkv) * head_dim and unit == 1, "qkv: too few columns, or columns with a stride")
     _lib.check_tensor(positions, "positions", torch.int32, dev)
     _lib.check_tensor(slot_mapping, "slot_mapping", torch.int64, dev)
     _lib.check_tensor(cos_sin, "cos_sin", torch.float32, dev)
@@ -201,7 +203,7 @@ def _rope_kv4_write(qkv, positions, slot_mapping, cos_sin, q_out, hq, hkv, head_
             need(w.numel() == head_dim, f"{name}: one value per dim")
         qw, kw = qw.data_ptr(), kw.data_ptr()
     _lib.call_on(dev, _lib.kv4_fn("daser_rope_kv4_write"), "rope_kv4_write", qkv.data_ptr(), int(qkv.dtype == torch.float32),
-                 qkv.stride(0), positions.data_ptr(), slot_mapping.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], q_out.data_ptr(), T,
+                 step, positions.data_ptr(), slot_mapping.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], q_out.data_ptr(), T,
                  hq, hkv, pool.c_ptr, layer, rank, int(zero_after), qw, kw, eps)
 
 

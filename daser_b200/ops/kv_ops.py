@@ -125,10 +125,10 @@ def quantize_fp4b16(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """bf16 CUDA tensor ``[..., D]`` -> (uint8 codes ``[..., D/2]``, uint8 scales ``[..., D/16]``); the format is
     described in :mod:`daser_b200.kv.codec`."""
     _lib.require(x.is_cuda and x.shape[-1] % 16 == 0, "quantize_fp4b16: needs a CUDA tensor whose last dimension is a multiple of 16")
-    _lib.check_tensor(x, "x", torch.bfloat16, x.device)
+    _lib.check_tensor(x, "x", torch.bfloat16, x.get_device())
     codes = torch.empty((*x.shape[:-1], x.shape[-1] // 2), dtype=torch.uint8, device=x.device)
     scales = torch.empty((*x.shape[:-1], x.shape[-1] // 16), dtype=torch.uint8, device=x.device)
-    _lib.call_on(x.device, _lib.kv4_fn("daser_quant_fp4b16"), "quant_fp4b16", x.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+    _lib.call_on(x.get_device(), _lib.kv4_fn("daser_quant_fp4b16"), "quant_fp4b16", x.data_ptr(), codes.data_ptr(), scales.data_ptr(),
                  x.numel())
     return codes, scales
 
@@ -137,10 +137,10 @@ def dequantize_fp4b16(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor
     """The values that :func:`quantize_fp4b16`'s result stands for, in bf16 (exact)."""
     _lib.require(codes.is_cuda and tuple(scales.shape) == (*codes.shape[:-1], codes.shape[-1] // 8) and codes.shape[-1] % 8 == 0,
                  "dequantize_fp4b16: codes [..., D/2] and scales [..., D/16] on a CUDA device")
-    _lib.check_tensor(codes, "codes", torch.uint8, codes.device)
-    _lib.check_tensor(scales, "scales", torch.uint8, codes.device)
+    _lib.check_tensor(codes, "codes", torch.uint8, codes.get_device())
+    _lib.check_tensor(scales, "scales", torch.uint8, codes.get_device())
     out = torch.empty((*codes.shape[:-1], codes.shape[-1] * 2), dtype=torch.bfloat16, device=codes.device)
-    _lib.call_on(codes.device, _lib.kv4_fn("daser_dequant_fp4b16"), "dequant_fp4b16", codes.data_ptr(), scales.data_ptr(),
+    _lib.call_on(codes.get_device(), _lib.kv4_fn("daser_dequant_fp4b16"), "dequant_fp4b16", codes.data_ptr(), scales.data_ptr(),
                  out.data_ptr(), out.numel())
     return out
 
@@ -173,6 +173,7 @@ class PagedKV4Pool:
         self.device = torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
+        self.index = self.device.index if self.device.type == "cuda" else -1
         self.keepalive = keepalive
         c = _lib.KV4Pool()
         for r, ptr in enumerate(self.record_ptrs):
@@ -203,19 +204,20 @@ class PagedKV4Pool:
         return cls.from_tensors([torch.zeros(num_layers, num_blocks, num_heads, KV4_RECORD, dtype=torch.uint8, device=device)])
 
     def check(self, layer: int, rank: int) -> None:
-        _lib.require(self.device.type == "cuda", "the pool's kernels need a CUDA device")
-        _lib.require(0 <= layer < self.num_layers and 0 <= rank < self.n_ranks, f"layer {layer} or rank {rank} outside the pool")
+        if self.index < 0:
+            raise ValueError("the pool's kernels need a CUDA device")
+        if not (0 <= layer < self.num_layers and 0 <= rank < len(self.record_ptrs)):
+            raise ValueError(f"layer {layer} or rank {rank} outside the pool")
 
 
 def kv_read(pool: PagedKV4Pool, layer: int, slot_mapping: torch.Tensor, rank: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
     """Keys and values bf16 ``[T, heads, 128]`` of the tokens at ``slot_mapping`` (int64 ``[T]``, block * 16 + offset,
     as ``rope_kv_write`` takes it), as the pool holds them; a negative slot reads as zeros."""
     pool.check(layer, rank)
-    _lib.check_tensor(slot_mapping, "slot_mapping", torch.int64, pool.device)
+    _lib.check_tensor(slot_mapping, "slot_mapping", torch.int64, pool.index)
     T = slot_mapping.numel()
-    k = torch.empty((T, pool.heads_per_rank, KV4_DIM), dtype=torch.bfloat16, device=pool.device)
-    v = torch.empty_like(k)
-    _lib.call_on(pool.device, _lib.kv4_fn("daser_kv4_read"), "kv4_read", pool.c_ptr, layer, rank, slot_mapping.data_ptr(),
+    k, v = torch.empty((2, T, pool.heads_per_rank, KV4_DIM), dtype=torch.bfloat16, device=pool.device).unbind(0)
+    _lib.call_on(pool.index, _lib.kv4_fn("daser_kv4_read"), "kv4_read", pool.c_ptr, layer, rank, slot_mapping.data_ptr(),
                  k.data_ptr(), v.data_ptr(), T)
     return k, v
 
@@ -230,10 +232,12 @@ class PageBounds:
     def __init__(self, codes: torch.Tensor, exps: torch.Tensor) -> None:
         _lib.require(codes.dim() == 5 and tuple(codes.shape[3:]) == (2, KV4_DIM) and tuple(exps.shape) == tuple(codes.shape[:3]),
                      "codes [layers, blocks, heads, 2, 128], exps [layers, blocks, heads]")
-        _lib.check_tensor(codes, "codes", torch.int8, codes.device)
-        _lib.check_tensor(exps, "exps", torch.int8, codes.device)
+        _lib.check_tensor(codes, "codes", torch.int8, codes.get_device())
+        _lib.check_tensor(exps, "exps", torch.int8, codes.get_device())
         _lib.require(codes.data_ptr() % 16 == 0, "codes have to start on a 16-byte boundary")
         self.codes, self.exps = codes, exps
+        self.index = codes.get_device()
+        self.shape = tuple(exps.shape)  # (layers, blocks, heads)
 
     @classmethod
     def for_pool(cls, pool: PagedKV4Pool) -> "PageBounds":
@@ -244,13 +248,27 @@ class PageBounds:
     def read(self, layer: int, blocks: torch.Tensor) -> torch.Tensor:
         """The bounds of ``blocks`` (int32, any shape) as float32 ``[..., heads, 2, 128]`` (high, low); of a page with a key that is not
         finite, infinities."""
-        dev = self.exps.device
-        _lib.require(dev.type == "cuda" and 0 <= layer < self.exps.shape[0], "bounds on a CUDA device, layer inside them")
-        _lib.check_tensor(blocks, "blocks", torch.int32, dev)
-        out = torch.empty((*blocks.shape, self.exps.shape[2], 2, KV4_DIM), dtype=torch.float32, device=dev)
-        _lib.call_on(dev, _lib.kv4_fn("daser_kv4_bounds_read"), "kv4_bounds_read", self.codes.data_ptr(), self.exps.data_ptr(), layer,
-                     self.exps.shape[1], self.exps.shape[2], blocks.data_ptr(), out.data_ptr(), blocks.numel())
+        layers, nb, heads = self.shape
+        _lib.require(self.index >= 0 and 0 <= layer < layers, "bounds on a CUDA device, layer inside them")
+        _lib.check_tensor(blocks, "blocks", torch.int32, self.index)
+        out = torch.empty((*blocks.shape, heads, 2, KV4_DIM), dtype=torch.float32, device=self.exps.device)
+        _lib.call_on(self.index, _lib.kv4_fn("daser_kv4_bounds_read"), "kv4_bounds_read", self.codes.data_ptr(), self.exps.data_ptr(), layer,
+                     nb, heads, blocks.data_ptr(), out.data_ptr(), blocks.numel())
         return out
+
+
+def check_sequences(index: int, block_tables: torch.Tensor, q_start: torch.Tensor, ctx_lens: torch.Tensor) -> int:
+    """How many sequences a step's tables describe (contiguous int32 tensors on CUDA device ``index``)."""
+    i32 = torch.int32
+    if not (block_tables.dtype is i32 and q_start.dtype is i32 and ctx_lens.dtype is i32
+            and block_tables.get_device() == index and q_start.get_device() == index and ctx_lens.get_device() == index
+            and block_tables.is_contiguous() and q_start.is_contiguous() and ctx_lens.is_contiguous()):
+        for t, name in ((block_tables, "block_tables"), (q_start, "q_start"), (ctx_lens, "ctx_lens")):
+            _lib.check_tensor(t, name, i32, index)
+    n = ctx_lens.numel()
+    if block_tables.dim() != 2 or block_tables.shape[0] < n or q_start.numel() != n + 1:
+        raise ValueError("one row of block_tables per sequence, one entry of q_start more")
+    return n
 
 
 def update_page_bounds(pool: PagedKV4Pool, bounds: PageBounds, layer: int, block_tables: torch.Tensor, q_start: torch.Tensor,
@@ -259,14 +277,10 @@ def update_page_bounds(pool: PagedKV4Pool, bounds: PageBounds, layer: int, block
     new ones; after a restore, the restored ones).  Arguments as ``paged_attention`` takes them; call it behind the step's
     ``rope_kv_write``."""
     pool.check(layer, rank)
-    _lib.require(tuple(bounds.exps.shape) == (pool.num_layers, pool.num_blocks, pool.heads_per_rank) and bounds.exps.device == pool.device,
+    _lib.require(bounds.shape == (pool.num_layers, pool.num_blocks, pool.heads_per_rank) and bounds.index == pool.index,
                  "the bounds belong to a pool of another shape or device")
-    n = ctx_lens.numel()
-    _lib.check_tensor(block_tables, "block_tables", torch.int32, pool.device)
-    _lib.check_tensor(q_start, "q_start", torch.int32, pool.device)
-    _lib.check_tensor(ctx_lens, "ctx_lens", torch.int32, pool.device)
-    _lib.require(block_tables.dim() == 2 and block_tables.shape[0] >= n and q_start.numel() >= n + 1, "one table row and one q_start per sequence")
-    _lib.call_on(pool.device, _lib.kv4_fn("daser_kv4_page_bounds"), "kv4_page_bounds", pool.c_ptr, layer, rank, bounds.codes.data_ptr(),
+    n = check_sequences(pool.index, block_tables, q_start, ctx_lens)
+    _lib.call_on(pool.index, _lib.kv4_fn("daser_kv4_page_bounds"), "kv4_page_bounds", pool.c_ptr, layer, rank, bounds.codes.data_ptr(),
                  bounds.exps.data_ptr(), block_tables.data_ptr(), block_tables.shape[1], q_start.data_ptr(), ctx_lens.data_ptr(), n,
                  max_q_len)
 
@@ -314,7 +328,7 @@ def kv_restore(work: KVWorkList, geo, pool: PagedKVPool | PagedKV4Pool, cos_sin:
     job.layer_begin, job.layer_count = int(layer_begin), int(layer_count)
     if isinstance(pool, PagedKV4Pool):
         pool.check(0, 0)
-        _lib.call_on(pool.device, _lib.kv4_fn("daser_kv4_restore"), "kv4_restore", C.addressof(job), pool.c_ptr, stream=stream)
+        _lib.call_on(pool.index, _lib.kv4_fn("daser_kv4_restore"), "kv4_restore", C.addressof(job), pool.c_ptr, stream=stream)
         return
     pool_c = pool.c_struct()
     _lib.check(_lib.lib().daser_kv_restore(C.byref(job), C.byref(pool_c), _lib.stream_ptr(stream)), "kv_restore")
@@ -329,7 +343,7 @@ def kv_save(work: KVWorkList, geo, pool: PagedKVPool | PagedKV4Pool, rank: int =
     job = _job(work, geo, geo.codec == "fp8b16", None, status, rank)
     if isinstance(pool, PagedKV4Pool):
         pool.check(0, rank)
-        _lib.call_on(pool.device, _lib.kv4_fn("daser_kv4_save"), "kv4_save", C.addressof(job), pool.c_ptr, stream=stream)
+        _lib.call_on(pool.index, _lib.kv4_fn("daser_kv4_save"), "kv4_save", C.addressof(job), pool.c_ptr, stream=stream)
         return
     pool_c = pool.c_struct()
     _lib.check(_lib.lib().daser_kv_save(C.byref(job), C.byref(pool_c), _lib.stream_ptr(stream)), "kv_save")

@@ -302,7 +302,7 @@ def _setup(q_lens, ctx_lens, hq, hkv, seed=0, extra_rows=0, layers=1):
 def _attend(pool, layer, tables, q, start, ctx_lens, max_q, hkv, split=None, ws=None, max_ctx=None, out=None):
     attention, _, _ = _ops()
     out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device="cuda") if out is None else out
-    kw = dict(nsplit=split[0], split_tokens=split[1] * B) if split else {}
+    kw = {} if split is None else dict(nsplit=split)
     attention.paged_attention(q.cuda(), out, pool, layer, tables.cuda(), start.cuda(), torch.tensor(ctx_lens, dtype=torch.int32, device="cuda"),
                               max_q, max_ctx or max(ctx_lens), hkv, D**-0.5, ws, **kw)
     torch.cuda.synchronize()
@@ -316,16 +316,20 @@ def _attend(pool, layer, tables, q, start, ctx_lens, max_q, hkv, split=None, ws=
     ([1], [17], 4, 4, None),                                 # one head per KV head
     ([1, 1, 1, 1], [15, 100, 33, 512], 16, 2, None),
     ([1, 1], [700, 1500], 64, 8, None),
-    ([1, 1], [700, 1500], 64, 8, (4, 24)),                   # forced splits; one is empty for the shorter context
-    ([1, 1], [2500, 90], 10, 2, (3, 60)),                    # five heads per KV head, many pages a warp
-    ([1], [3000], 7, 1, (1, 188)),                           # seven
+    ([1, 1], [700, 1500], 64, 8, 9),                         # nine CTAs share the pages of sixteen items
+    ([1, 1], [2500, 90], 10, 2, 7),                          # five heads per KV head
+    ([1], [3000], 7, 1, 0),                                  # seven
     ([1, 1], [900, 40], 32, 2, None),                        # sixteen: two column tiles
     ([2, 1, 3], [40, 300, 3], 8, 1, None),                   # several query rows; pure prefill of the last sequence
-    ([5, 0, 2], [37, 64, 1000], 16, 4, (2, 32)),             # a sequence without queries
+    ([5, 0, 2], [37, 64, 1000], 16, 4, 5),                   # a sequence without queries
     ([9], [333], 14, 2, None),                               # 63 rows: four row tiles
+    ([9, 1, 4], [333, 20, 700], 14, 2, 6),                   # tiles of several sequences over the CTAs
     ([1, 1, 1], [0, 20, 0], 8, 2, None),                     # no keys at all: zeros
     ([4], [2], 8, 2, None),                                  # the first rows see no key
-    ([1], [4800], 8, 1, (1, 300)),                           # 75 pages a warp: the page windows turn over twice
+    ([1], [9000], 8, 1, 0),                                  # 71 pages a warp: the page windows turn over twice
+    ([1], [9000], 8, 1, 300),                                # CTAs with less than a page a warp
+    ([1, 0, 1, 2], [0, 0, 1700, 5], 4, 2, 50),               # items without keys between shared ones
+    ([1] * 40, list(range(3, 1203, 30)), 8, 1, 31),          # more sequences than a warp has lanes
 ])
 def test_decode_matches_the_formula(q_lens, ctx_lens, hq, hkv, split):
     pool, rec, tables, q, start = _setup(q_lens, ctx_lens, hq, hkv, seed=len(q_lens) + hq, extra_rows=2)
@@ -341,9 +345,9 @@ def test_decode_matches_the_formula(q_lens, ctx_lens, hq, hkv, split):
     ([16], [16], 8, 1, None),                                # a single tile, causal inside it
     ([100], [100], 16, 2, None),
     ([20, 33], [500, 81], 32, 8, None),
-    ([13], [650], 32, 2, (3, 16)),                           # sixteen heads per KV head
-    ([70], [257], 2, 2, (1, 20)),                            # one head per KV head: 70 rows of a tile
-    ([14, 0, 15], [214, 50, 15], 10, 2, (2, 8)),             # five heads: 125 rows a tile; an empty sequence
+    ([13], [650], 32, 2, 3),                                # sixteen heads per KV head
+    ([70], [257], 2, 2, 1),                                  # one head per KV head: 70 rows of a tile
+    ([14, 0, 15], [214, 50, 15], 10, 2, 2),                  # five heads: 125 rows a tile; an empty sequence
     ([30], [12], 8, 2, None),                                # more queries than keys: the first rows see none
     ([130], [130], 7, 1, None),                              # 18 tokens of seven heads a tile
 ])
@@ -380,7 +384,7 @@ def test_what_lies_behind_the_context_does_not_reach_the_output(q_len):
 
 def test_a_key_that_is_not_finite_shows():
     """A NaN in a visible key or value is not turned into a number, in either kernel and through a merge of splits."""
-    for q_len, split in ((1, None), (1, (3, 8)), (16, None), (16, (2, 12))):
+    for q_len, split in ((1, None), (1, 3), (16, None), (16, 2)):
         pool, rec, tables, q, start = _setup([q_len], [300], 8, 1, seed=5)
         rec[0, tables[0, 4].long(), 0, 2048 : 2056] = 0xFF  # the scales of key 64
         from daser_b200.ops import kv_ops
@@ -730,9 +734,9 @@ def test_results_repeat_bit_for_bit():
     attention, _, _ = _ops()
     pool, rec, tables, q, start = _setup([1] * 6, [3000, 20, 800, 1601, 2999, 1], 64, 8, seed=51)
     ws = attention.AttentionWorkspace("cuda")
-    first = _attend(pool, 0, tables, q, start, [3000, 20, 800, 1601, 2999, 1], 1, 8, (6, 32), ws)
+    first = _attend(pool, 0, tables, q, start, [3000, 20, 800, 1601, 2999, 1], 1, 8, 70, ws)
     for _ in range(3):
-        assert torch.equal(_attend(pool, 0, tables, q, start, [3000, 20, 800, 1601, 2999, 1], 1, 8, (6, 32), ws), first)
+        assert torch.equal(_attend(pool, 0, tables, q, start, [3000, 20, 800, 1601, 2999, 1], 1, 8, 70, ws), first)
 
 
 def test_refusals_on_the_gpu():
@@ -745,7 +749,7 @@ def test_refusals_on_the_gpu():
     attention.paged_attention(**good)
     for change in (dict(layer=1), dict(layer=-1), dict(rank=1), dict(num_kv_heads=1), dict(q=qd.half()), dict(q=qd[..., :64]), dict(q=qd[:, :3]),
                    dict(out=out.float()), dict(out=out[:0]), dict(block_tables=t.long()), dict(block_tables=t[:0]), dict(q_start=s[:1]),
-                   dict(ctx_lens=c.cpu()), dict(block_tokens=32), dict(nsplit=2), dict(nsplit=1, split_tokens=16), dict(nsplit=1, split_tokens=40),
+                   dict(ctx_lens=c.cpu()), dict(block_tokens=32), dict(nsplit=1), dict(nsplit=-1), dict(nsplit=2, split_tokens=16),
                    dict(q=torch.zeros(1, 64, 128, dtype=torch.bfloat16, device="cuda"), out=torch.zeros(1, 64, 128, dtype=torch.bfloat16, device="cuda")),
                    dict(q=qd.expand(2, 8, 128), out=torch.empty(2, 8, 128, dtype=torch.bfloat16, device="cuda"))):
         with pytest.raises(ValueError):

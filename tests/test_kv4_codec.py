@@ -177,7 +177,7 @@ def test_c_entry_points_refuse_bad_pools(change, code):
     assert _lib.kv4_fn("daser_rope_kv4_write")(a, 1, 1536, a, a, a, 8, a, 1, 8, 2, p, 0, 0, 0, None, None, 0.0, None) == code
     assert _lib.kv4_fn("daser_kv4_page_bounds")(p, 0, 0, a, a, a, 4, a, a, 1, 1, None) == code
     assert _lib.kv4_fn("daser_paged_attention_kv4")(a, a, a, a, p, 0, 0, a, 4, a, a, 1, 1, 1, 8, 1, 4, 1.0, None) == code
-    assert _lib.kv4_fn("daser_sparse_attention_kv4")(a, a, a, a, p, 0, 0, a, 4, a, a, 1, 1, 1, 8, a, 4, 1, 4, 1.0, None) == code
+    assert _lib.kv4_fn("daser_sparse_attention_kv4")(a, a, a, a, p, 0, 0, a, 4, a, a, 1, 1, 1, 8, a, 4, 2, 1.0, None) == code
 
 
 def test_c_entry_points_refuse_bad_arguments():
@@ -196,13 +196,18 @@ def test_c_entry_points_refuse_bad_arguments():
         args[at] = bad
         assert write(*args) == code, at
     ok = [a, a, a, a, p, 0, 0, a, 4, a, a, 1, 1, 1, 8, 2, 4, 1.0, None]
-    for at, bad, code in ((14, 7, -1), (14, 34, -2), (15, 0, -1), (16, 0, -1), (2, None, -1), (8, 0, -1), (0, a + 2, -2), (11, -1, -1)):
+    for at, bad, code in ((14, 7, -1), (14, 34, -2), (15, 1, -1), (15, -1, -1), (15, 513, -3), (2, None, -1), (8, 0, -1), (0, a + 2, -2), (11, -1, -1)):
         args = list(ok)
         args[at] = bad
         assert att(*args) == code, at
     sparse = _lib.kv4_fn("daser_sparse_attention_kv4")
-    assert sparse(a, a, a, a, p, 0, 0, a, 4, a, a, 1, 1, 1, 8, a, 9, 2, 4, 1.0, None) == -1  # the splits do not cover the list
-    assert sparse(a, a, a, a, p, 0, 0, a, 4, a, a, 1, 1, 1, 8, a, 0, 2, 4, 1.0, None) == -1
+    assert sparse(a, a, a, a, p, 0, 0, a, 4, a, a, 1, 1, 1, 8, a, 9, 1, 1.0, None) == -1  # one CTA has nothing to share
+    assert sparse(a, a, a, a, p, 0, 0, a, 4, a, a, 1, 1, 1, 8, a, 0, 2, 1.0, None) == -1
+    prefill = [a, a, a, a, p, 0, 0, a, 4, a, a, 1, 64, 64, 8, 2, 4, 1.0, None]  # 4 heads x 64 queries: splits
+    for at, bad in ((15, 0), (16, 0)):
+        args = list(prefill)
+        args[at] = bad
+        assert att(*args) == -1, at
     sel = _lib.kv4_fn("daser_select_pages_kv4")
     ok = [a, a, a, 0, 4, a, 4, a, a, 1, 1, 1, 8, 2, a, 4, a, 8, 1, 4, None]
     for at, bad, code in ((17, 4, -1), (18, -1, -1), (19, 0, -1), (12, 9, -1), (12, 34, -2), (1, a + 4, -2), (15, 0, -1), (11, 70000, -3)):
@@ -211,20 +216,23 @@ def test_c_entry_points_refuse_bad_arguments():
         assert sel(*args) == code, at
     # nothing to do is not an error, and launches nothing
     assert read(p, 0, 0, None, None, None, 0, None) == 0
-    assert att(a, a, None, None, p, 0, 0, a, 4, a, a, 0, 0, 0, 8, 1, 4, 1.0, None) == 0
+    assert att(a, a, None, None, p, 0, 0, a, 4, a, a, 0, 0, 0, 8, 0, 0, 1.0, None) == 0
 
 
-def test_split_plans_cover_the_context():
+def test_plans_cover_the_context():
     from daser_b200.ops import attention
 
     for seqs in (1, 3, 64):
         for heads, group in ((1, 8), (8, 8), (8, 5), (2, 16), (4, 1)):
             for q in (1, 2, 9, 64, 500):
                 for pages in (0, 1, 2, 15, 17, 129, 8192, 65536):
-                    n, per = attention.plan_splits_kv4(seqs, heads, q, group, pages, rows=seqs * q * heads * group)
-                    assert n >= 1 and per >= 1 and n * per >= pages
-                    assert n == 1 or (n - 1) * per < pages  # no split is empty for the longest context
-                    assert n == 1 or n * seqs * q * heads * group <= attention.MAX_ROW_SPLITS
+                    n, per = attention.plan_kv4(seqs, heads, q, group, pages, rows=seqs * q * heads * group)
+                    if q * group >= 64:
+                        assert n >= 1 and per >= 1 and n * per >= pages
+                        assert n == 1 or (n - 1) * per < pages  # no split is empty for the longest context
+                        assert n == 1 or n * seqs * q * heads * group <= attention.MAX_ROW_SPLITS
+                    else:
+                        assert n == 0 or 2 <= n <= 296
 
 
 def test_outgrown_workspace_buffers_stay_alive():
