@@ -171,8 +171,8 @@ _KV4_ARGS = {
     "daser_kv4_bounds_read": [_P, _P, _I, _I, _I, _P, _P, _I, _P],
     "daser_quant_fp4b16": [_P, _P, _P, _L, _P],
     "daser_dequant_fp4b16": [_P, _P, _P, _L, _P],
-    "daser_paged_attention_kv4": [_P, _P, _P, _P, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P],
-    "daser_sparse_attention_kv4": [_P, _P, _P, _P, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _P, _I, _I, _F, _P],
+    "daser_paged_attention_kv4": [_P, _P, _P, _P, _P, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P],
+    "daser_sparse_attention_kv4": [_P, _P, _P, _P, _P, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _P, _I, _I, _F, _P],
     "daser_select_pages_kv4": [_P, _P, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _P, _I, _P, _I, _I, _I, _P],
 }
 _kv4_fns: dict = {}

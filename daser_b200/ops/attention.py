@@ -74,13 +74,10 @@ def plan_splits(num_seqs: int, kv_heads: int, max_q_len: int, group: int, max_ct
 
 
 def kv4_status() -> int:
-    """Non-zero if a CTA of the 4-bit attention kernels ever gave up on a bounded wait (synchronises): bit 0 decode,
-    bit 1 prefill."""
-    out, bits = C.c_uint32(0), 0
-    for bit, name in enumerate(("daser_attention4_status", "daser_attention4_tc_status")):
-        _lib.check(getattr(_lib.lib(), name)(C.byref(out)), name)
-        bits |= int(out.value != 0) << bit
-    return bits
+    """Non-zero if a CTA of the 4-bit prefill kernel ever gave up on a bounded wait (synchronises)."""
+    out = C.c_uint32(0)
+    _lib.check(_lib.lib().daser_attention4_tc_status(C.byref(out)), "attention4_tc_status")
+    return int(out.value)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -98,13 +95,12 @@ def plan_kv4(num_seqs: int, kv_heads: int, max_q_len: int, group: int, max_pages
             nsplit = max(1, min(nsplit, MAX_ROW_SPLITS // rows))
         per = -(--(-max_pages // nsplit) // 4) * 4
         return -(-max_pages // per), per
-    # up to 12 pages a warp, one CTA per item takes less than the merge kernel that sharing needs
+    # up to three pairs of pages a warp, one CTA per item takes less than the merge kernel that sharing needs
     if max_pages <= 96:
         return 0, 0
-    # two CTAs a SM (one with two column tiles), and four pages a warp at least
-    resident = NUM_SMS * (2 if max_q_len * group <= 8 else 1)
+    # one CTA per SM, and a pair of pages a warp at least
     pages = max(1, num_seqs) * kv_heads * -(-max_q_len * group // (8 if max_q_len * group <= 8 else 16)) * max_pages
-    return max(2, min(resident, pages // 32)), 0
+    return max(2, min(NUM_SMS, pages // 32)), 0
 
 
 class AttentionWorkspace:
@@ -118,6 +114,7 @@ class AttentionWorkspace:
         self.part_o: Optional[torch.Tensor] = None
         self.part_lse: Optional[torch.Tensor] = None
         self.scores: Optional[torch.Tensor] = None  # of select_pages
+        self.shared: Optional[torch.Tensor] = None  # which CTAs share an item of the 4-bit decode kernel
         self._outgrown: list = []
 
     def ensure(self, rows: int, nsplit: int, head_dim: int) -> None:
@@ -126,6 +123,12 @@ class AttentionWorkspace:
             self._outgrown += [self.part_o, self.part_lse]
             self.part_o = torch.empty(need * head_dim, dtype=torch.float32, device=self.device)
             self.part_lse = torch.empty(need, dtype=torch.float32, device=self.device)
+
+    def ensure_shared(self, items: int) -> torch.Tensor:
+        if self.shared is None or self.shared.numel() < 2 * items:
+            self._outgrown.append(self.shared)
+            self.shared = torch.empty(2 * items, dtype=torch.int32, device=self.device)
+        return self.shared
 
     def ensure_scores(self, need: int) -> torch.Tensor:
         if self.scores is None or self.scores.numel() < need:
@@ -228,7 +231,7 @@ def _attention_kv4(q, out, pool, layer, block_tables, q_start, ctx_lens, max_q_l
         split_pages = -(--(-max_pages // parts) // 4) * 4
     else:
         _lib.require(parts >= 0 and parts != 1, "nsplit: 0, or two CTAs at least")
-    po = pl = None
+    po = pl = sh = None
     if parts > 1:
         if workspace is None:
             workspace = AttentionWorkspace(q.device)
@@ -236,15 +239,16 @@ def _attention_kv4(q, out, pool, layer, block_tables, q_start, ctx_lens, max_q_l
             workspace.ensure(Tq * Hq, parts, KV4_DIM)
         else:
             workspace.ensure(16 if rows <= 8 else 32, parts, KV4_DIM)
+            sh = workspace.ensure_shared((Tq if pages is not None else n * -(-rows // 8)) * Hkv).data_ptr()
         _lib.require(workspace.part_o.get_device() == pool.index, "the workspace is on another device")
         po, pl = workspace.part_o.data_ptr(), workspace.part_lse.data_ptr()
         _lib.launch_count += 1  # the merge kernel
     if pages is None:
-        _lib.call_on(pool.index, _lib.kv4_fn("daser_paged_attention_kv4"), "paged_attention_kv4", q.data_ptr(), out.data_ptr(), po, pl,
+        _lib.call_on(pool.index, _lib.kv4_fn("daser_paged_attention_kv4"), "paged_attention_kv4", q.data_ptr(), out.data_ptr(), po, pl, sh,
                      pool.c_ptr, layer, rank, block_tables.data_ptr(), block_tables.shape[1], q_start.data_ptr(), ctx_lens.data_ptr(), n,
                      Tq, max_q_len, Hq, parts, split_pages, softmax_scale)
     else:
-        _lib.call_on(pool.index, _lib.kv4_fn("daser_sparse_attention_kv4"), "sparse_attention_kv4", q.data_ptr(), out.data_ptr(), po, pl,
+        _lib.call_on(pool.index, _lib.kv4_fn("daser_sparse_attention_kv4"), "sparse_attention_kv4", q.data_ptr(), out.data_ptr(), po, pl, sh,
                      pool.c_ptr, layer, rank, block_tables.data_ptr(), block_tables.shape[1], q_start.data_ptr(), ctx_lens.data_ptr(), n,
                      Tq, max_q_len, Hq, pages.data_ptr(), max_pages, parts, softmax_scale)
     return out

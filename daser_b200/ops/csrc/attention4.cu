@@ -4,15 +4,18 @@
 //   o_r = sum_k softmax_k(scale q_r . k_k) v_k over the keys k <= pos_r (of the listed pages, in the sparse form)
 //
 // In the reference's serving stack this is stock vLLM's paged decode kernel over a bf16 cache.  Here a step's time is
-// the 2304-byte records of the pages (0.5625 B per element against 2), as long as the tensor pipe and the dequantisation
-// keep up: per page and warp 64 conversions, 64 multiplications by scales, 16 MMAs.
+// the 2304-byte records of the pages (0.5625 B per element against 2), as long as the dequantisation keeps up: per page 64 conversions, 64
+// multiplications by scales and 16 MMAs of a warp, about 60 cycles of an SM where the memory needs 100.
 //
-// * One warp is one worker.  The eight warps of a CTA take pairs of pages of its range in turn; two lanes fetch a pair with one bulk copy
-//   each into the warp's own ring (3 pairs), so no CTA-wide barrier exists before the merge of the warps.
-// * An item is (sequence, tile of query rows, KV head).  With many pages a fixed number of CTAs (two a SM) shares the pages of ALL
+// * A CTA (one per SM) has 16 warps that take pairs of pages in turn and fetch their own, three pairs ahead, with 16-byte asynchronous
+//   copies: nine a lane and pair, no barrier in the CTA before an item is put together.  (One bulk copy a page, by each warp or by
+//   a producer warp, was measured first: the copy engine of an SM took about 90 cycles for a record of 2304 bytes whoever asked, which
+//   is 26 bytes a cycle, and a lane that asks waits for it: 150 us against 130 for 32 sequences of 4k - 32k tokens.)  The next item's first pages are on their way while the parts of the
+//   last one are put together.
+// * An item is (sequence, tile of query rows, KV head).  With many pages a fixed number of CTAs shares the pages of ALL
 //   items evenly: CTA c takes [c T / W, (c + 1) T / W) of the T pages in item order, whatever the lengths are, so that
-//   all finish together (splits of a fixed length left the last wave a third empty: 73 us against 5x us at 8 sequences of
-//   16k - 32k tokens).  An item that lies in several CTAs is put together by attn4_merge_kernel from their partial results.
+//   all finish together (splits of a fixed length left the last wave a third empty).  An item that lies in several CTAs is put
+//   together by attn4_merge_kernel from their partial results.
 // * The cache is the A operand of mma.sync m16n8k16, the queries the B operand: S^T = K Q^T (16 tokens x 8 rows) and
 //   O^T = V^T P^T (16 dims x 8 rows).  With at most 8 query heads per KV head that is half the MMAs (16 a page) of the form that puts
 //   queries in the 16 rows of A.  The contraction index may be permuted as long as A and B agree, so a lane (g = lane / 4,
@@ -26,14 +29,20 @@
 namespace daser {
 using namespace sm100;
 
-constexpr int A4_WARPS = 8;
 constexpr int A4_PAIR = 2 * DASER_KV4_RECORD;
-constexpr int A4_STAGES = 3;                           // pairs of pages
-constexpr int A4_RING = A4_STAGES * A4_PAIR;           // per warp
-constexpr int A4_OPITCH = 132;                         // floats per row of the merge buffer
+constexpr int A4_OPITCH = 132;  // floats per row of a warp's part
+// Warps and ring depth (pairs per warp) for NT column tiles: two tiles need twice the accumulators.
+template <int NT> struct A4 {
+  static constexpr int ROWS = 8 * NT;
+  static constexpr int WARPS = NT == 1 ? 16 : 8;
+  static constexpr int STAGES = NT == 1 ? 3 : 4;
+  static constexpr int RING = WARPS * STAGES * A4_PAIR;
+  // Where a warp leaves its part of an item: in the stage of its last pair if it fits in there.
+  static constexpr int PART = ROWS * A4_OPITCH * 4;
+  static constexpr bool IN_RING = PART <= A4_PAIR;
+  static constexpr int SMEM = RING + (IN_RING ? 0 : WARPS * PART);
+};
 constexpr float A4_RAISE_AT = 8.f;
-
-__device__ uint32_t g_attn4_status = 0;  // bit 0: a bounded wait ran out
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -63,14 +72,11 @@ __device__ __forceinline__ uint32_t movmatrix_t(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
   return r;
 }
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-               "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-
+// What beginning and finishing an item costs a CTA, in pages: items count that much more when the pages are shared out (about 8000
+// cycles against 100 a page; 32 sequences of 4k - 32k tokens: 148 us with 1, 133 with 48, 130 with 72 to 128).
+constexpr int A4_ITEM_COST = 80;
 // Pages of an item of the dense form: (query rows [row0, row0 + ROWS) of a sequence of q_len new tokens and ctx keys) sees the keys
-// below limit.  Every item counts one page at least: somebody has to write its zeros.
+// below limit.
 __device__ __forceinline__ int item_limit(int q_len, int q_all, int ctx, int G, int row0, int rows) {
   return ctx - q_all + min((row0 + rows - 1) / G, q_len - 1) + 1;
 }
@@ -89,13 +95,13 @@ __device__ __forceinline__ SeqInfo seq_info(const Attn4Params& p, int seq) {
   s.ctx = p.ctx_lens[seq];
   return s;
 }
-// Pages of all items of a sequence.
+// Pages of all items of a sequence, with what an item costs.
 template <int ROWS, bool SPARSE>
 __device__ __forceinline__ int64_t seq_pages(const Attn4Params& p, int seq) {
   const SeqInfo s = seq_info(p, seq);
-  if (SPARSE) return (int64_t)s.q_len * p.Hkv * p.n_pages;
+  if (SPARSE) return (int64_t)s.q_len * p.Hkv * (p.n_pages + A4_ITEM_COST);
   int64_t n = 0;
-  for (int row0 = 0; row0 < s.q_len * p.G; row0 += ROWS) n += max(1, item_pages(p, item_limit(s.q_len, s.q_all, s.ctx, p.G, row0, ROWS)));
+  for (int row0 = 0; row0 < s.q_len * p.G; row0 += ROWS) n += item_pages(p, item_limit(s.q_len, s.q_all, s.ctx, p.G, row0, ROWS)) + A4_ITEM_COST;
   return n * p.Hkv;
 }
 __device__ __forceinline__ int64_t warp_sum_i64(int64_t v) {
@@ -103,167 +109,206 @@ __device__ __forceinline__ int64_t warp_sum_i64(int64_t v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-// Pages of all sequences below `upto` (every lane of a warp calls it, and gets the sum).
-template <int ROWS, bool SPARSE>
-__device__ __forceinline__ int64_t pages_below(const Attn4Params& p, int upto) {
-  int64_t n = 0;
-  for (int s = threadIdx.x & 31; s < upto; s += 32) n += seq_pages<ROWS, SPARSE>(p, s);
-  return warp_sum_i64(n);
-}
 // The CTA that owns page x of T when W share them: CTA c owns [floor(c T / W), floor((c + 1) T / W)).
 __device__ __forceinline__ int owner_of(int64_t x, int64_t T, int W) { return (int)(((x + 1) * W - 1) / T); }
 
+// The items of a CTA, one after the other; its warps walk them on their own.
 template <int NT, bool SPARSE>
-__global__ void __launch_bounds__(A4_WARPS * 32, NT == 1 ? 2 : 1)
-attn4_kernel(const Attn4Params p) {
-  constexpr int ROWS = 8 * NT;
-  extern __shared__ __align__(128) uint8_t a4_smem[];
-  __shared__ __align__(8) uint64_t s_bar[A4_WARPS][A4_STAGES];
-  __shared__ uint32_t s_abort;
-  __shared__ float s_m[A4_WARPS][ROWS], s_l[A4_WARPS][ROWS];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, t = lane & 3;
-  if (lane == 0) {
-#pragma unroll
-    for (int s = 0; s < A4_STAGES; ++s) mbar_init(&s_bar[warp][s], 1);
-    if (warp == 0) s_abort = 0u;
-    mbar_init_fence();
-  }
-  __syncthreads();  // s_abort and the barriers, before any wait looks at them
-  pdl_enter();
-
-  const int G = p.G;
-  // ---- where this CTA starts: item (seq, tile, kvh), page p0 of it, and how many pages it takes ----
-  int seq, tile, kvh, p0 = 0;
-  int64_t todo = 1;  // pages left to this CTA (one CTA per item: the whole item, see below)
+struct Walk {
+  int seq, tile, kvh;  // the item
+  int p0;              // its first page that is this CTA's
+  int64_t at, todo, T; // p0 in the order of all pages, pages left to this CTA from there on, pages of all items
   SeqInfo si;
-  if (p.workers == 0) {
-    kvh = blockIdx.x;
-    seq = blockIdx.y;
-    tile = blockIdx.z;
-    si = seq_info(p, seq);
-    if (SPARSE ? tile >= si.q_len : tile * ROWS >= si.q_len * G) return;  // uniform over the CTA
-  } else {
-    const int64_t T = pages_below<ROWS, SPARSE>(p, p.num_seqs);
-    int64_t at = (int64_t)blockIdx.x * T / p.workers;
+  // of the item:
+  int row0, tok0, n_rows;  // rows: dense, ROWS consecutive ones (query token major, then head of the group); sparse, the heads of one token
+  int first_pos, limit;    // last key the first row may see, keys the last row sees
+  int n_item, p1;          // pages and the item's cost, end of this CTA's part
+  int page_end;            // the same of the pages alone
+  const int32_t* list;
+
+  __device__ __forceinline__ void item(const Attn4Params& p) {
+    constexpr int ROWS = A4<NT>::ROWS;
+    n_rows = SPARSE ? p.G : si.q_len * p.G;
+    row0 = SPARSE ? 0 : tile * ROWS;
+    tok0 = SPARSE ? tile : row0 / p.G;
+    first_pos = si.ctx - si.q_all + tok0;
+    limit = SPARSE ? first_pos + 1 : item_limit(si.q_len, si.q_all, si.ctx, p.G, row0, ROWS);
+    list = SPARSE ? p.pages + ((int64_t)(si.q0 + tok0) * p.Hkv + kvh) * p.n_pages : nullptr;
+    const int real = SPARSE ? p.n_pages : item_pages(p, limit);
+    n_item = real + A4_ITEM_COST;
+    if (p.workers == 0) todo = n_item;
+    p1 = (int)min((int64_t)n_item, p0 + todo);
+    page_end = min(p1, real);
+  }
+  // The first item; false if there is none.
+  __device__ __forceinline__ bool start(const Attn4Params& p) {
+    constexpr int ROWS = A4<NT>::ROWS;
+    const int lane = threadIdx.x & 31;
+    p0 = 0;
+    at = 0;
+    if (p.workers == 0) {
+      kvh = blockIdx.x;
+      seq = blockIdx.y;
+      tile = blockIdx.z;
+      si = seq_info(p, seq);
+      if (SPARSE ? tile >= si.q_len : tile * ROWS >= si.q_len * p.G) return false;
+      item(p);
+      return true;
+    }
+    int64_t mine = lane < p.num_seqs ? seq_pages<ROWS, SPARSE>(p, lane) : 0;  // of sequence base + lane
+    T = warp_sum_i64(mine);
+    for (int s = 32 + lane; s - lane < p.num_seqs; s += 32) T += warp_sum_i64(s < p.num_seqs ? seq_pages<ROWS, SPARSE>(p, s) : 0);
+    at = (int64_t)blockIdx.x * T / p.workers;
     todo = (int64_t)(blockIdx.x + 1) * T / p.workers - at;
-    if (todo == 0) return;
-    // the sequence that page `at` is in
-    seq = 0;
+    if (todo == 0) return false;
+    int64_t x = at;  // relative to the sequence, the tile, the item
     for (int base = 0;; base += 32) {
-      int64_t mine = base + lane < p.num_seqs ? seq_pages<ROWS, SPARSE>(p, base + lane) : 0;
+      if (base > 0) mine = base + lane < p.num_seqs ? seq_pages<ROWS, SPARSE>(p, base + lane) : 0;
       int64_t upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += y;
       }
-      const uint32_t behind = __ballot_sync(0xffffffffu, upto > at);
+      const uint32_t behind = __ballot_sync(0xffffffffu, upto > x);
       if (behind != 0u) {
         const int who = __ffs(behind) - 1;
         seq = base + who;
-        at -= __shfl_sync(0xffffffffu, upto - mine, who);
+        x -= __shfl_sync(0xffffffffu, upto - mine, who);
         break;
       }
-      at -= __shfl_sync(0xffffffffu, upto, 31);
+      x -= __shfl_sync(0xffffffffu, upto, 31);
     }
     si = seq_info(p, seq);
     for (tile = 0;; ++tile) {
-      const int n = SPARSE ? p.n_pages : max(1, item_pages(p, item_limit(si.q_len, si.q_all, si.ctx, G, tile * ROWS, ROWS)));
-      if (at < (int64_t)n * p.Hkv) {
-        kvh = (int)(at / n);
-        p0 = (int)(at - (int64_t)kvh * n);
+      const int n = (SPARSE ? p.n_pages : item_pages(p, item_limit(si.q_len, si.q_all, si.ctx, p.G, tile * ROWS, ROWS))) + A4_ITEM_COST;
+      if (x < (int64_t)n * p.Hkv) {
+        kvh = (int)(x / n);
+        p0 = (int)(x - (int64_t)kvh * n);
         break;
       }
-      at -= (int64_t)n * p.Hkv;
+      x -= (int64_t)n * p.Hkv;
     }
+    item(p);
+    return true;
   }
-  uint8_t* ring = a4_smem + warp * A4_RING;
+  __device__ __forceinline__ bool next(const Attn4Params& p) {
+    const int done = p1 - p0;
+    at += done;
+    todo -= done;
+    if (todo <= 0) return false;
+    p0 = 0;
+    if (++kvh == p.Hkv) {
+      kvh = 0;
+      ++tile;
+      if (SPARSE ? tile >= si.q_len : tile * A4<NT>::ROWS >= si.q_len * p.G) {
+        tile = 0;
+        // (pages are left, so a sequence with queries is)
+        do si = seq_info(p, ++seq);
+        while (si.q_len == 0 && seq + 1 < p.num_seqs);
+      }
+    }
+    item(p);
+    return true;
+  }
+};
+
+template <int NT, bool SPARSE>
+__global__ void __launch_bounds__(A4<NT>::WARPS * 32, 1)
+attn4_kernel(const Attn4Params p) {
+  using C = A4<NT>;
+  constexpr int ROWS = C::ROWS, WARPS = C::WARPS, STAGES = C::STAGES;
+  extern __shared__ __align__(128) uint8_t a4_smem[];  // ring [warp][stage][2 records], parts [warp][row][A4_OPITCH]
+  __shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS];
+  __shared__ int s_part[WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int G = p.G;
+  pdl_enter();
+  Walk<NT, SPARSE> it;
+  if (!it.start(p)) return;  // uniform over the CTA
+
+  const uint8_t* ring = a4_smem + warp * STAGES * A4_PAIR;
   const uint32_t ring_u32 = smem_u32(ring);
-  // the ring of this warp, over all items: where the next record goes, where the next one to use is, and its phase
-  int put = 0, get = 0;
-  uint32_t phase = 0;
-
-  while (todo > 0) {
-  // ---- the item ----
-  // rows: dense, ROWS consecutive rows (query token major, then head of the group); sparse, the heads of one query token
-  const int q0 = si.q0;
-  const int n_rows = SPARSE ? G : si.q_len * G;
-  const int row0 = SPARSE ? 0 : tile * ROWS;
-  const int tok0 = SPARSE ? tile : row0 / G;
-  const int first_pos = si.ctx - si.q_all + tok0;  // last key the first row may see
-  const int limit = SPARSE ? first_pos + 1 : item_limit(si.q_len, si.q_all, si.ctx, G, row0, ROWS);  // keys the last row sees
-  const int32_t* list = SPARSE ? p.pages + ((int64_t)(q0 + tok0) * p.Hkv + kvh) * p.n_pages : nullptr;
-  const int real = SPARSE ? p.n_pages : item_pages(p, limit);
-  const int n_item = max(1, real);
-  if (p.workers == 0) todo = n_item;
-  const int p1 = (int)min((int64_t)n_item, p0 + todo);
-  const int page_begin = p0, page_end = min(p1, real);
-  const int n_pairs = (page_end - page_begin + 1) >> 1;  // negative or zero: nothing to read
-  const int mine = n_pairs > warp ? (n_pairs - warp + A4_WARPS - 1) / A4_WARPS : 0;  // pairs of this warp: warp, warp + 8, ...
-
-  // ---- page fetch ----
-  // Page k of this warp (k = 2 * pair + which) is entry k & 31 of window k / 32, one per lane: its logical page (negative: skipped)
-  // and its record's offset, read a window ahead of their use.
-  const int32_t* table = p.block_tables + (int64_t)seq * p.max_blocks;
-  auto window = [&](int w, int& logical, int64_t& offset) {
+  // Page k of this warp (k = 2 * pair + which) of an item is entry k & 31 of window k / 32, one per lane: its logical page (sparse;
+  // negative: none) and its block (negative: not fetched), read a window ahead of their use.
+  int log_cur, log_nxt, blk_cur, blk_nxt;  // windows of the fetches
+  auto window = [&](int w, int& logical, int& block) {
     const int k = 32 * w + lane;
-    const int at = page_begin + 2 * (warp + (k >> 1) * A4_WARPS) + (k & 1);
+    const int at = it.p0 + 2 * (warp + (k >> 1) * WARPS) + (k & 1);
     logical = -1;
-    offset = 0;
-    if ((k >> 1) < mine && at < page_end) {
-      logical = SPARSE ? list[at] : at;
-      if (logical >= 0 && logical < p.max_blocks && (int64_t)logical * DASER_KV4_TOKENS < limit) {
-        int block = table[logical];
+    block = -1;
+    if (at < it.page_end) {
+      logical = SPARSE ? it.list[at] : at;
+      if (logical >= 0 && logical < p.max_blocks && (int64_t)logical * DASER_KV4_TOKENS < it.limit) {
+        block = p.block_tables[(int64_t)it.seq * p.max_blocks + logical];
         block = block < 0 ? 0 : (block >= p.num_blocks ? p.num_blocks - 1 : block);
-        offset = (int64_t)block * p.stride_block + (int64_t)kvh * p.stride_head;
       } else {
         logical = -1;
       }
     }
   };
-  int log_cur, log_nxt;  // windows of the fetches
-  int64_t off_cur, off_nxt;
-  window(0, log_cur, off_cur);
-  window(1, log_nxt, off_nxt);
-  int use_cur = log_cur, use_nxt = log_nxt;  // windows of the uses, which run behind
-  auto fetch = [&](int i) {  // all lanes; pairs 0, 1, 2, ...
+  int put = 0, get = 0;  // stages
+  // Pair i (0, 1, 2, ... of the item) into the next stage: 288 pieces of 16 bytes, page 0 then page 1.  One group a call.
+  auto fetch = [&](int i) {
     const int e = (2 * i) & 31;
     if (e == 0 && i > 0) {
       log_cur = log_nxt;
-      off_cur = off_nxt;
-      window((i >> 4) + 1, log_nxt, off_nxt);
+      blk_cur = blk_nxt;
+      window((i >> 4) + 1, log_nxt, blk_nxt);
     }
-    const int from = e + (lane & 1);
-    const int64_t off = __shfl_sync(0xffffffffu, off_cur, from);
-    const bool there = __shfl_sync(0xffffffffu, log_cur, from) >= 0;
-    const uint32_t pair = __ballot_sync(0xffffffffu, there) & 3u;
-    uint64_t* bar = &s_bar[warp][put];
-    if (lane == 0) mbar_expect_tx(bar, __popc(pair) * DASER_KV4_RECORD);
-    __syncwarp();
-    if (lane < 2 && there) bulk_load(ring_u32 + put * A4_PAIR + lane * DASER_KV4_RECORD, p.records + off, DASER_KV4_RECORD, bar);
-    put = put == A4_STAGES - 1 ? 0 : put + 1;
+    const int b0 = __shfl_sync(0xffffffffu, blk_cur, e), b1 = __shfl_sync(0xffffffffu, blk_cur, e + 1);
+    const uint8_t* head = p.records + (int64_t)it.kvh * p.stride_head + lane * 16;
+    const uint8_t* r0 = head + (int64_t)b0 * p.stride_block;
+    const uint8_t* r1 = head + (int64_t)b1 * p.stride_block - DASER_KV4_RECORD;  // piece 144 is its first
+    const uint32_t dst = ring_u32 + put * A4_PAIR + lane * 16;
+    if (b0 >= 0) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) cp_async16(dst + u * 512, r0 + u * 512);
+    }
+    if (lane < 16 ? b0 >= 0 : b1 >= 0) cp_async16(dst + 4 * 512, (lane < 16 ? r0 : r1) + 4 * 512);
+    if (b1 >= 0) {
+#pragma unroll
+      for (int u = 5; u < 9; ++u) cp_async16(dst + u * 512, r1 + u * 512);
+    }
+    cp_async_commit();
+    put = put == STAGES - 1 ? 0 : put + 1;
   };
-  int fetched = 0;
-  for (; fetched < A4_STAGES && fetched < mine; ++fetched) fetch(fetched);
+  auto first_windows = [&] {
+    window(0, log_cur, blk_cur);
+    window(1, log_nxt, blk_nxt);
+  };
+  uint4 qr[NT][4];  // the rows of the queries that this lane holds, as they are
+  auto load_q = [&] {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = it.row0 + 8 * nt + g;
+      const int tq = SPARSE ? it.tok0 : r / G, h = SPARSE ? r : r % G;
+      const __nv_bfloat16* qp = p.q + ((int64_t)(it.si.q0 + tq) * p.Hq + it.kvh * G + h) * ATT_D + 32 * t;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qr[nt][i] = r < it.n_rows ? *reinterpret_cast<const uint4*>(qp + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  first_windows();
+#pragma unroll
+  for (int i = 0; i < STAGES; ++i) fetch(i);  // (a pair that is not there is an empty group)
+  load_q();
+  bool parts_read = true;  // false: the parts of the last item are still being read
 
+  bool more;
+  do {
+  const int row0 = it.row0, tok0 = it.tok0, n_rows = it.n_rows, first_pos = it.first_pos, limit = it.limit, kvh = it.kvh, q0 = it.si.q0;
+  int use_cur = log_cur, use_nxt = log_nxt;  // windows of the uses, which run behind those of the fetches
   // ---- queries: B fragments, scaled, f16.  Column g of n-tile nt is row row0 + 8 nt + g ----
   uint32_t qf[NT][16];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = row0 + 8 * nt + g;
-    const bool ok = r < n_rows;
-    const int tq = SPARSE ? tok0 : r / G, h = SPARSE ? r : r % G;
-    const __nv_bfloat16* qp = p.q + ((int64_t)(q0 + tq) * p.Hq + kvh * G + h) * ATT_D + 32 * t;
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      uint4 w = make_uint4(0u, 0u, 0u, 0u);
-      if (ok) w = *reinterpret_cast<const uint4*>(qp + 8 * i);
-      const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+      const uint32_t ww[4] = {qr[nt][i].x, qr[nt][i].y, qr[nt][i].z, qr[nt][i].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) qf[nt][4 * i + e] = pack_half2(bf16_lo(ww[e]) * p.scale_log2, bf16_hi(ww[e]) * p.scale_log2);
     }
-  }
   // last visible key of this lane's columns 2t, 2t + 1 of every n-tile
   int pos[NT][2];
 #pragma unroll
@@ -284,10 +329,13 @@ attn4_kernel(const Attn4Params p) {
   }
   bool fresh = true;  // some row has seen no key yet
 
-  // ---- a pair of pages at a time: their chains of dependent MMAs run side by side ----
-  bool fail = false;
+  int part = -1;  // where this warp's part goes; none without a page
   int used = 0;
-  for (; used < mine; ++used) {
+  for (int page = it.p0 + 2 * warp; page < it.page_end; page += 2 * WARPS, ++used) {
+    if (parts_read) cp_async_wait<STAGES - 1>();
+    else cp_async_wait<STAGES - 2>();  // one group fewer is out
+    __syncwarp();
+    const uint8_t* st[2] = {ring + get * A4_PAIR, ring + get * A4_PAIR + DASER_KV4_RECORD};
     int key0[2];
     if (SPARSE) {
       // fetches run less than a window ahead: when a use enters window k, the fetches' next window is k + 1
@@ -299,16 +347,12 @@ attn4_kernel(const Attn4Params p) {
       key0[0] = __shfl_sync(0xffffffffu, use_cur, e);
       key0[1] = __shfl_sync(0xffffffffu, use_cur, e + 1);
     } else {
-      key0[0] = page_begin + 2 * (warp + used * A4_WARPS);
-      key0[1] = key0[0] + 1 < page_end ? key0[0] + 1 : -1;
+      key0[0] = page;
+      key0[1] = page + 1 < it.page_end ? page + 1 : -1;
     }
     // a page that is not there lies beyond every limit: its scores become -inf, its scales 0
     key0[0] = key0[0] < 0 ? 1 << 29 : key0[0] * DASER_KV4_TOKENS;
     key0[1] = key0[1] < 0 ? 1 << 29 : key0[1] * DASER_KV4_TOKENS;
-    const uint8_t* st[2] = {ring + get * A4_PAIR, ring + get * A4_PAIR + DASER_KV4_RECORD};
-    if (!mbar_wait(&s_bar[warp][get], phase, &s_abort)) { fail = true; break; }
-    if (++get == A4_STAGES) { get = 0; phase ^= 1u; }
-    __syncwarp();
     // some key of the pair is hidden from some row (pages are in ascending order)
     const bool special = max(key0[0], key0[1]) + DASER_KV4_TOKENS - 1 > first_pos;
     // ---- S^T - base = K Q^T - base: the tensor core takes the difference ----
@@ -432,20 +476,23 @@ attn4_kernel(const Attn4Params p) {
         }
       }
     }
-    __syncwarp();  // every lane is done with this stage before it is filled again
-    if (fetched < mine) fetch(fetched++);
-  }
-  if (fail) {
-    // give the copies in flight their own bounded wait before the shared memory goes away (`get` is the one that gave up)
-    for (int i = used + 1; i < fetched; ++i) {
-      if (++get == A4_STAGES) { get = 0; phase ^= 1u; }
-      uint32_t none = 0u;
-      mbar_wait(&s_bar[warp][get], phase, &none);
+    __syncwarp();  // every lane is done with this stage
+    part = C::IN_RING ? (warp * STAGES + get) * A4_PAIR : C::RING + warp * C::PART;
+    get = get == STAGES - 1 ? 0 : get + 1;
+    if (!parts_read) {
+      __syncthreads();  // the stage that held this warp's part, and what was said about it, are free
+      parts_read = true;
+      fetch(STAGES - 1);
     }
-    if (lane == 0) atomicOr(&g_attn4_status, 1u);
+    if (page + 2 * WARPS < it.page_end) fetch(used + STAGES);
+  }
+  if (!parts_read) {
+    __syncthreads();
+    parts_read = true;
+    fetch(STAGES - 1);
   }
 
-  // ---- merge the warps: O in shared memory over the rings ----
+  // ---- put the warps' parts together ----
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -453,39 +500,50 @@ attn4_kernel(const Attn4Params p) {
       l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 4);
       l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 8);
       l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
+      const int r = 8 * nt + 2 * t + e;
       if (g == 0) {
-        s_m[warp][8 * nt + 2 * t + e] = l[nt][e] == 0.f ? -INFINITY : base[nt][e];
-        s_l[warp][8 * nt + 2 * t + e] = l[nt][e];
+        s_m[warp][r] = l[nt][e] == 0.f ? -INFINITY : base[nt][e];
+        s_l[warp][r] = l[nt][e];
       }
-    }
-  if (__syncthreads_or(fail)) return;  // (the output of this launch is void; the status word says so)
-  float* buf = reinterpret_cast<float*>(a4_smem);  // [warp][row][A4_OPITCH]: every record has been used
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float* dst = buf + (warp * ROWS + 8 * nt + 2 * t + e) * A4_OPITCH + 16 * g;
+      float* dst = reinterpret_cast<float*>(a4_smem + max(part, 0)) + r * A4_OPITCH + 16 * g;
 #pragma unroll
       for (int j = 0; j < 8; j += 2)
-        *reinterpret_cast<float4*>(dst + 2 * j) = make_float4(o[nt][j][e], o[nt][j][2 + e], o[nt][j + 1][e], o[nt][j + 1][2 + e]);
+        if (part >= 0) *reinterpret_cast<float4*>(dst + 2 * j) = make_float4(o[nt][j][e], o[nt][j][2 + e], o[nt][j + 1][e], o[nt][j + 1][2 + e]);
     }
-  __syncthreads();
-  const bool whole = p0 == 0 && p1 == n_item;
-  const int64_t slot = ((int64_t)blockIdx.x * 2 + (p0 == 0 ? 1 : 0)) * ROWS;  // of a partial: 0 continues an item, 1 begins one
+  if (lane == 0) s_part[warp] = part;
+  const bool begins = it.p0 == 0, whole = begins && it.p1 == it.n_item;
+  const int64_t slot = ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * ROWS;  // of a partial: 0 continues an item, 1 begins one
+  if (p.workers && begins && threadIdx.x == 0) {
+    // who has the rest of the item: the owner of its last page is the last
+    const int64_t id = SPARSE ? (int64_t)(q0 + tok0) * p.Hkv + kvh : ((int64_t)it.seq * p.tiles + it.tile) * p.Hkv + kvh;
+    const int n = whole ? 1 : owner_of(it.at + it.n_item - 1, it.T, p.workers) - (int)blockIdx.x + 1;
+    p.shared[id] = make_int2((int)blockIdx.x, n);
+  }
+  // ---- the next item: its first pages, but for the stage that holds this warp's part ----
+  cp_async_wait<0>();  // (groups that were empty)
+  more = it.next(p);
+  put = get;
+  if (more) {
+    first_windows();
 #pragma unroll
-  for (int r = warp; r < ROWS; r += A4_WARPS) {  // a warp finishes a row, a lane four dims
+    for (int i = 0; i < STAGES - 1; ++i) fetch(i);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = warp; r < ROWS; r += WARPS) {  // a warp finishes a row, a lane four dims
     const int row = row0 + r;
     if (row >= n_rows) break;
     float mx = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < A4_WARPS; ++w) mx = fmaxf(mx, s_m[w][r]);
+    for (int w = 0; w < WARPS; ++w) mx = fmaxf(mx, s_m[w][r]);
     const float ref = mx == -INFINITY ? 0.f : mx;
     float lt = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < A4_WARPS; ++w) {
-      const float f = s_m[w][r] == -INFINITY ? 0.f : ex2f(s_m[w][r] - ref);
-      const float4 v = *reinterpret_cast<const float4*>(buf + (w * ROWS + r) * A4_OPITCH + 4 * lane);
+    for (int w = 0; w < WARPS; ++w) {
+      if (s_m[w][r] == -INFINITY) continue;  // saw no key: its part may not even be there
+      const float f = ex2f(s_m[w][r] - ref);
+      const float4 v = *reinterpret_cast<const float4*>(a4_smem + s_part[w] + (r * A4_OPITCH + 4 * lane) * 4);
       lt += f * s_l[w][r];
       acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
     }
@@ -501,75 +559,59 @@ attn4_kernel(const Attn4Params p) {
       if (lane == 0) p.part_lse[slot + r] = lt > 0.f ? mx + log2f(lt) : (lt == 0.f ? -INFINITY : lt);
     }
   }
-  // ---- the next item ----
-  todo -= p1 - p0;
-  if (todo > 0) {
-    p0 = 0;
-    if (++kvh == p.Hkv) {
-      kvh = 0;
-      ++tile;
-      if (SPARSE ? tile >= si.q_len : tile * ROWS >= si.q_len * G) {
-        tile = 0;
-        // (pages are left, so a sequence with queries is)
-        do si = seq_info(p, ++seq);
-        while (si.q_len == 0 && seq + 1 < p.num_seqs);
-      }
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the rings are written by copies again
-    __syncthreads();
-  }
-  }
+  if (more) load_q();
+  parts_read = false;  // warps that finish no row go on with the next item
+  } while (more);
 }
 
 // out = sum_i w_i O_i / sum_i w_i, w_i = 2^(lse_i - max): one CTA per output row.  The weights are made once, then its warps
 // take the partials in turn, eight loads in flight each: a few rows with many partials (one long sequence on one KV head) are
 // a matter of latency.  The order of the sums is fixed.
 // ROWS > 0: the partials of the CTAs that share the pages (attn4_kernel with tiles of ROWS rows): the first is the
-// begun item of its CTA, the others continue it.  ROWS = 0: nsplit partials per row (the prefill kernel).
-constexpr int MERGE_WARPS = 8;
-constexpr int MERGE_MAX = 512;
+// begun item of its CTA, the others continue it; grid (KV head, sequence, row) or (KV head, query row, head).
+// ROWS = 0: nsplit partials per row (the prefill kernel); grid (row).
+constexpr int MERGE_WARPS = 4;
+constexpr int MERGE_MAX = 256;
 template <int ROWS, bool SPARSE>
 __global__ void __launch_bounds__(MERGE_WARPS * 32)
 attn4_merge_kernel(const Attn4Params p) {
   __shared__ float s_w[MERGE_MAX];
   __shared__ float s_max[MERGE_WARPS], s_sum[MERGE_WARPS];
   __shared__ __align__(16) float s_o[MERGE_WARPS][ATT_D];
-  const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_enter();
-  const int tok = (int)(row / p.Hq), hq = (int)(row % p.Hq);
-  if (tok >= p.q_start[p.num_seqs]) return;  // a row behind the last sequence: nobody wrote its partials
   int n;             // partials
   int64_t at0, at1;  // where the first and the second of them are
   int64_t step;      // from one to the next, from the second on
+  int64_t row;       // of the output
   if constexpr (ROWS > 0) {
-    // the row's sequence: as many end at or before it
-    int seq = 0;
-    for (int s = lane; s < p.num_seqs; s += 32) seq += p.q_start[s + 1] <= tok;
-    seq = __reduce_add_sync(0xffffffffu, seq);
-    const SeqInfo si = seq_info(p, seq);
-    const int64_t before = pages_below<ROWS, SPARSE>(p, seq), T = pages_below<ROWS, SPARSE>(p, p.num_seqs);
-    const int kvh = hq / p.G, off = tok - si.q0;
-    const int in_seq = SPARSE ? hq % p.G : off * p.G + hq % p.G;  // row among the sequence's rows of this KV head
-    const int tile = SPARSE ? off : in_seq / ROWS, r = SPARSE ? in_seq : in_seq % ROWS;
-    int64_t begin = before;
-    int pages = p.n_pages;
+    const int kvh = blockIdx.x;
+    int r;
+    int64_t id;
     if (SPARSE) {
-      begin += ((int64_t)tile * p.Hkv + kvh) * p.n_pages;
+      const int tok = blockIdx.y;
+      r = blockIdx.z;
+      if (tok >= p.q_start[p.num_seqs]) return;  // behind the last sequence
+      id = (int64_t)tok * p.Hkv + kvh;
+      row = (int64_t)tok * p.Hq + kvh * p.G + r;
     } else {
-      for (int x = 0; x <= tile; ++x) {
-        pages = max(1, item_pages(p, item_limit(si.q_len, si.q_all, si.ctx, p.G, x * ROWS, ROWS)));
-        if (x < tile) begin += (int64_t)pages * p.Hkv;
-      }
-      begin += (int64_t)kvh * pages;
+      const int seq = blockIdx.y, in_seq = blockIdx.z;
+      const int q0 = p.q_start[seq], q1 = min(p.q_start[seq + 1], p.total_q);
+      const int tok = in_seq / p.G;
+      if (q0 < 0 || q0 + tok >= q1) return;
+      r = in_seq % ROWS;
+      id = ((int64_t)seq * p.tiles + in_seq / ROWS) * p.Hkv + kvh;
+      row = (int64_t)(q0 + tok) * p.Hq + kvh * p.G + in_seq % p.G;
     }
-    const int c0 = owner_of(begin, T, p.workers), c1 = owner_of(begin + pages - 1, T, p.workers);
-    n = c1 - c0 + 1;
+    const int2 s = p.shared[id];
+    n = s.y;
     if (n == 1) return;  // one CTA had it all and wrote the result
-    at0 = ((int64_t)c0 * 2 + 1) * ROWS + r;
-    at1 = (int64_t)(c0 + 1) * 2 * ROWS + r;
+    at0 = ((int64_t)s.x * 2 + 1) * ROWS + r;
+    at1 = (int64_t)(s.x + 1) * 2 * ROWS + r;
     step = 2 * ROWS;
   } else {
+    row = blockIdx.x;
+    if (row >= (int64_t)p.q_start[p.num_seqs] * p.Hq) return;  // behind the last sequence: nobody wrote its partials
     n = p.nsplit;
     at0 = row * n;
     at1 = at0 + 1;
@@ -617,38 +659,40 @@ attn4_merge_kernel(const Attn4Params p) {
   }
   *reinterpret_cast<float4*>(&s_o[warp][4 * lane]) = acc;
   __syncthreads();
-  if (tid < ATT_D) {
-    float total = 0.f, v = 0.f;
+  float total = 0.f, v = 0.f;
 #pragma unroll
-    for (int w = 0; w < MERGE_WARPS; ++w) {
-      total += s_sum[w];
-      v += s_o[w][tid];
-    }
-    p.out[row * ATT_D + tid] = __float2bfloat16(total == 0.f ? 0.f : v / total);  // no key: zeros
+  for (int w = 0; w < MERGE_WARPS; ++w) {
+    total += s_sum[w];
+    v += s_o[w][tid];
   }
+  p.out[row * ATT_D + tid] = __float2bfloat16(total == 0.f ? 0.f : v / total);  // no key: zeros
 }
 
 template <int ROWS, bool SPARSE>
-static int launch_merge(const Attn4Params& p, cudaStream_t stream) {
-  return (int)launch_pdl(attn4_merge_kernel<ROWS, SPARSE>, dim3((unsigned)(p.total_q * p.Hq)), dim3(MERGE_WARPS * 32), 0, stream, p);
+static int launch_merge(const Attn4Params& p, int max_q_len, cudaStream_t stream) {
+  const dim3 grid = ROWS == 0 ? dim3((unsigned)(p.total_q * p.Hq))
+                    : SPARSE  ? dim3((unsigned)p.Hkv, (unsigned)p.total_q, (unsigned)p.G)
+                              : dim3((unsigned)p.Hkv, (unsigned)p.num_seqs, (unsigned)(max_q_len * p.G));
+  return (int)launch_pdl(attn4_merge_kernel<ROWS, SPARSE>, grid, dim3(MERGE_WARPS * 32), 0, stream, p);
 }
 
 template <int NT, bool SPARSE>
-static int launch_attn4(const Attn4Params& p, int tiles, cudaStream_t stream) {
+static int launch_attn4(Attn4Params& p, int max_q_len, cudaStream_t stream) {
+  using C = A4<NT>;
   static bool configured[DASER_MAX_DEVICES] = {false};  // per device: the attribute is the device's
-  constexpr int smem = A4_WARPS * A4_RING;
-  static_assert(A4_WARPS * 8 * NT * A4_OPITCH * 4 <= smem, "the merge buffer lies over the rings");
+  constexpr int smem = C::SMEM;
   if (daser_first_use_on_device(configured)) {
     cudaError_t e = cudaFuncSetAttribute(attn4_kernel<NT, SPARSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;
   }
-  if (tiles > 65535 || p.num_seqs > 65535) return DASER_ERR_TOO_LARGE;
-  const dim3 grid = p.workers ? dim3((unsigned)p.workers) : dim3(p.Hkv, p.num_seqs, (unsigned)tiles);
-  const int rc = (int)launch_pdl(attn4_kernel<NT, SPARSE>, grid, dim3(A4_WARPS * 32), smem, stream, p);
-  return rc || p.workers == 0 ? rc : launch_merge<8 * NT, SPARSE>(p, stream);
+  p.tiles = SPARSE ? max_q_len : (max_q_len * p.G + C::ROWS - 1) / C::ROWS;
+  if (p.tiles > 65535 || p.num_seqs > 65535 || (SPARSE && p.total_q > 65535)) return DASER_ERR_TOO_LARGE;
+  const dim3 grid = p.workers ? dim3((unsigned)p.workers) : dim3((unsigned)p.Hkv, (unsigned)p.num_seqs, (unsigned)p.tiles);
+  const int rc = (int)launch_pdl(attn4_kernel<NT, SPARSE>, grid, dim3(C::WARPS * 32), smem, stream, p);
+  return rc || p.workers == 0 ? rc : launch_merge<C::ROWS, SPARSE>(p, max_q_len, stream);
 }
 
-static int fill_attn4(Attn4Params& p, const void* q, void* out, float* part_o, float* part_lse, const DaserKV4Pool* pool, int layer,
+static int fill_attn4(Attn4Params& p, const void* q, void* out, float* part_o, float* part_lse, void* shared, const DaserKV4Pool* pool, int layer,
                       int rank, const int32_t* block_tables, int max_blocks, const int32_t* q_start, const int32_t* ctx_lens,
                       int num_seqs, int total_q, int max_q_len, int Hq, int parts, float softmax_scale) {
   if (int e = kv4_check_pool(pool, layer, rank)) return e;
@@ -662,6 +706,8 @@ static int fill_attn4(Attn4Params& p, const void* q, void* out, float* part_o, f
   p.out = (__nv_bfloat16*)out;
   p.part_o = part_o;
   p.part_lse = part_lse;
+  p.shared = (int2*)shared;
+  p.tiles = 0;
   p.records = pool->records[rank] + (int64_t)layer * pool->stride_layer;
   p.stride_block = pool->stride_block;
   p.stride_head = pool->stride_head;
@@ -691,16 +737,17 @@ static int fill_attn4(Attn4Params& p, const void* q, void* out, float* part_o, f
 
 // Causal paged attention over the 4-bit pool.
 // Fewer than A4_TC_MIN_ROWS query rows per KV head (max_q_len * heads per KV head): parts is the number of CTAs that share the pages
-// (0: one CTA per item, no scratch); part_o / part_lse: parts * 2 * 16 partials of 128 floats / one float.
+// (0: one CTA per item, no scratch); part_o / part_lse: parts * 2 * 16 partials of 128 floats / one float; shared: two
+// ints per (sequence, tile of 8 rows, KV head), sparse per (query row, KV head).
 // Else parts is the number of splits per context, of split_pages pages (parts * split_pages has to cover the longest
 // context); scratch for total_q * Hq * parts partials when parts > 1.
-DASER_API int daser_paged_attention_kv4(const void* q, void* out, float* part_o, float* part_lse, const DaserKV4Pool* pool, int layer,
+DASER_API int daser_paged_attention_kv4(const void* q, void* out, float* part_o, float* part_lse, void* shared, const DaserKV4Pool* pool, int layer,
                                         int rank, const int32_t* block_tables, int max_blocks, const int32_t* q_start,
                                         const int32_t* ctx_lens, int num_seqs, int total_q, int max_q_len, int Hq, int parts,
                                         int split_pages, float softmax_scale, cudaStream_t stream) {
   using namespace daser;
   Attn4Params p;
-  if (int e = fill_attn4(p, q, out, part_o, part_lse, pool, layer, rank, block_tables, max_blocks, q_start, ctx_lens, num_seqs, total_q,
+  if (int e = fill_attn4(p, q, out, part_o, part_lse, shared, pool, layer, rank, block_tables, max_blocks, q_start, ctx_lens, num_seqs, total_q,
                          max_q_len, Hq, parts, softmax_scale))
     return e;
   const int64_t rows = (int64_t)max_q_len * p.G;
@@ -711,21 +758,22 @@ DASER_API int daser_paged_attention_kv4(const void* q, void* out, float* part_o,
     p.nsplit = parts;
     p.split_pages = split_pages;
     const int rc = daser_launch_attention4_tc(p, max_q_len, stream);
-    return rc || parts == 1 ? rc : launch_merge<0, false>(p, stream);
+    return rc || parts == 1 ? rc : launch_merge<0, false>(p, 0, stream);
   }
   p.workers = parts;
-  return rows <= 8 ? launch_attn4<1, false>(p, 1, stream) : launch_attn4<2, false>(p, (int)((rows + 15) / 16), stream);
+  if (parts && !shared) return DASER_ERR_BAD_ARG;
+  return rows <= 8 ? launch_attn4<1, false>(p, max_q_len, stream) : launch_attn4<2, false>(p, max_q_len, stream);
 }
 
 // The same over the pages listed for every (query row, KV head): pages int32 [total_q][Hkv][n_pages], ascending, -1 behind the last.
 // workers as parts above.
-DASER_API int daser_sparse_attention_kv4(const void* q, void* out, float* part_o, float* part_lse, const DaserKV4Pool* pool, int layer,
+DASER_API int daser_sparse_attention_kv4(const void* q, void* out, float* part_o, float* part_lse, void* shared, const DaserKV4Pool* pool, int layer,
                                          int rank, const int32_t* block_tables, int max_blocks, const int32_t* q_start,
                                          const int32_t* ctx_lens, int num_seqs, int total_q, int max_q_len, int Hq,
                                          const int32_t* pages, int n_pages, int workers, float softmax_scale, cudaStream_t stream) {
   using namespace daser;
   Attn4Params p;
-  if (int e = fill_attn4(p, q, out, part_o, part_lse, pool, layer, rank, block_tables, max_blocks, q_start, ctx_lens, num_seqs, total_q,
+  if (int e = fill_attn4(p, q, out, part_o, part_lse, shared, pool, layer, rank, block_tables, max_blocks, q_start, ctx_lens, num_seqs, total_q,
                          max_q_len, Hq, workers, softmax_scale))
     return e;
   if (n_pages < 1 || workers == 1) return DASER_ERR_BAD_ARG;
@@ -734,13 +782,6 @@ DASER_API int daser_sparse_attention_kv4(const void* q, void* out, float* part_o
   p.pages = pages;
   p.n_pages = n_pages;
   p.workers = workers;
+  if (workers && !shared) return DASER_ERR_BAD_ARG;
   return p.G <= 8 ? launch_attn4<1, true>(p, max_q_len, stream) : launch_attn4<2, true>(p, max_q_len, stream);
-}
-
-// Non-zero once any CTA of the 4-bit decode kernels gave up on a bounded wait (synchronises the device).
-DASER_API int daser_attention4_status(uint32_t* out) {
-  uint32_t v = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&v, daser::g_attn4_status, sizeof(v));
-  if (out) *out = v;
-  return (int)e;
 }

@@ -11,6 +11,7 @@ struct Attn4Params {
   __nv_bfloat16* out;           // [Tq, Hq, 128]
   float* part_o;                // partial outputs, 128 floats each, normalised ...
   float* part_lse;              // ... and their log2-sum-exp (where they lie: attention4.cu)
+  int2* shared;                 // decode: of every item, the first CTA that has a part of it, and how many have
   const uint8_t* records;       // the layer's records
   int64_t stride_block, stride_head;
   const int32_t* block_tables;  // [num_seqs, max_blocks]
@@ -20,6 +21,7 @@ struct Attn4Params {
   int max_blocks, num_blocks, num_seqs, Hq, Hkv, G;
   int n_pages;                  // sparse: pages listed per (query row, KV head)
   int workers;                  // decode: CTAs that share all pages evenly, 0 = one CTA per item
+  int tiles;                    // decode: row tiles of the longest query block
   int nsplit, split_pages;      // prefill: splits of a context, of split_pages pages each
   float scale_log2;             // softmax scale * log2(e)
   int total_q;

@@ -327,7 +327,7 @@ def _attend(pool, layer, tables, q, start, ctx_lens, max_q, hkv, split=None, ws=
     ([1, 1, 1], [0, 20, 0], 8, 2, None),                     # no keys at all: zeros
     ([4], [2], 8, 2, None),                                  # the first rows see no key
     ([1], [9000], 8, 1, 0),                                  # 71 pages a warp: the page windows turn over twice
-    ([1], [9000], 8, 1, 300),                                # CTAs with less than a page a warp
+    ([1], [9000], 8, 1, 200),                                # CTAs with less than a page a warp
     ([1, 0, 1, 2], [0, 0, 1700, 5], 4, 2, 50),               # items without keys between shared ones
     ([1] * 40, list(range(3, 1203, 30)), 8, 1, 31),          # more sequences than a warp has lanes
 ])

@@ -176,8 +176,8 @@ def test_c_entry_points_refuse_bad_pools(change, code):
     assert _lib.kv4_fn("daser_kv4_read")(p, 0, 0, a, a, a, 1, None) == code
     assert _lib.kv4_fn("daser_rope_kv4_write")(a, 1, 1536, a, a, a, 8, a, 1, 8, 2, p, 0, 0, 0, None, None, 0.0, None) == code
     assert _lib.kv4_fn("daser_kv4_page_bounds")(p, 0, 0, a, a, a, 4, a, a, 1, 1, None) == code
-    assert _lib.kv4_fn("daser_paged_attention_kv4")(a, a, a, a, p, 0, 0, a, 4, a, a, 1, 1, 1, 8, 1, 4, 1.0, None) == code
-    assert _lib.kv4_fn("daser_sparse_attention_kv4")(a, a, a, a, p, 0, 0, a, 4, a, a, 1, 1, 1, 8, a, 4, 2, 1.0, None) == code
+    assert _lib.kv4_fn("daser_paged_attention_kv4")(a, a, a, a, a, p, 0, 0, a, 4, a, a, 1, 1, 1, 8, 1, 4, 1.0, None) == code
+    assert _lib.kv4_fn("daser_sparse_attention_kv4")(a, a, a, a, a, p, 0, 0, a, 4, a, a, 1, 1, 1, 8, a, 4, 2, 1.0, None) == code
 
 
 def test_c_entry_points_refuse_bad_arguments():
@@ -195,16 +195,17 @@ def test_c_entry_points_refuse_bad_arguments():
         args = list(ok)
         args[at] = bad
         assert write(*args) == code, at
-    ok = [a, a, a, a, p, 0, 0, a, 4, a, a, 1, 1, 1, 8, 2, 4, 1.0, None]
-    for at, bad, code in ((14, 7, -1), (14, 34, -2), (15, 1, -1), (15, -1, -1), (15, 513, -3), (2, None, -1), (8, 0, -1), (0, a + 2, -2), (11, -1, -1)):
+    ok = [a, a, a, a, a, p, 0, 0, a, 4, a, a, 1, 1, 1, 8, 2, 4, 1.0, None]
+    for at, bad, code in ((15, 7, -1), (15, 34, -2), (16, 1, -1), (16, -1, -1), (16, 257, -3), (2, None, -1), (4, None, -1), (9, 0, -1),
+                          (0, a + 2, -2), (12, -1, -1)):
         args = list(ok)
         args[at] = bad
         assert att(*args) == code, at
     sparse = _lib.kv4_fn("daser_sparse_attention_kv4")
-    assert sparse(a, a, a, a, p, 0, 0, a, 4, a, a, 1, 1, 1, 8, a, 9, 1, 1.0, None) == -1  # one CTA has nothing to share
-    assert sparse(a, a, a, a, p, 0, 0, a, 4, a, a, 1, 1, 1, 8, a, 0, 2, 1.0, None) == -1
-    prefill = [a, a, a, a, p, 0, 0, a, 4, a, a, 1, 64, 64, 8, 2, 4, 1.0, None]  # 4 heads x 64 queries: splits
-    for at, bad in ((15, 0), (16, 0)):
+    assert sparse(a, a, a, a, a, p, 0, 0, a, 4, a, a, 1, 1, 1, 8, a, 9, 1, 1.0, None) == -1  # one CTA has nothing to share
+    assert sparse(a, a, a, a, a, p, 0, 0, a, 4, a, a, 1, 1, 1, 8, a, 0, 2, 1.0, None) == -1
+    prefill = [a, a, a, a, None, p, 0, 0, a, 4, a, a, 1, 64, 64, 8, 2, 4, 1.0, None]  # 4 heads x 64 queries: splits
+    for at, bad in ((16, 0), (17, 0)):
         args = list(prefill)
         args[at] = bad
         assert att(*args) == -1, at
@@ -216,7 +217,7 @@ def test_c_entry_points_refuse_bad_arguments():
         assert sel(*args) == code, at
     # nothing to do is not an error, and launches nothing
     assert read(p, 0, 0, None, None, None, 0, None) == 0
-    assert att(a, a, None, None, p, 0, 0, a, 4, a, a, 0, 0, 0, 8, 0, 0, 1.0, None) == 0
+    assert att(a, a, None, None, None, p, 0, 0, a, 4, a, a, 0, 0, 0, 8, 0, 0, 1.0, None) == 0
 
 
 def test_plans_cover_the_context():
@@ -232,7 +233,7 @@ def test_plans_cover_the_context():
                         assert n == 1 or (n - 1) * per < pages  # no split is empty for the longest context
                         assert n == 1 or n * seqs * q * heads * group <= attention.MAX_ROW_SPLITS
                     else:
-                        assert n == 0 or 2 <= n <= 296
+                        assert n == 0 or 2 <= n <= 148
 
 
 def test_outgrown_workspace_buffers_stay_alive():
