@@ -88,9 +88,9 @@ def plan_kv4(num_seqs: int, kv_heads: int, max_q_len: int, group: int, max_pages
     pages evenly, 0 for one CTA per (sequence, row tile, KV head) and no merge."""
     max_pages = max(1, max_pages)
     if max_q_len * group >= TC_MIN_ROWS:
-        # a CTA of 128 query rows, two per SM, tiles of four pages; splits of two tiles at the shortest
-        items = num_seqs * kv_heads * -(-max_q_len // (128 // group))
-        nsplit = max(1, min((NUM_SMS * 2) // max(items, 1), -(-max_pages // 8), 64))
+        # a CTA of two tiles of 128 query rows, one per SM, tiles of four pages; splits of two tiles at the shortest
+        items = num_seqs * kv_heads * -(-max_q_len // (2 * (128 // group)))
+        nsplit = max(1, min(NUM_SMS // max(items, 1), -(-max_pages // 8), 64))
         if rows > 0:
             nsplit = max(1, min(nsplit, MAX_ROW_SPLITS // rows))
         per = -(--(-max_pages // nsplit) // 4) * 4

@@ -1,15 +1,15 @@
 // Chunked-prefill attention over the 4-bit pool on the 5th-generation tensor cores (tcgen05 + TMEM).
 //
-// The same organisation as attention_tc.cu (its fp8 counterpart), with records instead of scattered rows:
-//   * one CTA = 128 / G query tokens x the G heads of one KV head, and one range of pages (split-KV, merged by
-//     attn4_merge_kernel); tiles of 64 keys;
-//   * a tile is four bulk copies of 2304 bytes, two tiles ahead of their use;
-//   * all threads dequantise it to f16 (exact) in the 128-byte-swizzled K-major layout of the MMA descriptors: K as
-//     [key][dim], V transposed to [dim][key].  V's codes of two neighbouring tokens are interleaved nibble by nibble, so that one
-//     conversion yields the two neighbours of a V^T row;
-//   * S = Q K^T and O += P V are tcgen05.mma with the accumulators in TMEM; a thread owns one row of S, so the softmax needs no
-//     shuffles; P = 2^(S - m) is f16, a column of ones in V^T sums it, and O is rescaled only when the maximum rises by more
-//     than 2^8.
+// One CTA per SM works on two tiles of 128 query rows (128 / G query tokens x the G heads of one KV head, each) against tiles of 64 keys, so
+// that a tile of keys is dequantised once for 256 rows and one row tile's softmax runs under the other's MMAs.  14 warps:
+//   * 0-3, 4-7   softmax of row tile 0, 1: a thread owns a row of S (tcgen05.ld 32x32b), takes it into registers and frees it at once,
+//                so that the next S is under way while P = 2^(S - m) is made: f16, into shared memory, as the MMA operand.  The running
+//                maximum m is raised only when a tile exceeds it by 2^8, and only then is O rescaled (tcgen05.ld / st);
+//   * 8-11       dequantise: K as [key][dim], V transposed to [dim][key], f16 (exact), in the 128-byte-swizzled K-major layout of the
+//                MMA descriptors, two buffers each.  V's codes of two neighbouring tokens are interleaved nibble by nibble, so that
+//                one conversion yields the two neighbours of a V^T row.  A row of ones in V^T sums the rows of the P that was multiplied;
+//   * 12         issues the MMAs, S0(i), O0 += P0(i-1) V(i-1), S1(i), O1 += P1(i-1) V(i-1): M 128, N 64, K 128 and M 128, N 144, K 64;
+//   * 13         fetches: a tile is four bulk copies of 2304 bytes, three tiles ahead.
 // Every mbarrier wait is bounded; on expiry the CTA records it in a status word, frees its TMEM and returns.
 #include "attention4_params.cuh"
 
@@ -21,27 +21,34 @@ constexpr int T4_PAGES = T4_NK / DASER_KV4_TOKENS;
 constexpr int T4_PITCH = DASER_KV4_RECORD + 16;         // of a page in shared memory: pages start on other banks
 constexpr int T4_RAW = T4_PAGES * T4_PITCH;
 constexpr int T4_STAGES = 3;
-constexpr int T4_Q_BYTES = 128 * ATT_D * 2;             // two sub-tiles [128 rows][64 dims]
-constexpr int T4_KP_BYTES = 16384;                      // K: two sub-tiles [64 keys][64 dims]; later P: [128 rows][64 keys]
+constexpr int T4_Q_BYTES = 128 * ATT_D * 2;             // of a row tile: two sub-tiles [128 rows][64 dims]
+constexpr int T4_K_BYTES = T4_NK * ATT_D * 2;           // two sub-tiles [64 keys][64 dims]
+constexpr int T4_P_BYTES = 128 * T4_NK * 2;             // [128 rows][64 keys]
 constexpr int T4_ON = ATT_D + 16;                       // output columns: 128 dims, the row sum, 15 unused
 constexpr int T4_VT_BYTES = T4_ON * 128;
-constexpr int T4_SMEM = 1024 + T4_Q_BYTES + T4_KP_BYTES + T4_VT_BYTES + T4_STAGES * T4_RAW + 128;
-constexpr uint32_t T4_TMEM_COLS = 256;                  // S in columns [0, 64), O in [64, 208)
-constexpr uint32_t T4_O_COL = 64;
+constexpr int T4_THREADS = 14 * 32;
+constexpr int T4_SMEM = 1024 + 2 * T4_Q_BYTES + 2 * T4_K_BYTES + 2 * T4_VT_BYTES + 2 * T4_P_BYTES + T4_STAGES * T4_RAW;
+constexpr uint32_t T4_TMEM_COLS = 512;                  // S of tile t in columns [64 t, 64 t + 64), O in [128 + 192 t, + 144)
 constexpr float T4_RAISE_AT = 8.f;
 
 __device__ uint32_t g_attn4_tc_status = 0;  // bit 0: a bounded wait ran out
 
 __device__ __forceinline__ void t4_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void t4_tmem_st(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void t4_tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {  // 32 lanes x 16 columns
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
-        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void t4_tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void t4_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -59,32 +66,44 @@ __device__ __forceinline__ void t4_bulk_load(uint32_t dst, const void* src, uint
                : "memory");
 }
 
-__global__ void __launch_bounds__(128, 2)
-attn4_tc_kernel(const Attn4Params p) {
+// The whole warp waits; one answer for all lanes, so that they leave a loop together.
+__device__ __forceinline__ bool t4_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+
+struct T4Bars {
+  uint64_t raw_full[T4_STAGES], raw_free[T4_STAGES];
+  uint64_t k_ready[2], k_free[2], v_ready[2], v_free[2];  // by buffer
+  uint64_t s_ready[2], s_free[2], p_ready[2], o_done[2];  // by row tile
+  uint64_t q_ready, drain;
+  uint32_t tmem, abort;
+};
+
+__global__ void __launch_bounds__(T4_THREADS, 1)
+attn4_tc_kernel(const Attn4Params p, int groups) {
   extern __shared__ uint8_t t4_smem_raw[];
+  __shared__ T4Bars bars;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(t4_smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_s = smem;
-  uint8_t* kp_s = q_s + T4_Q_BYTES;
-  uint8_t* vt_s = kp_s + T4_KP_BYTES;
-  uint8_t* raw_s = vt_s + T4_VT_BYTES;
-  uint64_t* bar_s = reinterpret_cast<uint64_t*>(raw_s + T4_STAGES * T4_RAW);
-  uint64_t* bar_o = bar_s + 1;
-  uint64_t* bar_raw = bar_s + 2;  // [T4_STAGES]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_raw + T4_STAGES);
-  volatile uint32_t* abort_flag = tmem_slot + 1;
+  uint8_t* k_s = q_s + 2 * T4_Q_BYTES;
+  uint8_t* vt_s = k_s + 2 * T4_K_BYTES;
+  uint8_t* p_s = vt_s + 2 * T4_VT_BYTES;
+  uint8_t* raw_s = p_s + 2 * T4_P_BYTES;
+  volatile uint32_t* abort_flag = &bars.abort;
 
-  const int tid = threadIdx.x, warp = tid >> 5;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kvh = blockIdx.x, seq = blockIdx.y;
-  const int grp = blockIdx.z / p.nsplit, sp = blockIdx.z % p.nsplit;
+  const int grp = groups - 1 - (int)(blockIdx.z / p.nsplit), sp = blockIdx.z % p.nsplit;  // the longest first
   pdl_wait();  // launched ahead of its predecessor's end: nothing is read before this returns
   const int q0 = p.q_start[seq];
   const int q_all = p.q_start[seq + 1] - q0;
   const int q_len = min(p.q_start[seq + 1], p.total_q) - q0;
   const int G = p.G;
-  const int toks_per_cta = 128 / G;
-  const int tok0 = grp * toks_per_cta;
+  const int toks = 128 / G;  // of a row tile
+  const int tok0 = grp * 2 * toks;
   if (q0 < 0 || tok0 >= q_len) return;  // uniform over the CTA
-  const int last_tok = min(tok0 + toks_per_cta, q_len) - 1;
+  const int tiles = tok0 + toks < q_len ? 2 : 1;  // live row tiles
+  const int last_tok = min(tok0 + tiles * toks, q_len) - 1;
   const int limit = p.ctx_lens[seq] - q_all + last_tok + 1;  // keys visible to the last row
   const int n_all = limit > 0 ? (min(limit, p.max_blocks * DASER_KV4_TOKENS) + DASER_KV4_TOKENS - 1) / DASER_KV4_TOKENS : 0;
   const int page_begin = sp * p.split_pages;
@@ -92,99 +111,210 @@ attn4_tc_kernel(const Attn4Params p) {
   const int n_tiles = page_begin < page_end ? (page_end - page_begin + T4_PAGES - 1) / T4_PAGES : 0;
   const int key_end = min(page_end * DASER_KV4_TOKENS, limit);
 
-  // this thread's row
-  const int tq = tok0 + tid / G, hq = kvh * G + tid % G;
-  const bool valid = tid < toks_per_cta * G && tq < q_len;
+  // softmax threads: this thread's row
+  const int tile = warp >> 2, rt = tid & 127;
+  const int tq = tok0 + tile * toks + rt / G, hq = kvh * G + rt % G;
+  const bool valid = tile < tiles && rt < toks * G && tq < q_len;
   const int pos = p.ctx_lens[seq] - q_all + tq;  // last key this row may see
   const int64_t row = (int64_t)(q0 + tq) * p.Hq + hq;
 
-  float m = -INFINITY;  // the maximum the accumulated P are relative to
+  if (n_tiles == 0) {  // no keys in this split: an empty partial
+    if (valid) {
+      if (p.nsplit == 1) {
+        __nv_bfloat16* dst = p.out + row * ATT_D;
+#pragma unroll
+        for (int ck = 0; ck < 16; ++ck) *reinterpret_cast<uint4*>(dst + 8 * ck) = make_uint4(0u, 0u, 0u, 0u);
+      } else {
+        float* dst = p.part_o + (row * p.nsplit + sp) * ATT_D;
+#pragma unroll
+        for (int ck = 0; ck < 32; ++ck) *reinterpret_cast<float4*>(dst + 4 * ck) = make_float4(0.f, 0.f, 0.f, 0.f);
+        p.part_lse[row * p.nsplit + sp] = -INFINITY;
+      }
+    }
+    return;
+  }
 
-  if (n_tiles > 0) {
-    const uint32_t q_u32 = smem_u32(q_s), kp_u32 = smem_u32(kp_s), vt_u32 = smem_u32(vt_s), raw_u32 = smem_u32(raw_s);
-    if (tid == 0) {
-      mbar_init(bar_s, 1);
-      mbar_init(bar_o, 1);
+  const uint32_t q_u32 = smem_u32(q_s), k_u32 = smem_u32(k_s), vt_u32 = smem_u32(vt_s), p_u32 = smem_u32(p_s), raw_u32 = smem_u32(raw_s);
+  if (tid == 0) {
 #pragma unroll
-      for (int s = 0; s < T4_STAGES; ++s) mbar_init(bar_raw + s, 1);
-      *abort_flag = 0u;
-      mbar_init_fence();
+    for (int s = 0; s < T4_STAGES; ++s) {
+      mbar_init(&bars.raw_full[s], 1);
+      mbar_init(&bars.raw_free[s], 4);
     }
-    if (warp == 0) {
-      tmem_alloc(tmem_slot, T4_TMEM_COLS);
-      tmem_relinquish();
-    }
-    const int32_t* table = p.block_tables + (int64_t)seq * p.max_blocks;
-    // Thread 0 fetches; block ids are read one tile ahead of the copies that need them.
-    int blk_next[T4_PAGES];
-    auto ids = [&](int ti) {
 #pragma unroll
-      for (int pg = 0; pg < T4_PAGES; ++pg) blk_next[pg] = __ldg(table + min(page_begin + ti * T4_PAGES + pg, p.max_blocks - 1));
-    };
-    auto issue = [&](int ti) {
-      const int n = min(T4_PAGES, page_end - page_begin - ti * T4_PAGES);
-      uint64_t* bar = bar_raw + ti % T4_STAGES;
-      const uint32_t dst = raw_u32 + (ti % T4_STAGES) * T4_RAW;
-      mbar_expect_tx(bar, n * DASER_KV4_RECORD);
-#pragma unroll
-      for (int pg = 0; pg < T4_PAGES; ++pg) {
-        if (pg >= n) break;
-        int blk = blk_next[pg];
-        blk = blk < 0 ? 0 : (blk >= p.num_blocks ? p.num_blocks - 1 : blk);
-        t4_bulk_load(dst + pg * T4_PITCH, p.records + (int64_t)blk * p.stride_block + (int64_t)kvh * p.stride_head, DASER_KV4_RECORD, bar);
-      }
-    };
-    int issued = 0;
-    if (tid == 0) {
-      ids(0);
-      for (; issued < T4_STAGES - 1 && issued < n_tiles; ++issued) {
-        issue(issued);
-        ids(issued + 1);
-      }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&bars.k_ready[b], 4);
+      mbar_init(&bars.k_free[b], 1);
+      mbar_init(&bars.v_ready[b], 4);
+      mbar_init(&bars.v_free[b], 1);
+      mbar_init(&bars.s_ready[b], 1);
+      mbar_init(&bars.s_free[b], 4);
+      mbar_init(&bars.p_ready[b], 4);
+      mbar_init(&bars.o_done[b], 1);
     }
-    {  // Q row -> f16, times scale * log2(e), into the swizzled A tile
-      const __nv_bfloat16* qp = p.q + row * ATT_D;
-#pragma unroll
-      for (int ck = 0; ck < 16; ++ck) {
-        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (valid) w = *reinterpret_cast<const uint4*>(qp + ck * 8);
-        uint4 h;
-        h.x = pack_half2(bf16_lo(w.x) * p.scale_log2, bf16_hi(w.x) * p.scale_log2);
-        h.y = pack_half2(bf16_lo(w.y) * p.scale_log2, bf16_hi(w.y) * p.scale_log2);
-        h.z = pack_half2(bf16_lo(w.z) * p.scale_log2, bf16_hi(w.z) * p.scale_log2);
-        h.w = pack_half2(bf16_lo(w.w) * p.scale_log2, bf16_hi(w.w) * p.scale_log2);
-        *reinterpret_cast<uint4*>(q_s + (ck >> 3) * 16384 + tid * 128 + ((((ck & 7) ^ (tid & 7))) << 4)) = h;
-      }
-    }
-    {  // rows 128..143 of V^T: row 128 all ones (it sums the rows of P), the rest zero
-      const uint32_t v = tid < 8 ? 0x3c003c00u : 0u;
-      *reinterpret_cast<uint4*>(vt_s + ATT_D * 128 + tid * 16) = make_uint4(v, v, v, v);
-    }
-    tc_fence_before();
-    __syncthreads();  // barriers initialised, TMEM address published
-    tc_fence_after();
-    pdl_launch_dependents();  // only now: this CTA holds its tensor memory, a successor cannot take it
-    const uint32_t tmem = *tmem_slot;
-    const uint32_t tmem_row = tmem + ((uint32_t)(warp * 32) << 16);
-    constexpr uint32_t idesc_s = make_idesc_f16(128, T4_NK, 0);
-    constexpr uint32_t idesc_o = make_idesc_f16(128, T4_ON, 0);
-    int fail = 0;
+    mbar_init(&bars.q_ready, 4 * tiles);
+    mbar_init(&bars.drain, 1);
+    bars.abort = 0u;
+    mbar_init_fence();
+  }
+  if (warp == 12) {
+    tmem_alloc(&bars.tmem, T4_TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();  // barriers initialised, TMEM address published
+  tc_fence_after();
+  pdl_launch_dependents();  // only now: this CTA holds its tensor memory, a successor cannot take it
+  const uint32_t tmem = bars.tmem;
+  bool ok = true;
 
-    int ti = 0;
-    for (; ti < n_tiles; ++ti) {
-      if (!mbar_wait(bar_raw + ti % T4_STAGES, (ti / T4_STAGES) & 1, abort_flag)) fail = 1;
-      if (__syncthreads_or(fail)) break;  // K/P and V^T are free (P V of ti - 1 has completed), raw stage ti - 1 has been read
-      if (tid == 0 && issued < n_tiles) {
-        issue(issued++);
-        ids(issued);
+  if (warp < 8) {
+    // ======== softmax ========
+    if (tile < tiles) {
+      const uint32_t tmem_s = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 64u * tile;
+      const uint32_t tmem_o = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128u + 192u * tile;
+      uint8_t* my_q = q_s + tile * T4_Q_BYTES;
+      uint8_t* my_p = p_s + tile * T4_P_BYTES;
+      {  // Q row -> f16, times scale * log2(e), into the swizzled A tile
+        const __nv_bfloat16* qp = p.q + row * ATT_D;
+#pragma unroll
+        for (int ck = 0; ck < 16; ++ck) {
+          uint4 w = make_uint4(0u, 0u, 0u, 0u);
+          if (valid) w = *reinterpret_cast<const uint4*>(qp + ck * 8);
+          uint4 h;
+          h.x = pack_half2(bf16_lo(w.x) * p.scale_log2, bf16_hi(w.x) * p.scale_log2);
+          h.y = pack_half2(bf16_lo(w.y) * p.scale_log2, bf16_hi(w.y) * p.scale_log2);
+          h.z = pack_half2(bf16_lo(w.z) * p.scale_log2, bf16_hi(w.z) * p.scale_log2);
+          h.w = pack_half2(bf16_lo(w.w) * p.scale_log2, bf16_hi(w.w) * p.scale_log2);
+          *reinterpret_cast<uint4*>(my_q + (ck >> 3) * 16384 + rt * 128 + ((((ck & 7) ^ (rt & 7))) << 4)) = h;
+        }
       }
+      t4_fence_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.q_ready);
+
+      float m = -INFINITY;  // the maximum the accumulated P are relative to
+      for (int ti = 0; ti < n_tiles; ++ti) {
+        const int key0 = (page_begin + ti * T4_PAGES) * DASER_KV4_TOKENS;
+        if (!(ok = t4_wait(&bars.s_ready[tile], ti & 1, abort_flag))) break;
+        tc_fence_after();
+        uint32_t sr[2][32];
+        tmem_ld_32x32(tmem_s, sr[0]);
+        tmem_ld_32x32(tmem_s + 32, sr[1]);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.s_free[tile]);
+        if (!(valid && key0 + T4_NK - 1 <= pos && key0 + T4_NK <= key_end)) {
+          // the causal edge or the end of the range runs through this tile
+#pragma unroll
+          for (int j = 0; j < T4_NK; ++j) {
+            const int key = key0 + j;
+            if (!(valid && key < key_end && key <= pos)) sr[j >> 5][j & 31] = 0xff800000u;  // -inf
+          }
+        }
+        float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          mx0 = fmaxf(mx0, __uint_as_float(sr[0][j]));
+          mx1 = fmaxf(mx1, __uint_as_float(sr[1][j]));
+        }
+        const float mx = fmaxf(mx0, mx1);
+        // raise m only when this tile is far above it: P then stays below 2^8, well inside f16
+        const bool raise = mx > m + T4_RAISE_AT || (m == -INFINITY && mx > -INFINITY);
+        // the previous P V has completed: its P may be overwritten, and O may be touched
+        if (ti > 0 && !(ok = t4_wait(&bars.o_done[tile], (ti - 1) & 1, abort_flag))) break;
+        if (ti > 0 && __any_sync(0xffffffffu, raise)) {
+          tc_fence_after();
+          const float alpha = raise ? ex2f(m - mx) : 1.f;
+#pragma unroll
+          for (int cc = 0; cc < 9; ++cc) {
+            uint32_t r[16];
+            t4_tmem_ld16(tmem_o + 16 * cc, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int x = 0; x < 16; ++x) r[x] = __float_as_uint(__uint_as_float(r[x]) * alpha);
+            t4_tmem_st16(tmem_o + 16 * cc, r);
+          }
+          t4_tmem_st_wait();
+        }
+        if (raise) m = mx;
+        const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int ck = 0; ck < 8; ++ck) {
+          uint32_t h[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = ck * 8 + 2 * e;
+            h[e] = t4_ex2_f16x2(__uint_as_float(sr[j >> 5][j & 31]) - base, __uint_as_float(sr[(j + 1) >> 5][(j + 1) & 31]) - base);
+          }
+          *reinterpret_cast<uint4*>(my_p + rt * 128 + ((ck ^ (rt & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        t4_fence_async();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.p_ready[tile]);
+      }
+      if (ok) ok = t4_wait(&bars.o_done[tile], (n_tiles - 1) & 1, abort_flag);
+      tc_fence_after();
+      if (ok) {
+        // ---- O / l from TMEM (column 128 holds l).  The TMEM loads are warp-wide (.sync.aligned): every thread
+        // executes them, only the global stores depend on `valid`.
+        uint32_t r[32];
+        tmem_ld_32x32(tmem_o + ATT_D, r);
+        tmem_ld_wait();
+        const float l = __uint_as_float(r[0]);
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) {
+          __syncwarp();  // reconverge after the predicated stores of the previous chunk
+          tmem_ld_32x32(tmem_o + 32 * cc, r);
+          tmem_ld_wait();
+          if (!valid) continue;
+          if (p.nsplit == 1) {
+            __nv_bfloat16* dst = p.out + row * ATT_D + 32 * cc;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              uint4 w;
+              w.x = pack_bf16x2(__uint_as_float(r[8 * x]) * inv, __uint_as_float(r[8 * x + 1]) * inv);
+              w.y = pack_bf16x2(__uint_as_float(r[8 * x + 2]) * inv, __uint_as_float(r[8 * x + 3]) * inv);
+              w.z = pack_bf16x2(__uint_as_float(r[8 * x + 4]) * inv, __uint_as_float(r[8 * x + 5]) * inv);
+              w.w = pack_bf16x2(__uint_as_float(r[8 * x + 6]) * inv, __uint_as_float(r[8 * x + 7]) * inv);
+              *reinterpret_cast<uint4*>(dst + 8 * x) = w;
+            }
+          } else {
+            float* dst = p.part_o + (row * p.nsplit + sp) * ATT_D + 32 * cc;
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              *reinterpret_cast<float4*>(dst + 4 * x) =
+                  make_float4(__uint_as_float(r[4 * x]) * inv, __uint_as_float(r[4 * x + 1]) * inv,
+                              __uint_as_float(r[4 * x + 2]) * inv, __uint_as_float(r[4 * x + 3]) * inv);
+          }
+        }
+        if (valid && p.nsplit > 1) p.part_lse[row * p.nsplit + sp] = l > 0.f ? m + log2f(l) : (l == 0.f ? -INFINITY : l);
+        __syncwarp();
+      }
+    }
+  } else if (warp < 12) {
+    // ======== dequantise ========
+    const int dt = tid - 256;  // 0 .. 127
+    {  // rows 128..143 of both V^T buffers: row 128 all ones (it sums the rows of P), the rest zero
+      const uint32_t v = dt < 8 ? 0x3c003c00u : 0u;
+      *reinterpret_cast<uint4*>(vt_s + ATT_D * 128 + dt * 16) = make_uint4(v, v, v, v);
+      *reinterpret_cast<uint4*>(vt_s + T4_VT_BYTES + ATT_D * 128 + dt * 16) = make_uint4(v, v, v, v);
+    }
+    for (int ti = 0; ti < n_tiles; ++ti) {
+      const int b = ti & 1;
       const uint8_t* st = raw_s + (ti % T4_STAGES) * T4_RAW;
       const int key0 = (page_begin + ti * T4_PAGES) * DASER_KV4_TOKENS;
-
+      uint8_t* kb = k_s + b * T4_K_BYTES;
+      uint8_t* vb = vt_s + b * T4_VT_BYTES;
+      if (!(ok = t4_wait(&bars.raw_full[ti % T4_STAGES], (ti / T4_STAGES) & 1, abort_flag))) break;
+      if (ti >= 2 && !(ok = t4_wait(&bars.k_free[b], (ti / 2 - 1) & 1, abort_flag))) break;
       // ---- K: (key, 16-dim group) items, four per thread ----
 #pragma unroll
       for (int rep = 0; rep < 4; ++rep) {
-        const int item = tid + 128 * rep;
+        const int item = dt + 128 * rep;
         const int kt = item >> 3, c = item & 7;
         uint32_t h[8];
         if (key0 + kt < key_end) {
@@ -192,25 +322,29 @@ attn4_tc_kernel(const Attn4Params p) {
           const int tok = kt & 15;
           const uint2 w = *reinterpret_cast<const uint2*>(rec + tok * 64 + c * 8);
           const uint32_t sc = (uint32_t)rec[DASER_KV4_KS + tok * 8 + c] * 0x00800080u;  // f16 bits = byte << 7, in both halves
-          uint32_t a[4], b[4];
-          e2m1x8_to_f16x2(w.x, a);
-          e2m1x8_to_f16x2(w.y, b);
+          uint32_t x[4], y[4];
+          e2m1x8_to_f16x2(w.x, x);
+          e2m1x8_to_f16x2(w.y, y);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            h[i] = hmul2_u32(a[i], sc);
-            h[4 + i] = hmul2_u32(b[i], sc);
+            h[i] = hmul2_u32(x[i], sc);
+            h[4 + i] = hmul2_u32(y[i], sc);
           }
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) h[i] = 0u;
         }
-        uint8_t* dst = kp_s + (c >> 2) * 8192 + kt * 128;
+        uint8_t* dst = kb + (c >> 2) * 8192 + kt * 128;
         *reinterpret_cast<uint4*>(dst + (((2 * (c & 3)) ^ (kt & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
         *reinterpret_cast<uint4*>(dst + (((2 * (c & 3) + 1) ^ (kt & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
       }
+      t4_fence_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.k_ready[b]);
+      if (ti >= 2 && !(ok = t4_wait(&bars.v_free[b], (ti / 2 - 1) & 1, abort_flag))) break;
       // ---- V^T: 8 keys x 8 dims per thread ----
       {
-        const int ko = tid & 7, g = tid >> 4, hf = (tid >> 3) & 1;
+        const int ko = dt & 7, g = dt >> 4, hf = (dt >> 3) & 1;
         const uint8_t* rec = st + (ko >> 1) * T4_PITCH;
         const int left = key_end - (key0 + 8 * ko);  // keys of this octet that exist
         uint32_t v[8][4];  // [dim][key pair]
@@ -238,153 +372,95 @@ attn4_tc_kernel(const Attn4Params p) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int d = 16 * g + 8 * hf + j;
-          *reinterpret_cast<uint4*>(vt_s + d * 128 + ((ko ^ j) << 4)) = make_uint4(v[j][0], v[j][1], v[j][2], v[j][3]);
+          *reinterpret_cast<uint4*>(vb + d * 128 + ((ko ^ j) << 4)) = make_uint4(v[j][0], v[j][1], v[j][2], v[j][3]);
         }
       }
       t4_fence_async();
-      tc_fence_before();
-      __syncthreads();
-      if (tid == 0 && !*abort_flag) {
-        tc_fence_after();
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-          const uint64_t da = make_desc_k_sw128(q_u32 + sub * 16384);
-          const uint64_t db = make_desc_k_sw128(kp_u32 + sub * 8192);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) umma_f16(tmem, da + 2 * k, db + 2 * k, idesc_s, (sub | k) ? 1u : 0u);
-        }
-        umma_commit(bar_s);
-      }
-      if (!mbar_wait(bar_s, ti & 1, abort_flag)) fail = 1;
       __syncwarp();
-      tc_fence_after();
-
-      // ---- softmax on this thread's row ----
-      {
-        uint32_t sr[2][32];
-        tmem_ld_32x32(tmem_row, sr[0]);
-        tmem_ld_32x32(tmem_row + 32, sr[1]);
-        tmem_ld_wait();
-        if (!(valid && key0 + T4_NK - 1 <= pos && key0 + T4_NK <= key_end)) {
-          // the causal edge or the end of the range runs through this tile
-#pragma unroll
-          for (int j = 0; j < T4_NK; ++j) {
-            const int key = key0 + j;
-            if (!(valid && key < key_end && key <= pos)) sr[j >> 5][j & 31] = 0xff800000u;  // -inf
-          }
-        }
-        float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          mx0 = fmaxf(mx0, __uint_as_float(sr[0][j]));
-          mx1 = fmaxf(mx1, __uint_as_float(sr[1][j]));
-        }
-        const float mx = fmaxf(mx0, mx1);
-        // raise m only when this tile is far above it: P then stays below 2^8, well inside f16
-        const bool raise = mx > m + T4_RAISE_AT || (m == -INFINITY && mx > -INFINITY);
-        if (ti > 0 && __any_sync(0xffffffffu, raise)) {
-          // the previous P V has completed (its barrier was waited for before this tile's K was written)
-          const float alpha = raise ? ex2f(m - mx) : 1.f;
-#pragma unroll
-          for (int cc = 0; cc < 5; ++cc) {
-            uint32_t r[32];
-            tmem_ld_32x32(tmem_row + T4_O_COL + 32 * cc, r);
-            tmem_ld_wait();
-#pragma unroll
-            for (int x = 0; x < 32; ++x) r[x] = __float_as_uint(__uint_as_float(r[x]) * alpha);
-            t4_tmem_st(tmem_row + T4_O_COL + 32 * cc, r);
-          }
-          t4_tmem_st_wait();
-        }
-        if (raise) m = mx;
-        const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-        for (int ck = 0; ck < 8; ++ck) {
-          uint32_t h[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = ck * 8 + 2 * e;
-            h[e] = t4_ex2_f16x2(__uint_as_float(sr[j >> 5][j & 31]) - base, __uint_as_float(sr[(j + 1) >> 5][(j + 1) & 31]) - base);
-          }
-          *reinterpret_cast<uint4*>(kp_s + tid * 128 + ((ck ^ (tid & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-        }
+      if (lane == 0) {
+        mbar_arrive(&bars.v_ready[b]);
+        mbar_arrive(&bars.raw_free[ti % T4_STAGES]);
       }
-      t4_fence_async();
-      tc_fence_before();
-      __syncthreads();
-      if (tid == 0 && !*abort_flag) {
-        tc_fence_after();
-        const uint64_t da = make_desc_k_sw128(kp_u32);
-        const uint64_t db = make_desc_k_sw128(vt_u32);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) umma_f16(tmem + T4_O_COL, da + 2 * k, db + 2 * k, idesc_o, (ti | k) ? 1u : 0u);
-        umma_commit(bar_o);
-      }
-      if (!mbar_wait(bar_o, ti & 1, abort_flag)) fail = 1;
-      __syncwarp();
-      tc_fence_after();
     }
-    const bool aborted = __syncthreads_or(fail) != 0;
-    if (aborted && tid == 0) {
-      // give the copies in flight their own bounded wait before the shared memory goes away
+  } else if (warp == 12) {
+    // ======== MMAs, by one thread ========
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = make_idesc_f16(128, T4_NK, 0);
+      constexpr uint32_t idesc_o = make_idesc_f16(128, T4_ON, 0);
+      ok = mbar_wait(&bars.q_ready, 0, abort_flag);
+      for (int ti = 0; ok && ti <= n_tiles; ++ti) {
+        if (ti < n_tiles) ok = mbar_wait(&bars.k_ready[ti & 1], (ti >> 1) & 1, abort_flag);
+        for (int t = 0; ok && t < tiles; ++t) {
+          if (ti < n_tiles) {
+            if (ti > 0 && !(ok = mbar_wait(&bars.s_free[t], (ti - 1) & 1, abort_flag))) break;
+            tc_fence_after();
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub) {
+              const uint64_t da = make_desc_k_sw128(q_u32 + t * T4_Q_BYTES + sub * 16384);
+              const uint64_t db = make_desc_k_sw128(k_u32 + (ti & 1) * T4_K_BYTES + sub * 8192);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) umma_f16(tmem + 64u * t, da + 2 * k, db + 2 * k, idesc_s, (sub | k) ? 1u : 0u);
+            }
+            umma_commit(&bars.s_ready[t]);
+            if (t == tiles - 1) umma_commit(&bars.k_free[ti & 1]);
+          }
+          if (ti > 0) {
+            const int pi = ti - 1;
+            if (t == 0 && !(ok = mbar_wait(&bars.v_ready[pi & 1], (pi >> 1) & 1, abort_flag))) break;
+            if (!(ok = mbar_wait(&bars.p_ready[t], pi & 1, abort_flag))) break;
+            tc_fence_after();
+            const uint64_t da = make_desc_k_sw128(p_u32 + t * T4_P_BYTES);
+            const uint64_t db = make_desc_k_sw128(vt_u32 + (pi & 1) * T4_VT_BYTES);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) umma_f16(tmem + 128u + 192u * t, da + 2 * k, db + 2 * k, idesc_o, (pi | k) ? 1u : 0u);
+            umma_commit(&bars.o_done[t]);
+            if (t == tiles - 1) umma_commit(&bars.v_free[pi & 1]);
+          }
+        }
+      }
+      // nothing may be in flight when the tensor memory goes back
+      umma_commit(&bars.drain);
       uint32_t none = 0u;
-      for (int i = ti + 1; i < issued; ++i) mbar_wait(bar_raw + i % T4_STAGES, (i / T4_STAGES) & 1, &none);
+      if (!mbar_wait(&bars.drain, 0, &none)) ok = false;
     }
-    if (!aborted) {
-      // ---- epilogue: O / l from TMEM (column 128 holds l).  The TMEM loads are warp-wide
-      // (.sync.aligned): every thread executes them, only the global stores depend on `valid`.
-      uint32_t r[32];
-      __syncwarp();
-      tmem_ld_32x32(tmem_row + T4_O_COL + ATT_D, r);
-      tmem_ld_wait();
-      const float l = __uint_as_float(r[0]);
-      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays
+    __syncwarp();
+  } else if (lane == 0) {
+    // ======== fetch ========
+    const int32_t* table = p.block_tables + (int64_t)seq * p.max_blocks;
+    const uint8_t* base = p.records + (int64_t)kvh * p.stride_head;
+    int blk[T4_PAGES];
+    auto ids = [&](int ti) {  // a tile ahead of the copies that need them
 #pragma unroll
-      for (int cc = 0; cc < 4; ++cc) {
-        __syncwarp();  // reconverge after the predicated stores of the previous chunk
-        tmem_ld_32x32(tmem_row + T4_O_COL + 32 * cc, r);
-        tmem_ld_wait();
-        if (!valid) continue;
-        if (p.nsplit == 1) {
-          __nv_bfloat16* dst = p.out + row * ATT_D + 32 * cc;
+      for (int pg = 0; pg < T4_PAGES; ++pg) blk[pg] = __ldg(table + min(page_begin + ti * T4_PAGES + pg, p.max_blocks - 1));
+    };
+    ids(0);
+    int issued = 0;
+    for (; issued < n_tiles; ++issued) {
+      const int s = issued % T4_STAGES;
+      if (issued >= T4_STAGES && !(ok = mbar_wait(&bars.raw_free[s], (issued / T4_STAGES - 1) & 1, abort_flag))) break;
+      const int n = min(T4_PAGES, page_end - page_begin - issued * T4_PAGES);
+      mbar_expect_tx(&bars.raw_full[s], n * DASER_KV4_RECORD);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            uint4 w;
-            w.x = pack_bf16x2(__uint_as_float(r[8 * x]) * inv, __uint_as_float(r[8 * x + 1]) * inv);
-            w.y = pack_bf16x2(__uint_as_float(r[8 * x + 2]) * inv, __uint_as_float(r[8 * x + 3]) * inv);
-            w.z = pack_bf16x2(__uint_as_float(r[8 * x + 4]) * inv, __uint_as_float(r[8 * x + 5]) * inv);
-            w.w = pack_bf16x2(__uint_as_float(r[8 * x + 6]) * inv, __uint_as_float(r[8 * x + 7]) * inv);
-            *reinterpret_cast<uint4*>(dst + 8 * x) = w;
-          }
-        } else {
-          float* dst = p.part_o + (row * p.nsplit + sp) * ATT_D + 32 * cc;
-#pragma unroll
-          for (int x = 0; x < 8; ++x)
-            *reinterpret_cast<float4*>(dst + 4 * x) =
-                make_float4(__uint_as_float(r[4 * x]) * inv, __uint_as_float(r[4 * x + 1]) * inv,
-                            __uint_as_float(r[4 * x + 2]) * inv, __uint_as_float(r[4 * x + 3]) * inv);
-        }
+      for (int pg = 0; pg < T4_PAGES; ++pg) {
+        if (pg >= n) break;
+        const int bk = blk[pg] < 0 ? 0 : (blk[pg] >= p.num_blocks ? p.num_blocks - 1 : blk[pg]);
+        t4_bulk_load(raw_u32 + s * T4_RAW + pg * T4_PITCH, base + (int64_t)bk * p.stride_block, DASER_KV4_RECORD, &bars.raw_full[s]);
       }
-      if (valid && p.nsplit > 1) p.part_lse[row * p.nsplit + sp] = l > 0.f ? m + log2f(l) : (l == 0.f ? -INFINITY : l);
-      __syncwarp();
+      ids(issued + 1);
     }
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 0) tmem_dealloc(tmem, T4_TMEM_COLS);
-    if (aborted && tid == 0) atomicOr(&g_attn4_tc_status, 1u);
-  } else if (valid) {
-    // no keys in this split: an empty partial
-    if (p.nsplit == 1) {
-      __nv_bfloat16* dst = p.out + row * ATT_D;
-#pragma unroll
-      for (int ck = 0; ck < 16; ++ck) *reinterpret_cast<uint4*>(dst + 8 * ck) = make_uint4(0u, 0u, 0u, 0u);
-    } else {
-      float* dst = p.part_o + (row * p.nsplit + sp) * ATT_D;
-#pragma unroll
-      for (int ck = 0; ck < 32; ++ck) *reinterpret_cast<float4*>(dst + 4 * ck) = make_float4(0.f, 0.f, 0.f, 0.f);
-      p.part_lse[row * p.nsplit + sp] = -INFINITY;
+    // the copies in flight have landed before the shared memory goes away (the others wait for them too, unless they gave up)
+    for (int i = max(0, issued - T4_STAGES); i < issued; ++i) {
+      uint32_t none = 0u;
+      if (!mbar_wait(&bars.raw_full[i % T4_STAGES], (i / T4_STAGES) & 1, &none)) ok = false;
     }
   }
+  tc_fence_before();
+  const bool aborted = __syncthreads_or(!ok) != 0;
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, T4_TMEM_COLS);
+  }
+  if (aborted && tid == 0) atomicOr(&g_attn4_tc_status, 1u);
 }
 
 }  // namespace daser
@@ -396,10 +472,11 @@ int daser_launch_attention4_tc(const daser::Attn4Params& p, int max_q_len, cudaS
     cudaError_t e = cudaFuncSetAttribute(attn4_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T4_SMEM);
     if (e != cudaSuccess) return (int)e;
   }
-  const int toks = 128 / p.G;
-  const int64_t z = (int64_t)((max_q_len + toks - 1) / toks) * p.nsplit;
+  const int toks = 2 * (128 / p.G);
+  const int groups = (max_q_len + toks - 1) / toks;
+  const int64_t z = (int64_t)groups * p.nsplit;
   if (z > 65535 || p.num_seqs > 65535) return DASER_ERR_TOO_LARGE;
-  return (int)launch_pdl(attn4_tc_kernel, dim3(p.Hkv, p.num_seqs, (unsigned)z), dim3(128), T4_SMEM, stream, p);
+  return (int)launch_pdl(attn4_tc_kernel, dim3(p.Hkv, p.num_seqs, (unsigned)z), dim3(T4_THREADS), T4_SMEM, stream, p, groups);
 }
 
 // Non-zero once any CTA of the 4-bit prefill kernel gave up on a bounded wait (synchronises the device).
