@@ -383,47 +383,61 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
       }
     }
   } else if (warp == 12) {
-    // ======== MMAs, by one thread ========
-    if (lane == 0) {
-      constexpr uint32_t idesc_s = make_idesc_f16(128, T4_NK, 0);
-      constexpr uint32_t idesc_o = make_idesc_f16(128, T4_ON, 0);
-      ok = mbar_wait(&bars.q_ready, 0, abort_flag);
-      for (int ti = 0; ok && ti <= n_tiles; ++ti) {
-        if (ti < n_tiles) ok = mbar_wait(&bars.k_ready[ti & 1], (ti >> 1) & 1, abort_flag);
-        for (int t = 0; ok && t < tiles; ++t) {
-          if (ti < n_tiles) {
-            if (ti > 0 && !(ok = mbar_wait(&bars.s_free[t], (ti - 1) & 1, abort_flag))) break;
-            tc_fence_after();
+    // ======== MMAs: the warp walks the tiles together (its values stay in uniform registers), one lane issues ========
+    constexpr uint32_t idesc_s = make_idesc_f16(128, T4_NK, 0);
+    constexpr uint32_t idesc_o = make_idesc_f16(128, T4_ON, 0);
+    const bool leader = elect_one();
+    // descriptors: the low word moves by (bytes >> 4), the high word is common
+    const uint32_t hi = (uint32_t)(make_desc_k_sw128(0) >> 32);
+    const uint32_t lo_q = (uint32_t)make_desc_k_sw128(q_u32), lo_k = (uint32_t)make_desc_k_sw128(k_u32);
+    const uint32_t lo_p = (uint32_t)make_desc_k_sw128(p_u32), lo_v = (uint32_t)make_desc_k_sw128(vt_u32);
+    auto desc = [&](uint32_t lo) { return (uint64_t)hi << 32 | lo; };
+    auto scores = [&](int t, int ti) {  // S of row tile t against key tile ti
+      tc_fence_after();
+      if (leader) {
+        const uint32_t da = lo_q + t * (T4_Q_BYTES >> 4), db = lo_k + (ti & 1) * (T4_K_BYTES >> 4);
+        const uint32_t d = tmem + 64u * t;
 #pragma unroll
-            for (int sub = 0; sub < 2; ++sub) {
-              const uint64_t da = make_desc_k_sw128(q_u32 + t * T4_Q_BYTES + sub * 16384);
-              const uint64_t db = make_desc_k_sw128(k_u32 + (ti & 1) * T4_K_BYTES + sub * 8192);
+        for (int k = 0; k < 8; ++k)
+          umma_f16(d, desc(da + (k >> 2) * (16384 >> 4) + 2 * (k & 3)), desc(db + (k >> 2) * (8192 >> 4) + 2 * (k & 3)), idesc_s, k ? 1u : 0u);
+        umma_commit(&bars.s_ready[t]);
+        if (t == tiles - 1) umma_commit(&bars.k_free[ti & 1]);
+      }
+      __syncwarp();
+    };
+    auto outputs = [&](int t, int pi) {  // O of row tile t += P V of key tile pi
+      tc_fence_after();
+      if (leader) {
+        const uint32_t da = lo_p + t * (T4_P_BYTES >> 4), db = lo_v + (pi & 1) * (T4_VT_BYTES >> 4);
+        const uint32_t d = tmem + 128u + 192u * t;
 #pragma unroll
-              for (int k = 0; k < 4; ++k) umma_f16(tmem + 64u * t, da + 2 * k, db + 2 * k, idesc_s, (sub | k) ? 1u : 0u);
-            }
-            umma_commit(&bars.s_ready[t]);
-            if (t == tiles - 1) umma_commit(&bars.k_free[ti & 1]);
-          }
-          if (ti > 0) {
-            const int pi = ti - 1;
-            if (t == 0 && !(ok = mbar_wait(&bars.v_ready[pi & 1], (pi >> 1) & 1, abort_flag))) break;
-            if (!(ok = mbar_wait(&bars.p_ready[t], pi & 1, abort_flag))) break;
-            tc_fence_after();
-            const uint64_t da = make_desc_k_sw128(p_u32 + t * T4_P_BYTES);
-            const uint64_t db = make_desc_k_sw128(vt_u32 + (pi & 1) * T4_VT_BYTES);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) umma_f16(tmem + 128u + 192u * t, da + 2 * k, db + 2 * k, idesc_o, (pi | k) ? 1u : 0u);
-            umma_commit(&bars.o_done[t]);
-            if (t == tiles - 1) umma_commit(&bars.v_free[pi & 1]);
-          }
+        for (int k = 0; k < 4; ++k) umma_f16(d, desc(da + 2 * k), desc(db + 2 * k), idesc_o, (pi | k) ? 1u : 0u);
+        umma_commit(&bars.o_done[t]);
+        if (t == tiles - 1) umma_commit(&bars.v_free[pi & 1]);
+      }
+      __syncwarp();
+    };
+    ok = t4_wait(&bars.q_ready, 0, abort_flag);
+    for (int ti = 0; ok && ti <= n_tiles; ++ti) {
+      const int pi = ti - 1;
+      if (ti < n_tiles && !(ok = t4_wait(&bars.k_ready[ti & 1], (ti >> 1) & 1, abort_flag))) break;
+      for (int t = 0; t < tiles; ++t) {
+        if (ti < n_tiles) {
+          if (ti > 0 && !(ok = t4_wait(&bars.s_free[t], pi & 1, abort_flag))) break;
+          scores(t, ti);
+        }
+        if (ti > 0) {
+          if (t == 0 && !(ok = t4_wait(&bars.v_ready[pi & 1], (pi >> 1) & 1, abort_flag))) break;
+          if (!(ok = t4_wait(&bars.p_ready[t], pi & 1, abort_flag))) break;
+          outputs(t, pi);
         }
       }
-      // nothing may be in flight when the tensor memory goes back
-      umma_commit(&bars.drain);
-      uint32_t none = 0u;
-      if (!mbar_wait(&bars.drain, 0, &none)) ok = false;
     }
+    // nothing may be in flight when the tensor memory goes back
+    if (leader) umma_commit(&bars.drain);
     __syncwarp();
+    uint32_t none = 0u;
+    if (!t4_wait(&bars.drain, 0, &none)) ok = false;
   } else if (lane == 0) {
     // ======== fetch ========
     const int32_t* table = p.block_tables + (int64_t)seq * p.max_blocks;
