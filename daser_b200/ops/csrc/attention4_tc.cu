@@ -3,7 +3,7 @@
 // One CTA per SM works on two tiles of 128 query rows (128 / G query tokens x the G heads of one KV head, each) against tiles of 64 keys, so
 // that a tile of keys is dequantised once for 256 rows and one row tile's softmax runs under the other's MMAs.  14 warps:
 //   * 0-3, 4-7   softmax of row tile 0, 1: a thread owns a row of S (tcgen05.ld 32x32b), takes it into registers and frees it at once,
-//                so that the next S is under way while P = 2^(S - m) is made: f16, into shared memory, as the MMA operand.  The running
+//                so that the next S is under way while P = 2^(S - m) is made: f16, back into TMEM, as the MMA operand.  The running
 //                maximum m is raised only when a tile exceeds it by 2^8, and only then is O rescaled (tcgen05.ld / st);
 //   * 8-11       dequantise: K as [key][dim], V transposed to [dim][key], f16 (exact), in the 128-byte-swizzled K-major layout of the
 //                MMA descriptors, two buffers each.  V's codes of two neighbouring tokens are interleaved nibble by nibble, so that
@@ -23,12 +23,15 @@ constexpr int T4_RAW = T4_PAGES * T4_PITCH;
 constexpr int T4_STAGES = 3;
 constexpr int T4_Q_BYTES = 128 * ATT_D * 2;             // of a row tile: two sub-tiles [128 rows][64 dims]
 constexpr int T4_K_BYTES = T4_NK * ATT_D * 2;           // two sub-tiles [64 keys][64 dims]
-constexpr int T4_P_BYTES = 128 * T4_NK * 2;             // [128 rows][64 keys]
 constexpr int T4_ON = ATT_D + 16;                       // output columns: 128 dims, the row sum, 15 unused
 constexpr int T4_VT_BYTES = T4_ON * 128;
 constexpr int T4_THREADS = 14 * 32;
-constexpr int T4_SMEM = 1024 + 2 * T4_Q_BYTES + 2 * T4_K_BYTES + 2 * T4_VT_BYTES + 2 * T4_P_BYTES + T4_STAGES * T4_RAW;
-constexpr uint32_t T4_TMEM_COLS = 512;                  // S of tile t in columns [64 t, 64 t + 64), O in [128 + 192 t, + 144)
+constexpr int T4_SMEM = 1024 + 2 * T4_Q_BYTES + 2 * T4_K_BYTES + 2 * T4_VT_BYTES + T4_STAGES * T4_RAW;
+constexpr uint32_t T4_TMEM_COLS = 512;
+// Of row tile t: S in columns [64 t, + 64), O in [128 + 192 t, + 144), P (two f16 a column) in [288 + 192 t, + 32).
+__device__ __forceinline__ uint32_t t4_s_col(int t) { return 64u * t; }
+__device__ __forceinline__ uint32_t t4_o_col(int t) { return 128u + 192u * t; }
+__device__ __forceinline__ uint32_t t4_p_col(int t) { return 288u + 192u * t; }
 constexpr float T4_RAISE_AT = 8.f;
 
 __device__ uint32_t g_attn4_tc_status = 0;  // bit 0: a bounded wait ran out
@@ -49,6 +52,26 @@ __device__ __forceinline__ void t4_tmem_st16(uint32_t taddr, const uint32_t (&r)
       "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void t4_tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]^T, f16.
+__device__ __forceinline__ void t4_umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void t4_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -87,8 +110,7 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
   uint8_t* q_s = smem;
   uint8_t* k_s = q_s + 2 * T4_Q_BYTES;
   uint8_t* vt_s = k_s + 2 * T4_K_BYTES;
-  uint8_t* p_s = vt_s + 2 * T4_VT_BYTES;
-  uint8_t* raw_s = p_s + 2 * T4_P_BYTES;
+  uint8_t* raw_s = vt_s + 2 * T4_VT_BYTES;
   volatile uint32_t* abort_flag = &bars.abort;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -134,7 +156,7 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
     return;
   }
 
-  const uint32_t q_u32 = smem_u32(q_s), k_u32 = smem_u32(k_s), vt_u32 = smem_u32(vt_s), p_u32 = smem_u32(p_s), raw_u32 = smem_u32(raw_s);
+  const uint32_t q_u32 = smem_u32(q_s), k_u32 = smem_u32(k_s), vt_u32 = smem_u32(vt_s), raw_u32 = smem_u32(raw_s);
   if (tid == 0) {
 #pragma unroll
     for (int s = 0; s < T4_STAGES; ++s) {
@@ -171,10 +193,10 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
   if (warp < 8) {
     // ======== softmax ========
     if (tile < tiles) {
-      const uint32_t tmem_s = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 64u * tile;
-      const uint32_t tmem_o = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128u + 192u * tile;
+      const uint32_t tmem_s = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t4_s_col(tile);
+      const uint32_t tmem_o = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t4_o_col(tile);
+      const uint32_t tmem_p = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t4_p_col(tile);
       uint8_t* my_q = q_s + tile * T4_Q_BYTES;
-      uint8_t* my_p = p_s + tile * T4_P_BYTES;
       {  // Q row -> f16, times scale * log2(e), into the swizzled A tile
         const __nv_bfloat16* qp = p.q + row * ATT_D;
 #pragma unroll
@@ -240,17 +262,12 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
         }
         if (raise) m = mx;
         const float base = m == -INFINITY ? 0.f : m;
+        // P, two keys a register, over the first half of the scores' registers
 #pragma unroll
-        for (int ck = 0; ck < 8; ++ck) {
-          uint32_t h[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = ck * 8 + 2 * e;
-            h[e] = t4_ex2_f16x2(__uint_as_float(sr[j >> 5][j & 31]) - base, __uint_as_float(sr[(j + 1) >> 5][(j + 1) & 31]) - base);
-          }
-          *reinterpret_cast<uint4*>(my_p + rt * 128 + ((ck ^ (rt & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-        }
-        t4_fence_async();
+        for (int j = 0; j < T4_NK; j += 2)
+          sr[0][j >> 1] = t4_ex2_f16x2(__uint_as_float(sr[j >> 5][j & 31]) - base, __uint_as_float(sr[(j + 1) >> 5][(j + 1) & 31]) - base);
+        t4_tmem_st32(tmem_p, sr[0]);
+        t4_tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.p_ready[tile]);
@@ -314,8 +331,9 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
       // ---- K: (key, 16-dim group) items, four per thread ----
 #pragma unroll
       for (int rep = 0; rep < 4; ++rep) {
+        // four groups of a row on neighbouring lanes: their 16-byte pieces, and those of the row behind, are in different banks
         const int item = dt + 128 * rep;
-        const int kt = item >> 3, c = item & 7;
+        const int kt = (item >> 2) & 63, c = (item & 3) + 4 * (item >> 8);
         uint32_t h[8];
         if (key0 + kt < key_end) {
           const uint8_t* rec = st + (kt >> 4) * T4_PITCH;
@@ -390,13 +408,13 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
     // descriptors: the low word moves by (bytes >> 4), the high word is common
     const uint32_t hi = (uint32_t)(make_desc_k_sw128(0) >> 32);
     const uint32_t lo_q = (uint32_t)make_desc_k_sw128(q_u32), lo_k = (uint32_t)make_desc_k_sw128(k_u32);
-    const uint32_t lo_p = (uint32_t)make_desc_k_sw128(p_u32), lo_v = (uint32_t)make_desc_k_sw128(vt_u32);
+    const uint32_t lo_v = (uint32_t)make_desc_k_sw128(vt_u32);
     auto desc = [&](uint32_t lo) { return (uint64_t)hi << 32 | lo; };
     auto scores = [&](int t, int ti) {  // S of row tile t against key tile ti
       tc_fence_after();
       if (leader) {
         const uint32_t da = lo_q + t * (T4_Q_BYTES >> 4), db = lo_k + (ti & 1) * (T4_K_BYTES >> 4);
-        const uint32_t d = tmem + 64u * t;
+        const uint32_t d = tmem + t4_s_col(t);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           umma_f16(d, desc(da + (k >> 2) * (16384 >> 4) + 2 * (k & 3)), desc(db + (k >> 2) * (8192 >> 4) + 2 * (k & 3)), idesc_s, k ? 1u : 0u);
@@ -408,10 +426,10 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
     auto outputs = [&](int t, int pi) {  // O of row tile t += P V of key tile pi
       tc_fence_after();
       if (leader) {
-        const uint32_t da = lo_p + t * (T4_P_BYTES >> 4), db = lo_v + (pi & 1) * (T4_VT_BYTES >> 4);
-        const uint32_t d = tmem + 128u + 192u * t;
+        const uint32_t db = lo_v + (pi & 1) * (T4_VT_BYTES >> 4);
+        const uint32_t d = tmem + t4_o_col(t), a = tmem + t4_p_col(t);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_f16(d, desc(da + 2 * k), desc(db + 2 * k), idesc_o, (pi | k) ? 1u : 0u);
+        for (int k = 0; k < 4; ++k) t4_umma_ts(d, a + 8 * k, desc(db + 2 * k), idesc_o, (pi | k) ? 1u : 0u);
         umma_commit(&bars.o_done[t]);
         if (t == tiles - 1) umma_commit(&bars.v_free[pi & 1]);
       }
