@@ -101,14 +101,17 @@ __device__ __forceinline__ uint32_t fp4_scale_byte(float absmax) {
   return (b + 63u + ((b >> 7) & 1u)) >> 7;
 }
 
-// Pairs of values -> codes.  The quotient x / s is correctly rounded, as two fused corrections of x * (1 / s): with inv the
+// Pairs of values -> codes; inv = fp4_inverse(scale_byte).  The quotient x / s is correctly rounded, as two fused corrections of x * (1 / s): with inv the
 // correctly rounded reciprocal and q within one unit of the quotient, q + (x - q s) * inv rounds correctly (P. Markstein,
 // "Computation of elementary functions on the IBM RISC System/6000 processor", 1990).  x * inv alone is not enough:
 // 3.5 * 1.875 / 1.875 would come out above the border between 3 and 4.
-template <int N>
-__device__ __forceinline__ void fp4_encode(const uint64_t (&x)[N], uint32_t scale_byte, uint32_t (&codes)[N / 4]) {
+__device__ __forceinline__ float fp4_inverse(uint32_t scale_byte) {
   const float s = fp4_scale(scale_byte);
-  const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+  return s > 0.f ? __frcp_rn(s) : 0.f;
+}
+template <int N>
+__device__ __forceinline__ void fp4_encode(const uint64_t (&x)[N], uint32_t scale_byte, float inv, uint32_t (&codes)[N / 4]) {
+  const float s = fp4_scale(scale_byte);
   const uint64_t inv2 = pair2(inv, inv), ns2 = pair2(-s, -s);
   float y[2 * N];
 #pragma unroll

@@ -132,8 +132,8 @@ kv4_write_kernel(TIn* __restrict__ qkv, int64_t qkv_stride, const int32_t* __res
       mb = max3_nan(mb, __shfl_xor_sync(0xffffffffu, mb, 1), 0.f);
       const uint32_t sa = fp4_scale_byte(ma), sb = fp4_scale_byte(mb);
       uint32_t ca[1], cb[1];
-      fp4_encode<4>(a, sa, ca);
-      fp4_encode<4>(b, sb, cb);
+      fp4_encode<4>(a, sa, fp4_inverse(sa), ca);
+      fp4_encode<4>(b, sb, fp4_inverse(sb), cb);
       if (in && !is_q && live) {
         const int kv = is_v ? 1 : 0;
         uint8_t* rec = pool + block * stride_block + (int64_t)(hd - Hq - kv * Hkv) * stride_head;
@@ -181,9 +181,9 @@ kv4_read_kernel(const uint8_t* __restrict__ pool, int64_t stride_block, int64_t 
 // rotated by the slot's delta (keys), quantised, and put into the record's place in shared memory; whole records
 // then leave as 16-byte stores.  Stored directly, the 8-byte pieces of V would each be a quarter of a 32-byte sector.
 constexpr int KV4_HEADS = 8;
+constexpr int KV4_PITCH = DASER_KV4_RECORD + 32;  // of a record in shared memory: the rows of eight heads start in different banks
 
-__device__ __forceinline__ void load_fp8_group(const uint8_t* p, float scale, uint64_t (&x)[8]) {
-  const uint4 q = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ void decode_fp8_group(const uint4& q, float scale, uint64_t (&x)[8]) {
   const uint32_t w[4] = {q.x, q.y, q.z, q.w};
   const uint64_t s = pair2(scale, scale);
 #pragma unroll
@@ -192,8 +192,7 @@ __device__ __forceinline__ void load_fp8_group(const uint8_t* p, float scale, ui
     x[i] = mul2(pair2(f.x, f.y), s);
   }
 }
-__device__ __forceinline__ void load_bf16_group(const __nv_bfloat16* p, uint64_t (&x)[8]) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p), b = *reinterpret_cast<const uint4*>(p + 8);
+__device__ __forceinline__ void decode_bf16_group(const uint4& a, const uint4& b, uint64_t (&x)[8]) {
   const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = pair2(bf16_lo(w[i]), bf16_hi(w[i]));
@@ -204,7 +203,8 @@ __global__ void __launch_bounds__(256)
 kv4_restore_kernel(const DaserKVJob job, const DaserKV4Pool pool) {
   constexpr int D = DASER_KV4_DIM, B = DASER_KV4_TOKENS;
   __shared__ __align__(16) float s_cs[D];
-  __shared__ __align__(16) uint8_t s_rec[KV4_HEADS * DASER_KV4_RECORD];
+  __shared__ float s_inv[256];  // of every scale byte: a reciprocal, correctly rounded, takes more instructions than a group otherwise
+  __shared__ __align__(16) uint8_t s_rec[KV4_HEADS * KV4_PITCH];
   const int H = job.num_kv_heads;
   const int slot = blockIdx.x / job.layer_count;
   const int layer = job.layer_begin + blockIdx.x % job.layer_count;
@@ -221,6 +221,7 @@ kv4_restore_kernel(const DaserKVJob job, const DaserKV4Pool pool) {
     if (threadIdx.x == 0) kv4_report(job.status, bad, slot);
     return;
   }
+  s_inv[threadIdx.x] = fp4_inverse(threadIdx.x);
   if (delta != 0 && threadIdx.x < D) {
     const float v = job.cos_sin[adelta * D + threadIdx.x];
     s_cs[threadIdx.x] = (threadIdx.x >= D / 2 && delta < 0) ? -v : v;  // sin(-x) = -sin(x)
@@ -232,21 +233,42 @@ kv4_restore_kernel(const DaserKVJob job, const DaserKV4Pool pool) {
   const float* img_scales = reinterpret_cast<const float*>(base + elems);
   const int items = 2 * B * nh * 4;
   const int lg = (nh & (nh - 1)) == 0 ? __ffs(nh) - 1 : -1;
-  for (int item = threadIdx.x; item < items; item += 256) {
-    const int j = item & 3;
+  // what an item reads, and its (kv * B + token, head), one item ahead of its use
+  uint4 n1, n2, n3, n4;
+  float ns1 = 0.f, ns2 = 0.f;
+  int n_rr = 0, n_hl = 0;
+  auto load = [&](int item) {
     const int r = item >> 2;
-    const int rr = lg >= 0 ? r >> lg : r / nh;  // kv * B + token
-    const int hl = r - rr * nh;
-    const int tok = rr & (B - 1), kv = rr / B;
-    const int64_t e1 = ((int64_t)rr * H + head0 + hl) * D + j * FP8_GROUP, e2 = e1 + D / 2;
+    n_rr = lg >= 0 ? r >> lg : r / nh;
+    n_hl = r - n_rr * nh;
+    const int e1 = (n_rr * H + head0 + n_hl) * D + (item & 3) * FP8_GROUP, e2 = e1 + D / 2;  // (a layer of a slot: far below 2^31)
+    if (IMG_FP8) {
+      n1 = *reinterpret_cast<const uint4*>(base + e1);
+      n2 = *reinterpret_cast<const uint4*>(base + e2);
+      ns1 = img_scales[e1 / FP8_GROUP];
+      ns2 = img_scales[e2 / FP8_GROUP];
+    } else {
+      const uint4* h1 = reinterpret_cast<const uint4*>(base + 2 * e1);
+      const uint4* h2 = reinterpret_cast<const uint4*>(base + 2 * e2);
+      n1 = h1[0];
+      n2 = h2[0];
+      n3 = h1[1];
+      n4 = h2[1];
+    }
+  };
+  const int j = threadIdx.x & 3;
+  if (threadIdx.x < items) load(threadIdx.x);
+  for (int item = threadIdx.x; item < items; item += 256) {
+    const int hl = n_hl, tok = n_rr & (B - 1), kv = n_rr / B;
     uint64_t x1[8], x2[8];
     if (IMG_FP8) {
-      load_fp8_group(base + e1, img_scales[e1 / FP8_GROUP], x1);
-      load_fp8_group(base + e2, img_scales[e2 / FP8_GROUP], x2);
+      decode_fp8_group(n1, ns1, x1);
+      decode_fp8_group(n2, ns2, x2);
     } else {
-      load_bf16_group(reinterpret_cast<const __nv_bfloat16*>(base) + e1, x1);
-      load_bf16_group(reinterpret_cast<const __nv_bfloat16*>(base) + e2, x2);
+      decode_bf16_group(n1, n3, x1);
+      decode_bf16_group(n2, n4, x2);
     }
+    if (item + 256 < items) load(item + 256);
     if (kv == 0 && delta != 0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -256,29 +278,31 @@ kv4_restore_kernel(const DaserKVJob job, const DaserKV4Pool pool) {
         rotate2(x1[2 * i + 1], x2[2 * i + 1], c.y, s.y);
       }
     }
-    uint8_t* rec = s_rec + hl * DASER_KV4_RECORD;
+    uint8_t* rec = s_rec + hl * KV4_PITCH;
     uint32_t codes[2];
     const uint32_t s1 = fp4_scale_byte(fp4_absmax<8>(x1)), s2 = fp4_scale_byte(fp4_absmax<8>(x2));
-    fp4_encode<8>(x1, s1, codes);
+    fp4_encode<8>(x1, s1, s_inv[s1], codes);
     *reinterpret_cast<uint2*>(rec + kv4_code_at(kv, tok, 2 * j)) = make_uint2(codes[0], codes[1]);
-    fp4_encode<8>(x2, s2, codes);
+    fp4_encode<8>(x2, s2, s_inv[s2], codes);
     *reinterpret_cast<uint2*>(rec + kv4_code_at(kv, tok, 8 + 2 * j)) = make_uint2(codes[0], codes[1]);
     rec[kv4_scale_at(kv, tok, j)] = (uint8_t)s1;
     rec[kv4_scale_at(kv, tok, 4 + j)] = (uint8_t)s2;
   }
   __syncthreads();
-  // with more ranks than KV heads a head is kept by `replicas` ranks
+  // a warp a head; with more ranks than KV heads a head is kept by `replicas` ranks
   const bool wide = pool.n_ranks > H;
   const int replicas = wide ? pool.n_ranks / H : 1;
   constexpr int VECS = DASER_KV4_RECORD / 16;
-  for (int i = threadIdx.x; i < nh * VECS; i += 256) {
-    const int hl = i / VECS, at = (i - hl * VECS) * 16;
-    const int head = head0 + hl;
-    const int rank0 = wide ? head * replicas : head / pool.heads_per_rank;
-    const int64_t off = (int64_t)layer * pool.stride_layer + (int64_t)block * pool.stride_block +
-                        (int64_t)(wide ? 0 : head % pool.heads_per_rank) * pool.stride_head + at;
-    const uint4 v = *reinterpret_cast<const uint4*>(s_rec + hl * DASER_KV4_RECORD + at);
-    for (int rep = 0; rep < replicas; ++rep) *reinterpret_cast<uint4*>(pool.records[rank0 + rep] + off) = v;
+  const int hl = threadIdx.x >> 5, head = head0 + hl;
+  if (hl >= nh) return;
+  const int rank0 = wide ? head * replicas : head / pool.heads_per_rank;
+  const int64_t off = (int64_t)layer * pool.stride_layer + (int64_t)block * pool.stride_block +
+                      (int64_t)(wide ? 0 : head - rank0 * pool.heads_per_rank) * pool.stride_head;
+  const uint4* src = reinterpret_cast<const uint4*>(s_rec + hl * KV4_PITCH);
+  for (int rep = 0; rep < replicas; ++rep) {
+    uint4* dst = reinterpret_cast<uint4*>(pool.records[rank0 + rep] + off);
+#pragma unroll
+    for (int i = threadIdx.x & 31; i < VECS; i += 32) dst[i] = src[i];
   }
 }
 
@@ -290,7 +314,7 @@ template <bool IMG_FP8>
 __global__ void __launch_bounds__(256)
 kv4_save_kernel(const DaserKVJob job, const DaserKV4Pool pool) {
   constexpr int D = DASER_KV4_DIM, B = DASER_KV4_TOKENS;
-  __shared__ __align__(16) uint8_t s_rec[KV4_HEADS * DASER_KV4_RECORD];
+  __shared__ __align__(16) uint8_t s_rec[KV4_HEADS * KV4_PITCH];
   const int H = job.num_kv_heads;
   const int slot = blockIdx.x / job.num_layers, layer = blockIdx.x % job.num_layers;
   const int block = job.block_id[slot];
@@ -312,11 +336,12 @@ kv4_save_kernel(const DaserKVJob job, const DaserKV4Pool pool) {
   const int l0 = blockIdx.y * KV4_HEADS, nh = min(KV4_HEADS, owned - l0);
   if (nh <= 0) return;
   constexpr int VECS = DASER_KV4_RECORD / 16;
-  const uint8_t* src = pool.records[job.rank] + (int64_t)layer * pool.stride_layer + (int64_t)block * pool.stride_block;
-  for (int i = threadIdx.x; i < nh * VECS; i += 256) {
-    const int hl = i / VECS, at = (i - hl * VECS) * 16;
-    *reinterpret_cast<uint4*>(s_rec + hl * DASER_KV4_RECORD + at) =
-        *reinterpret_cast<const uint4*>(src + (int64_t)(l0 + hl) * pool.stride_head + at);
+  if (const int hl = threadIdx.x >> 5; hl < nh) {  // a warp a head
+    const uint4* src = reinterpret_cast<const uint4*>(pool.records[job.rank] + (int64_t)layer * pool.stride_layer +
+                                                      (int64_t)block * pool.stride_block + (int64_t)(l0 + hl) * pool.stride_head);
+    uint4* dst = reinterpret_cast<uint4*>(s_rec + hl * KV4_PITCH);
+#pragma unroll
+    for (int i = threadIdx.x & 31; i < VECS; i += 32) dst[i] = src[i];
   }
   __syncthreads();
   const int64_t elems = (int64_t)2 * B * H * D;
@@ -331,8 +356,8 @@ kv4_save_kernel(const DaserKVJob job, const DaserKV4Pool pool) {
     const int rr = lg >= 0 ? r >> lg : r / nh;  // kv * B + token
     const int hl = r - rr * nh;
     const int tok = rr & (B - 1), kv = rr / B;
-    const uint8_t* rec = s_rec + hl * DASER_KV4_RECORD;
-    const int64_t row = (int64_t)rr * H + first + l0 + hl;
+    const uint8_t* rec = s_rec + hl * KV4_PITCH;
+    const int row = rr * H + first + l0 + hl;  // (a layer of a slot: far below 2^31)
     if (IMG_FP8) {
       float x[16];
       const uint2 w = *reinterpret_cast<const uint2*>(rec + kv4_code_at(kv, tok, 2 * p));
@@ -449,10 +474,11 @@ __global__ void __launch_bounds__(256)
 quant_fp4b16_kernel(const __nv_bfloat16* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t groups) {
   for (int64_t g = blockIdx.x * (int64_t)256 + threadIdx.x; g < groups; g += (int64_t)gridDim.x * 256) {
     uint64_t v[8];
-    load_bf16_group(x + g * 16, v);
+    const uint4* src = reinterpret_cast<const uint4*>(x + g * 16);
+    decode_bf16_group(src[0], src[1], v);
     const uint32_t s = fp4_scale_byte(fp4_absmax<8>(v));
     uint32_t c[2];
-    fp4_encode<8>(v, s, c);
+    fp4_encode<8>(v, s, fp4_inverse(s), c);
     *reinterpret_cast<uint2*>(codes + g * 8) = make_uint2(c[0], c[1]);
     scales[g] = (uint8_t)s;
   }
