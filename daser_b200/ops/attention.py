@@ -95,12 +95,16 @@ def plan_kv4(num_seqs: int, kv_heads: int, max_q_len: int, group: int, max_pages
             nsplit = max(1, min(nsplit, MAX_ROW_SPLITS // rows))
         per = -(--(-max_pages // nsplit) // 4) * 4
         return -(-max_pages // per), per
-    # up to three pairs of pages a warp, one CTA per item takes less than the merge kernel that sharing needs
-    if max_pages <= 96:
+    # One CTA per item: about 2 us and 0.051 us a page, in as many waves as the items need.  Shared: the same over all pages and 80 pages'
+    # time per item, and 6 us for the merge kernel and the partial results.  Measured: 128 items of 128 pages 9 us against
+    # 24, 8 items of 256 pages 17 against 15, 256 items of 256 - 2048 pages 210 against 130.
+    items = max(1, num_seqs) * kv_heads * -(-max_q_len * group // (8 if max_q_len * group <= 8 else 16))
+    workers = min(NUM_SMS, items * max_pages // 32)  # a pair of pages a warp at least
+    if workers < 2:
         return 0, 0
-    # one CTA per SM, and a pair of pages a warp at least
-    pages = max(1, num_seqs) * kv_heads * -(-max_q_len * group // (8 if max_q_len * group <= 8 else 16)) * max_pages
-    return max(2, min(NUM_SMS, pages // 32)), 0
+    alone = -(-items // NUM_SMS) * (2.0 + 0.051 * max_pages)
+    shared = 8.0 + 0.051 * items * (max_pages + 80) / workers
+    return (0 if alone <= shared else workers), 0
 
 
 class AttentionWorkspace:

@@ -14,7 +14,8 @@ namespace daser {
 
 constexpr int SCORE_PAGES = 128;    // pages per CTA of the score kernel: 8 per half-warp
 constexpr int SELECT_THREADS = 1024;
-constexpr int SELECT_BINS = 2048;
+constexpr int SELECT_DIGIT = 11;
+constexpr int SELECT_BINS = 1 << SELECT_DIGIT;
 static_assert(SELECT_THREADS == 32 * 32, "one warp can hold a value of every warp");
 constexpr int SELECT_SMEM_KEYS = 40960;  // longer lists are read from global memory in every pass
 
@@ -29,6 +30,7 @@ struct Select4Params {
   int32_t* pages;            // [Tq, Hkv, n_pages]
   int max_blocks, num_blocks, Hq, Hkv, G, max_q_len, total_q;
   int stride, n_pages, sink, recent;
+  int batches;               // of SCORE_PAGES pages per CTA of the score kernel
 };
 
 // The query row of (sequence, offset) and the pages it sees; false if there is no such row.
@@ -47,7 +49,7 @@ __device__ __forceinline__ double warp_max_f64(double v) {
   return v;
 }
 
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 3)
 attn4_score_kernel(const Select4Params p) {
   __shared__ double s_max[4];
   __shared__ __align__(16) int8_t s_q[2 * ATT_D];
@@ -55,24 +57,33 @@ attn4_score_kernel(const Select4Params p) {
   const int seq = blockIdx.z / p.max_q_len, off = blockIdx.z % p.max_q_len, kvh = blockIdx.y;
   int row, count;
   if (!select_row(p, seq, off, row, count)) return;
-  const int lo_page = max(p.sink, (int)blockIdx.x * SCORE_PAGES);
-  const int hi_page = min(count - p.recent, ((int)blockIdx.x + 1) * SCORE_PAGES);
+  const int span = SCORE_PAGES * p.batches;
+  const int lo_page = max(p.sink, (int)blockIdx.x * span);
+  const int hi_page = min(count - p.recent, ((int)blockIdx.x + 1) * span);
   if (count <= p.n_pages || lo_page >= hi_page) return;  // everything is chosen, or nothing here needs a score
 
-  // Sixteen lanes a page, 16 bytes a lane, eight pages a half-warp.  All loads are issued before the query is prepared: the block
-  // id is a dependent load in front of them, and nothing else hides either.
+  // Sixteen lanes a page, 16 bytes a lane, eight pages a half-warp and batch.  A batch's loads are issued before the batch in front of it
+  // is worked on (the first one's before the query is prepared): the block id is a dependent load in front of them, and nothing
+  // else hides either.
   const int lane = threadIdx.x & 31, sub = lane & 15;
-  const int page0 = blockIdx.x * SCORE_PAGES + (threadIdx.x >> 4) * 8;
-  const int my_page = page0 + (sub >> 1);  // whose score this lane ends up with
-  int blk = p.block_tables[(int64_t)seq * p.max_blocks + min(my_page, count - 1)];
-  blk = blk < 0 ? 0 : (blk >= p.num_blocks ? p.num_blocks - 1 : blk);
+  const int32_t* table = p.block_tables + (int64_t)seq * p.max_blocks;
+  int my_page = blockIdx.x * span + (threadIdx.x >> 4) * 8 + (sub >> 1);  // whose score this lane ends up with
+  auto block_of = [&](int page) {
+    const int blk = table[min(page, count - 1)];
+    return blk < 0 ? 0 : (blk >= p.num_blocks ? p.num_blocks - 1 : blk);
+  };
   int4 c[8];
+  int e = 0;
+  auto load = [&](int blk) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int b = __shfl_sync(0xffffffffu, blk, (lane & 16) + 2 * i);
-    c[i] = *reinterpret_cast<const int4*>(p.codes + ((int64_t)b * p.Hkv + kvh) * (2 * ATT_D) + 16 * sub);
-  }
-  const int e = p.exps[(int64_t)blk * p.Hkv + kvh];
+    for (int i = 0; i < 8; ++i) {
+      const int b = __shfl_sync(0xffffffffu, blk, (lane & 16) + 2 * i);
+      c[i] = *reinterpret_cast<const int4*>(p.codes + ((int64_t)b * p.Hkv + kvh) * (2 * ATT_D) + 16 * sub);
+    }
+    e = p.exps[(int64_t)blk * p.Hkv + kvh];
+  };
+  load(block_of(my_page));
+  int blk_next = block_of(my_page + SCORE_PAGES);
 
   double up = 0.0, down = 0.0;  // sums of at most 16 bf16 values: exact
   if (threadIdx.x < ATT_D) {
@@ -103,24 +114,33 @@ attn4_score_kernel(const Select4Params p) {
   }
   __syncthreads();
   const int4 qv = *reinterpret_cast<const int4*>(s_q + 16 * sub);
-  int dot[8];
+  float* dst = p.scores + ((int64_t)row * p.Hkv + kvh) * p.stride;
+  const int batches = min(p.batches, (hi_page - (int)blockIdx.x * span + SCORE_PAGES - 1) / SCORE_PAGES);
+  for (int k = 0; k < batches; ++k) {
+    int dot[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) dot[i] = __dp4a(c[i].x, qv.x, __dp4a(c[i].y, qv.y, __dp4a(c[i].z, qv.z, __dp4a(c[i].w, qv.w, 0))));
-  // sum over the sixteen lanes and transpose: a lane keeps half of its pages at each step, in the end page sub / 2
-#pragma unroll
-  for (int n = 4, o = 8; n > 0; n >>= 1, o >>= 1) {
-#pragma unroll
-    for (int i = 0; i < n; ++i) {
-      const bool high = (sub & o) != 0;
-      const int keep = high ? dot[n + i] : dot[i], give = high ? dot[i] : dot[n + i];
-      dot[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    for (int i = 0; i < 8; ++i) dot[i] = __dp4a(c[i].x, qv.x, __dp4a(c[i].y, qv.y, __dp4a(c[i].z, qv.z, __dp4a(c[i].w, qv.w, 0))));
+    // exponent 127: a key of the page is not finite; such a page is always read
+    const float scale = e == 127 ? INFINITY : __uint_as_float((uint32_t)(max(e, -126) + 127) << 23);
+    const int page = my_page;
+    my_page += SCORE_PAGES;
+    if (k + 1 < batches) {
+      load(blk_next);
+      blk_next = block_of(my_page + SCORE_PAGES);
     }
+    // sum over the sixteen lanes and transpose: a lane keeps half of its pages at each step, in the end page sub / 2
+#pragma unroll
+    for (int n = 4, o = 8; n > 0; n >>= 1, o >>= 1) {
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        const bool high = (sub & o) != 0;
+        const int keep = high ? dot[n + i] : dot[i], give = high ? dot[i] : dot[n + i];
+        dot[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+      }
+    }
+    dot[0] += __shfl_xor_sync(0xffffffffu, dot[0], 1);
+    if ((sub & 1) == 0 && page >= lo_page && page < hi_page) dst[page] = scale == INFINITY ? INFINITY : (float)dot[0] * scale;
   }
-  dot[0] += __shfl_xor_sync(0xffffffffu, dot[0], 1);
-  // exponent 127: a key of the page is not finite; such a page is always read
-  if ((sub & 1) == 0 && my_page >= lo_page && my_page < hi_page)
-    p.scores[((int64_t)row * p.Hkv + kvh) * p.stride + my_page] =
-        e == 127 ? INFINITY : (float)dot[0] * __uint_as_float((uint32_t)(max(e, -126) + 127) << 23);
 }
 
 // Floats in the order of unsigned integers.
@@ -184,13 +204,13 @@ attn4_select_kernel(const Select4Params p) {
   __syncthreads();  // s_lo and s_hi are used again below
   auto key = [&](int i) { return cached ? s_keys[i] : ordered(src[i]); };
 
-  // The need-th largest key, by digits of up to 11 bits from the first bit in which the keys differ.
+  // The need-th largest key, by digits of up to SELECT_DIGIT bits from the first bit in which the keys differ.
   // Invariant: keys whose bits from `shift` up exceed `prefix` are chosen, `need` more are among those equal to it.
   int shift = lo == hi ? 0 : 32 - __clz(lo ^ hi);
   uint32_t prefix = shift >= 32 ? 0u : hi >> shift;
   bool whole = false;  // all keys that match the prefix are chosen
   while (shift > 0 && !whole) {
-    const int width = min(shift, 11);
+    const int width = min(shift, SELECT_DIGIT);
     const int at = shift - width;
     const uint32_t mask = (1u << width) - 1u;
     for (int i = tid; i < SELECT_BINS; i += SELECT_THREADS) s_bins[i] = 0u;
@@ -301,7 +321,10 @@ DASER_API int daser_select_pages_kv4(const void* q, const int8_t* codes, const i
     if (e != cudaSuccess) return (int)e;
   }
   if (stride > n_pages) {
-    cudaError_t e = launch_pdl(attn4_score_kernel, dim3((unsigned)((stride + SCORE_PAGES - 1) / SCORE_PAGES), (unsigned)Hkv, (unsigned)rows),
+    // one batch a CTA while that fills the GPU no more than twice (4 resident an SM), four beyond
+    const int64_t chunks = (stride + SCORE_PAGES - 1) / SCORE_PAGES;
+    p.batches = chunks * Hkv * rows > 2 * 148 * 4 ? 4 : 1;
+    cudaError_t e = launch_pdl(attn4_score_kernel, dim3((unsigned)((chunks + p.batches - 1) / p.batches), (unsigned)Hkv, (unsigned)rows),
                                dim3(256), 0, stream, p);
     if (e != cudaSuccess) return (int)e;
   }
