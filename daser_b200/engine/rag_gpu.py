@@ -55,7 +55,7 @@ class GpuRagEngine(SchedulingMixin):
                  seed: int = 0, model_id: str = "default", tp_ctx=None, weights: Optional[LlamaWeights] = None,
                  staging_slots: int = 512, max_blocks: int = 512, use_graphs: bool = True,
                  compose_after: int = 0, repair_tokens: int = 0, layer_groups: int = 8, pp_link=None,
-                 write_behind: bool = False) -> None:
+                 write_behind: bool = False, kv_format: str = "fp8b16") -> None:
         self.cfg = cfg
         # pipeline parallelism: this process is one stage (``parallel/pp.py::StageLink``); it runs a
         # contiguous range of layers, keeps their KV in a pool and a store file of its own, and a
@@ -89,7 +89,7 @@ class GpuRagEngine(SchedulingMixin):
             self.weights.interleave_gate_up_(gemm_ops.GATE_UP_BLOCK)
         self.runner = GpuModelRunner(cfg, self.weights, num_blocks, max_tokens, max_seqs, tp_ctx, self.device,
                                      max_blocks=max_blocks, use_graphs=use_graphs, layer_groups=layer_groups,
-                                     layer_range=layer_range, pool_layers=pool_layers, pp_link=pp_link)
+                                     layer_range=layer_range, pool_layers=pool_layers, pp_link=pp_link, kv_format=kv_format)
         self.blocks = BlockAllocator(num_blocks)
         self.max_blocks_per_seq = max_blocks  # the runner's block tables are this wide
         self.geo = self.runner.geo

@@ -6,7 +6,8 @@ The reference has no engine (stock vLLM's ``GPUModelRunner`` plays this part).  
 * this rank's weight shards (bf16),
 * this rank's slice of the paged KV pool: block-scaled fp8, head-major
   ``[layer, block, k|v, head, token, dim]`` payload plus fp32 scales, which is what the fused
-  restore kernel writes into and the attention kernel reads from,
+  restore kernel writes into and the attention kernel reads from
+  (``kv_format="fp4b16"``: the 4-bit pool instead, 0.45 times the bytes per token; stored slots stay fp8),
 * persistent activation buffers, so a step allocates nothing.
 
 Per layer the step is: tcgen05 GEMM (QKV) -> RoPE + KV write -> fp8 paged attention ->
@@ -78,9 +79,15 @@ class GpuModelRunner:
     def __init__(self, cfg: LlamaConfig, weights: LlamaWeights, num_blocks: int, max_tokens: int = 256,
                  max_seqs: int = 64, tp_ctx=None, device: Optional[torch.device] = None,
                  max_blocks: int = 512, use_graphs: bool = True, layer_groups: int = 8,
-                 layer_range: Optional[range] = None, pool_layers: Optional[int] = None, pp_link=None) -> None:
+                 layer_range: Optional[range] = None, pool_layers: Optional[int] = None, pp_link=None, kv_format: str = "fp8b16") -> None:
         self.cfg = cfg
         self.w = weights
+        if kv_format not in ("fp8b16", "fp4b16"):
+            raise ValueError(f"kv_format {kv_format!r}: fp8b16 or fp4b16")
+        self.kv4 = kv_format == "fp4b16"
+        if self.kv4 and (tp_ctx is not None or (cfg.head_dim, cfg.block_tokens) != (kv_ops.KV4_DIM, kv_ops.KV4_TOKENS)
+                         or weights.heads_local > 16 * weights.kv_heads_local):
+            raise ValueError("the 4-bit pool takes head_dim 128, 16 tokens per block, up to 16 query heads per KV head, and one GPU")
         # pipeline stage: the layers this process runs, its links to the neighbouring stages
         # (``parallel/pp.py::StageLink``) and how many layers its pool and slot images have room for
         self.layers = layer_range if layer_range is not None else range(cfg.num_layers)
@@ -104,7 +111,9 @@ class GpuModelRunner:
         if n_pool_layers < len(self.layers):
             raise ValueError("the pool has fewer layers than the stage runs")
         shape = (n_pool_layers, num_blocks, 2, self.hkv, B, D)
-        if tp_ctx is not None:
+        if self.kv4:
+            self.local_pool = kv_ops.PagedKV4Pool.zeros(n_pool_layers, num_blocks, self.hkv, dev)
+        elif tp_ctx is not None:
             self.kv_payload = tp_ctx.alloc("kv_payload", shape, torch.uint8)
             self.kv_scales = tp_ctx.alloc("kv_scales", shape[:-1] + (D // 16,), torch.float32)
             self.kv_payload.zero_()
@@ -112,7 +121,8 @@ class GpuModelRunner:
         else:
             self.kv_payload = torch.zeros(shape, dtype=torch.uint8, device=dev)
             self.kv_scales = torch.ones(shape[:-1] + (D // 16,), dtype=torch.float32, device=dev)
-        self.local_pool = kv_ops.PagedKVPool.from_tensors([self.kv_payload], [self.kv_scales], "LNKHTD")
+        if not self.kv4:
+            self.local_pool = kv_ops.PagedKVPool.from_tensors([self.kv_payload], [self.kv_scales], "LNKHTD")
         # geometry of a stored slot: ALL kv heads, fp8b16
         self.geo = KVGeometry(n_pool_layers, cfg.num_kv_heads, D, B, 2, "fp8b16")
         self.cos_sin = kv_ops.rope_table(min(cfg.max_position, 32768), cfg.inv_freq(), dev)
@@ -139,6 +149,8 @@ class GpuModelRunner:
         self.best_idx = torch.zeros(max_seqs, dtype=torch.int32, device=dev)
         self.attn_ws = attention.AttentionWorkspace(dev)
         self.attn_ws.ensure(attention.MAX_ROW_SPLITS, 1, D)  # sized once: captured graphs keep its address
+        if self.kv4:  # likewise: below TC_MIN_ROWS query rows per KV head a sequence is up to TC_MIN_ROWS / 8 items
+            self.attn_ws.ensure_shared(max_seqs * self.hkv * (attention.TC_MIN_ROWS // 8))
         self.status = torch.zeros(4, dtype=torch.int32, device=dev)
         self.tile_counters = torch.zeros(4096, dtype=torch.int32, device=dev)  # split-K "last CTA of a tile" counts
         import os as _os
@@ -148,7 +160,7 @@ class GpuModelRunner:
         # default: at serving shapes these GEMMs run split-K, the fused work then falls to the one CTA
         # that completes a tile, and measured on the 70B 64-token step that serial tail costs more
         # than the launch it saves (all-warm TTFT 30.8 ms fused against 30.3 ms with the two kernels).
-        self.fuse_qkv_rope = (gemm.can_fuse_qkv_rope(D, cfg.qk_norm) and _os.environ.get("DASER_FUSE_QKV_ROPE", "0") == "1"
+        self.fuse_qkv_rope = (not self.kv4 and gemm.can_fuse_qkv_rope(D, cfg.qk_norm) and _os.environ.get("DASER_FUSE_QKV_ROPE", "0") == "1"
                               and -(-max_tokens // 128) * -(-qkv_n // 128) <= self.tile_counters.numel())
         self.fuse_swiglu_split = _os.environ.get("DASER_FUSE_SWIGLU_SPLIT", "0") == "1"
         self.softmax_scale = D**-0.5
@@ -237,6 +249,11 @@ class GpuModelRunner:
         step = 16 if n <= 128 else 64 if n <= 512 else 128
         return -(-n // step) * step
 
+    @staticmethod
+    def ctx_bucket(max_ctx: int) -> int:
+        """The context a step is planned for: powers of two, few graph shapes."""
+        return max(2048, 1 << (max(max_ctx, 1) - 1).bit_length())
+
     # -- step inputs ---------------------------------------------------------------------------------
     def stage_inputs(self, seqs: list[dict]) -> StepInputs:
         """Write one step's inputs into the runner's fixed buffers (pinned host -> device, one
@@ -320,9 +337,13 @@ class GpuModelRunner:
         if T > self.max_tokens or inp.num_seqs > self.max_seqs:
             raise ValueError("step exceeds the runner's buffers")
         group = self.hq // self.hkv
-        ctx_bucket = max(2048, 1 << (max(inp.max_ctx, 1) - 1).bit_length())  # powers of two: few graph shapes
-        nsplit, split_tokens = attention.plan_splits(inp.num_seqs, self.hkv, inp.max_q_len, group, ctx_bucket,
-                                                     self.cfg.block_tokens, rows=T * self.hq)
+        ctx_bucket = self.ctx_bucket(inp.max_ctx)
+        if self.kv4:
+            nsplit, split_tokens = attention.plan_kv4(inp.num_seqs, self.hkv, inp.max_q_len, group,
+                                                      ctx_bucket // self.cfg.block_tokens, T * self.hq)
+        else:
+            nsplit, split_tokens = attention.plan_splits(inp.num_seqs, self.hkv, inp.max_q_len, group, ctx_bucket,
+                                                         self.cfg.block_tokens, rows=T * self.hq)
         body = self._body if self.tp == 1 else (lambda *a: self.tp_ctx.forward_body(self, *a))
         shape = (T, inp.num_seqs, inp.max_q_len, nsplit, split_tokens)
         link = self.pp_link
@@ -380,9 +401,10 @@ class GpuModelRunner:
             pl = li - first  # layer index inside this stage's pool
             self.qkv_rope(normed, lw, inp, T, pl)
             attn = self.attn_out[:T].view(T, self.hq, D)
+            # (the 4-bit kernels cut the context that they are told of into nsplit: the bucket, which a replayed graph's steps share)
             attention.paged_attention(self.q_rot[:T], attn, self.local_pool, pl, inp.block_tables, inp.q_start,
-                                      inp.ctx_lens, inp.max_q_len, inp.max_ctx, self.hkv, self.softmax_scale,
-                                      self.attn_ws, nsplit=nsplit, split_tokens=split_tokens)
+                                      inp.ctx_lens, inp.max_q_len, self.ctx_bucket(inp.max_ctx) if self.kv4 else inp.max_ctx, self.hkv,
+                                      self.softmax_scale, self.attn_ws, nsplit=nsplit, split_tokens=None if self.kv4 else split_tokens)
             o, f32 = self._linear(self.attn_out[:T], lw.wo, self.hid_acc, self.hid_bf)
             ew.add_rmsnorm(o, lw.post_norm, residual=h, out=normed, eps=cfg.rms_eps, zero_after=f32)
             self.mlp_up(normed, lw, T)
@@ -416,7 +438,7 @@ class GpuModelRunner:
         if int(self.status[0].item()) != 0:
             self.status.zero_()
             raise RuntimeError("a GEMM wait ran out (status word set); the step's output is invalid")
-        if attention.tc_status() != 0:
+        if (attention.kv4_status() if self.kv4 else attention.tc_status()) != 0:
             raise RuntimeError("an attention CTA gave up on a bounded wait; the step's output is invalid")
 
 

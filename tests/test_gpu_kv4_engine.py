@@ -1,0 +1,136 @@
+"""The runner and the RAG engine on a 4-bit pool (``kv_format="fp4b16"``)."""
+
+import random
+
+import pytest
+import torch
+
+from conftest import LiveControlPlane
+from daser_b200.models.llama import PRESETS, LlamaWeights
+from test_gpu_kv4 import D, _oracle, _ops
+
+pytestmark = pytest.mark.gpu
+
+
+def _step(runner, seqs):
+    out = runner.forward(runner.stage_inputs(seqs)).clone()
+    torch.cuda.synchronize()
+    return out.tolist()
+
+
+@pytest.mark.parametrize("preset", ["tiny-gqa", "tiny-8kv", "tiny-gqa-qk"])
+def test_the_runners_attention_is_the_formula_over_its_pool(preset):
+    """After each step the last layer's queries, its pool and its attention output are still in the runner's buffers.  Prompts of
+    several lengths in one step (prefill kernel), then decode steps: eager, captured and replayed."""
+    from daser_b200.engine.runner import GpuModelRunner
+
+    cfg = PRESETS[preset]
+    w = LlamaWeights.random(cfg, "cuda", torch.bfloat16, seed=3, std=0.05)
+    runner = GpuModelRunner(cfg, w, num_blocks=64, max_tokens=256, max_seqs=8, max_blocks=32, kv_format="fp4b16")
+    rng = random.Random(0)
+    lens = [33, 7, 90]
+    perm = torch.randperm(64, generator=torch.Generator().manual_seed(1)).tolist()
+    seqs, at = [], 0
+    for n in lens:
+        need = -(-(n + 5) // 16)
+        seqs.append({"tokens": [rng.randrange(cfg.vocab_size) for _ in range(n)], "start_pos": 0, "block_table": perm[at : at + need]})
+        at += need
+    tables = torch.zeros(3, 32, dtype=torch.int64)
+    for i, s in enumerate(seqs):
+        tables[i, : len(s["block_table"])] = torch.tensor(s["block_table"])
+    for step in range(4):
+        nxt = _step(runner, seqs)
+        q_lens, ctx = [len(s["tokens"]) for s in seqs], [s["start_pos"] + len(s["tokens"]) for s in seqs]
+        T = sum(q_lens)
+        rec = runner.local_pool.keepalive[0][0][len(w.layers) - 1].cpu()
+        q = runner.q_rot[:T].float().cpu()
+        group = runner.hq // runner.hkv
+        want, tol = _oracle(rec, tables, q, q_lens, ctx, D**-0.5, prefill=max(q_lens) * group >= 64)
+        got = runner.attn_out[:T].view(T, runner.hq, D).double().cpu()
+        assert (got.isfinite().all()) and ((got - want).abs() <= tol).all(), (step, ((got - want).abs() / tol).max())
+        seqs = [{"tokens": [t], "start_pos": c, "block_table": s["block_table"]} for s, t, c in zip(seqs, nxt, ctx)]
+    runner.check_status()
+
+
+def test_replayed_steps_across_the_contexts_at_which_they_are_planned_anew():
+    """Steps of one shape share a graph over a range of context lengths.  A long prompt in pieces, then decode steps from 2040 keys on:
+    the plan changes behind 2048, every step's attention is the formula's.  (Tokens are not compared with an eager run's: projections
+    that are split along K add their parts in no fixed order.)"""
+    from daser_b200.engine.runner import GpuModelRunner
+
+    cfg = PRESETS["tiny-gqa"]
+    w = LlamaWeights.random(cfg, "cuda", torch.bfloat16, seed=5, std=0.05)
+    rng = random.Random(4)
+    prompt = [rng.randrange(cfg.vocab_size) for _ in range(2040)]
+    table = list(range(160, 160 - 131, -1))
+    runner = GpuModelRunner(cfg, w, num_blocks=161, max_tokens=256, max_seqs=4, max_blocks=256, kv_format="fp4b16")
+
+    def check(n, ctx):
+        rec = runner.local_pool.keepalive[0][0][len(w.layers) - 1].cpu()
+        want, tol = _oracle(rec, torch.tensor([table]), runner.q_rot[:n].float().cpu(), [n], [ctx], D**-0.5, prefill=n > 1)
+        got = runner.attn_out[:n].view(n, runner.hq, D).double().cpu()
+        assert ((got - want).abs() <= tol).all(), (n, ctx, ((got - want).abs() / tol).max())
+
+    for i in range(0, len(prompt), 256):
+        piece = prompt[i : i + 256]
+        token = _step(runner, [{"tokens": piece, "start_pos": i, "block_table": table}])
+    check(len(piece), len(prompt))
+    for i in range(14):
+        token = _step(runner, [{"tokens": token, "start_pos": len(prompt) + i, "block_table": table}])
+        check(1, len(prompt) + i + 1)
+    runner.check_status()
+    assert len(runner._graphs) >= 2 * len(runner.layer_groups)  # pieces of 256 tokens, decode steps
+
+
+def test_rag_engine_restores_into_a_4_bit_pool(tmp_path):
+    from daser_b200.engine.rag_gpu import GpuRagEngine, RagRequest
+
+    _, _, kv_ops = _ops()
+    cfg = PRESETS["tiny-gqa"]
+    lp = LiveControlPlane(tmp_path, total_slots=256,
+                          slot_size=cfg.num_layers * 2 * 16 * cfg.num_kv_heads * cfg.head_dim * 5 // 4).start()
+    eng = GpuRagEngine(cfg, lp.socket_path, lp.cfg.store_path, num_blocks=256, max_tokens=128, hbm_slots=64, kv_format="fp4b16")
+    try:
+        rng = random.Random(1)
+        chunks = [[rng.randrange(cfg.vocab_size) for _ in range(n)] for n in (64, 128, 48)]
+        for c in chunks:
+            eng.store_chunk(c)
+        query = [rng.randrange(cfg.vocab_size) for _ in range(20)]
+        runs = []
+        for attempt in range(2):  # from the store file, then from the HBM tier
+            req = eng.generate([chunks[2], chunks[0], chunks[1]], query, max_new_tokens=4)
+            assert req.restored_chunks == 3 and len(req.generated) == 4
+            runs.append(req.generated)
+        assert runs[0] == runs[1]  # the same slots, the same kernels
+        r = eng.submit(RagRequest([chunks[2], chunks[0]], query, 2))
+        eng._ttft_step(eng.waiting.pop(0))
+        off = len(chunks[2])
+        restored = r.block_table[off // 16 : (off + 64) // 16]
+        fresh = eng.blocks.alloc(4)
+        eng._prefill_tokens(chunks[0], off, [0] * (off // 16) + fresh)
+        slots = lambda blocks: (torch.tensor(blocks)[:, None] * 16 + torch.arange(16)).flatten().cuda()
+        pool = eng.runner.local_pool
+        # Layer 0 depends on token and position alone.  With largest magnitude A, a rounding to 4 bits is off by at most one scale, 0.178 A
+        # (A / 6 * (1 + 2^-4)); the stored value was rounded so, then to fp8 for the slot (2^-4 of itself), and again after its rotation,
+        # which mixes two values of a key (factor sqrt 2, before and behind it); the fresh one once.  2^-4: the largest value's
+        # own rounding; 2^-6: the products' order and bf16.  In the mean each rounding changes some 10 % of the root mean square.
+        for got, want, p in zip(kv_ops.kv_read(pool, 0, slots(restored)), kv_ops.kv_read(pool, 0, slots(fresh)), (2**0.5, 1.0)):
+            got, want = got.float().flatten(), want.float().flatten()
+            e1 = (0.178 + 2.0**-4 * 1.178) * p * p
+            bound = (e1 + 0.178 * (1 + e1) + 0.178 + 2.0**-6) / (1 - 2.0**-4)
+            assert (got - want).abs().max() <= bound * want.abs().max()
+            assert torch.nn.functional.cosine_similarity(got, want, dim=0) > 0.9
+        eng.runner.check_status()
+    finally:
+        eng.close()
+        lp.stop()
+
+
+def test_the_runner_refuses_what_the_pool_cannot_hold():
+    from daser_b200.engine.runner import GpuModelRunner
+
+    w = LlamaWeights.random(PRESETS["toy-qk"], "cuda", torch.bfloat16)  # head_dim 64
+    with pytest.raises(ValueError, match="head_dim 128"):
+        GpuModelRunner(PRESETS["toy-qk"], w, num_blocks=8, max_tokens=16, kv_format="fp4b16")
+    with pytest.raises(ValueError, match="kv_format"):
+        GpuModelRunner(PRESETS["toy-qk"], w, num_blocks=8, max_tokens=16, kv_format="int4")
