@@ -567,9 +567,8 @@ attn4_kernel(const Attn4Params p) {
 // out = sum_i w_i O_i / sum_i w_i, w_i = 2^(lse_i - max): one CTA per output row.  The weights are made once, then its warps
 // take the partials in turn, eight loads in flight each: a few rows with many partials (one long sequence on one KV head) are
 // a matter of latency.  The order of the sums is fixed.
-// ROWS > 0: the partials of the CTAs that share the pages (attn4_kernel with tiles of ROWS rows): the first is the
-// begun item of its CTA, the others continue it; grid (KV head, sequence, row) or (KV head, query row, head).
-// ROWS = 0: nsplit partials per row (the prefill kernel); grid (row).
+// The partials of the CTAs that share the pages (attn4_kernel with tiles of ROWS rows): the first is the begun item of its CTA, the
+// others continue it; grid (KV head, sequence, row) or (KV head, query row, head).
 constexpr int MERGE_WARPS = 4;
 constexpr int MERGE_MAX = 256;
 template <int ROWS, bool SPARSE>
@@ -584,39 +583,30 @@ attn4_merge_kernel(const Attn4Params p) {
   int64_t at0, at1;  // where the first and the second of them are
   int64_t step;      // from one to the next, from the second on
   int64_t row;       // of the output
-  if constexpr (ROWS > 0) {
-    const int kvh = blockIdx.x;
-    int r;
-    int64_t id;
-    if (SPARSE) {
-      const int tok = blockIdx.y;
-      r = blockIdx.z;
-      if (tok >= p.q_start[p.num_seqs]) return;  // behind the last sequence
-      id = (int64_t)tok * p.Hkv + kvh;
-      row = (int64_t)tok * p.Hq + kvh * p.G + r;
-    } else {
-      const int seq = blockIdx.y, in_seq = blockIdx.z;
-      const int q0 = p.q_start[seq], q1 = min(p.q_start[seq + 1], p.total_q);
-      const int tok = in_seq / p.G;
-      if (q0 < 0 || q0 + tok >= q1) return;
-      r = in_seq % ROWS;
-      id = ((int64_t)seq * p.tiles + in_seq / ROWS) * p.Hkv + kvh;
-      row = (int64_t)(q0 + tok) * p.Hq + kvh * p.G + in_seq % p.G;
-    }
-    const int2 s = p.shared[id];
-    n = s.y;
-    if (n == 1) return;  // one CTA had it all and wrote the result
-    at0 = ((int64_t)s.x * 2 + 1) * ROWS + r;
-    at1 = (int64_t)(s.x + 1) * 2 * ROWS + r;
-    step = 2 * ROWS;
+  const int kvh = blockIdx.x;
+  int r;
+  int64_t id;
+  if (SPARSE) {
+    const int tok = blockIdx.y;
+    r = blockIdx.z;
+    if (tok >= p.q_start[p.num_seqs]) return;  // behind the last sequence
+    id = (int64_t)tok * p.Hkv + kvh;
+    row = (int64_t)tok * p.Hq + kvh * p.G + r;
   } else {
-    row = blockIdx.x;
-    if (row >= (int64_t)p.q_start[p.num_seqs] * p.Hq) return;  // behind the last sequence: nobody wrote its partials
-    n = p.nsplit;
-    at0 = row * n;
-    at1 = at0 + 1;
-    step = 1;
+    const int seq = blockIdx.y, in_seq = blockIdx.z;
+    const int q0 = p.q_start[seq], q1 = min(p.q_start[seq + 1], p.total_q);
+    const int tok = in_seq / p.G;
+    if (q0 < 0 || q0 + tok >= q1) return;
+    r = in_seq % ROWS;
+    id = ((int64_t)seq * p.tiles + in_seq / ROWS) * p.Hkv + kvh;
+    row = (int64_t)(q0 + tok) * p.Hq + kvh * p.G + in_seq % p.G;
   }
+  const int2 s = p.shared[id];
+  n = s.y;
+  if (n == 1) return;  // one CTA had it all and wrote the result
+  at0 = ((int64_t)s.x * 2 + 1) * ROWS + r;
+  at1 = (int64_t)(s.x + 1) * 2 * ROWS + r;
+  step = 2 * ROWS;
   auto where = [&](int i) { return i == 0 ? at0 : at1 + (i - 1) * step; };
   // NaN marks a row that saw one: it has to survive the maximum
   float lse[MERGE_MAX / (MERGE_WARPS * 32)], wm = -INFINITY;
@@ -668,11 +658,49 @@ attn4_merge_kernel(const Attn4Params p) {
   p.out[row * ATT_D + tid] = __float2bfloat16(total == 0.f ? 0.f : v / total);  // no key: zeros
 }
 
+// The same for nsplit partials per row, one behind the other (the prefill kernel's): many rows with few partials, a warp per row.
+__global__ void __launch_bounds__(MERGE_WARPS * 32)
+attn4_merge_rows_kernel(const Attn4Params p) {
+  const int lane = threadIdx.x & 31;
+  pdl_enter();
+  const int64_t row = (int64_t)blockIdx.x * MERGE_WARPS + (threadIdx.x >> 5);
+  if (row >= (int64_t)min(p.q_start[p.num_seqs], p.total_q) * p.Hq) return;  // behind the last sequence: nobody wrote its partials
+  const int n = p.nsplit;
+  const float* lse = p.part_lse + row * n;
+  const float* part = p.part_o + row * n * ATT_D + 4 * lane;
+  float wm = -INFINITY;
+  for (int i = lane; i < n; i += 32) wm = fmaxf(wm, lse[i] != lse[i] ? INFINITY : lse[i]);  // a NaN has to survive the maximum
+  const float mx = warp_max(wm);
+  float total = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const float mine = i0 + lane < n ? lse[i0 + lane] : -INFINITY;
+    const float wt = mine != mine ? NAN : (mine == -INFINITY ? 0.f : ex2f(mine - mx));
+    total += wt;
+    for (int i = 0; i < 32 && i0 + i < n; i += 8) {
+      float4 x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        x[u] = i0 + i + u < n ? *reinterpret_cast<const float4*>(part + (int64_t)(i0 + i + u) * ATT_D) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float w = __shfl_sync(0xffffffffu, wt, i + u);  // (0 behind the last)
+        acc.x += w * x[u].x; acc.y += w * x[u].y; acc.z += w * x[u].z; acc.w += w * x[u].w;
+      }
+    }
+  }
+  total = warp_sum(total);
+  auto div = [&](float v) { return total == 0.f ? 0.f : v / total; };  // no key: zeros
+  uint2 w2;
+  w2.x = pack_bf16x2(div(acc.x), div(acc.y));
+  w2.y = pack_bf16x2(div(acc.z), div(acc.w));
+  *reinterpret_cast<uint2*>(p.out + row * ATT_D + 4 * lane) = w2;
+}
+
 template <int ROWS, bool SPARSE>
 static int launch_merge(const Attn4Params& p, int max_q_len, cudaStream_t stream) {
-  const dim3 grid = ROWS == 0 ? dim3((unsigned)(p.total_q * p.Hq))
-                    : SPARSE  ? dim3((unsigned)p.Hkv, (unsigned)p.total_q, (unsigned)p.G)
-                              : dim3((unsigned)p.Hkv, (unsigned)p.num_seqs, (unsigned)(max_q_len * p.G));
+  const dim3 grid = SPARSE ? dim3((unsigned)p.Hkv, (unsigned)p.total_q, (unsigned)p.G)
+                           : dim3((unsigned)p.Hkv, (unsigned)p.num_seqs, (unsigned)(max_q_len * p.G));
   return (int)launch_pdl(attn4_merge_kernel<ROWS, SPARSE>, grid, dim3(MERGE_WARPS * 32), 0, stream, p);
 }
 
@@ -758,7 +786,9 @@ DASER_API int daser_paged_attention_kv4(const void* q, void* out, float* part_o,
     p.nsplit = parts;
     p.split_pages = split_pages;
     const int rc = daser_launch_attention4_tc(p, max_q_len, stream);
-    return rc || parts == 1 ? rc : launch_merge<0, false>(p, 0, stream);
+    if (rc || parts == 1) return rc;
+    const unsigned ctas = (unsigned)(((int64_t)total_q * Hq + MERGE_WARPS - 1) / MERGE_WARPS);
+    return (int)launch_pdl(attn4_merge_rows_kernel, dim3(ctas), dim3(MERGE_WARPS * 32), 0, stream, p);
   }
   p.workers = parts;
   if (parts && !shared) return DASER_ERR_BAD_ARG;

@@ -156,6 +156,26 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
     return;
   }
 
+  // Q: half a warp reads a row of 256 bytes, two rows an instruction (a row per thread took 8000 cycles, tags bound).  The loads are out
+  // before the barriers are set up, and so are those of the first block ids.
+  uint4 qw[16];
+  if (tile < tiles) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int src = 2 * i + (lane >> 4);
+      const int64_t r = __shfl_sync(0xffffffffu, row, src);
+      const bool live = __shfl_sync(0xffffffffu, (int)valid, src) != 0;
+      qw[i] = live ? *reinterpret_cast<const uint4*>(p.q + r * ATT_D + (lane & 15) * 8) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  const int32_t* table = p.block_tables + (int64_t)seq * p.max_blocks;
+  int blk[T4_PAGES];
+  auto ids = [&](int ti) {  // a tile ahead of the copies that need them
+#pragma unroll
+    for (int pg = 0; pg < T4_PAGES; ++pg) blk[pg] = __ldg(table + min(page_begin + ti * T4_PAGES + pg, p.max_blocks - 1));
+  };
+  if (warp == 13) ids(0);
+
   const uint32_t q_u32 = smem_u32(q_s), k_u32 = smem_u32(k_s), vt_u32 = smem_u32(vt_s), raw_u32 = smem_u32(raw_s);
   if (tid == 0) {
 #pragma unroll
@@ -197,19 +217,17 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
       const uint32_t tmem_o = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t4_o_col(tile);
       const uint32_t tmem_p = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t4_p_col(tile);
       uint8_t* my_q = q_s + tile * T4_Q_BYTES;
-      {  // Q row -> f16, times scale * log2(e), into the swizzled A tile
-        const __nv_bfloat16* qp = p.q + row * ATT_D;
+      // Q -> f16, times scale * log2(e), into the swizzled A tile
 #pragma unroll
-        for (int ck = 0; ck < 16; ++ck) {
-          uint4 w = make_uint4(0u, 0u, 0u, 0u);
-          if (valid) w = *reinterpret_cast<const uint4*>(qp + ck * 8);
-          uint4 h;
-          h.x = pack_half2(bf16_lo(w.x) * p.scale_log2, bf16_hi(w.x) * p.scale_log2);
-          h.y = pack_half2(bf16_lo(w.y) * p.scale_log2, bf16_hi(w.y) * p.scale_log2);
-          h.z = pack_half2(bf16_lo(w.z) * p.scale_log2, bf16_hi(w.z) * p.scale_log2);
-          h.w = pack_half2(bf16_lo(w.w) * p.scale_log2, bf16_hi(w.w) * p.scale_log2);
-          *reinterpret_cast<uint4*>(my_q + (ck >> 3) * 16384 + rt * 128 + ((((ck & 7) ^ (rt & 7))) << 4)) = h;
-        }
+      for (int i = 0; i < 16; ++i) {
+        const int r = (warp & 3) * 32 + 2 * i + (lane >> 4), ck = lane & 15;
+        const uint4 w = qw[i];
+        uint4 h;
+        h.x = pack_half2(bf16_lo(w.x) * p.scale_log2, bf16_hi(w.x) * p.scale_log2);
+        h.y = pack_half2(bf16_lo(w.y) * p.scale_log2, bf16_hi(w.y) * p.scale_log2);
+        h.z = pack_half2(bf16_lo(w.z) * p.scale_log2, bf16_hi(w.z) * p.scale_log2);
+        h.w = pack_half2(bf16_lo(w.w) * p.scale_log2, bf16_hi(w.w) * p.scale_log2);
+        *reinterpret_cast<uint4*>(my_q + (ck >> 3) * 16384 + r * 128 + (((ck & 7) ^ (r & 7)) << 4)) = h;
       }
       t4_fence_async();
       __syncwarp();
@@ -282,32 +300,42 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
         tmem_ld_wait();
         const float l = __uint_as_float(r[0]);
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays
+        // Through shared memory, so that half a warp writes 256 bytes of a row (a row per thread: 11000 cycles for the partials).  The Q
+        // tile's scores are all done, it is free: 8 KB per warp, [32 rows][16 pieces of 16 bytes], piece ^ (row & 7).
+        uint8_t* stage = my_q + (warp & 3) * 8192;
+        const bool partial = p.nsplit > 1;
+        const int64_t at = partial ? (row * p.nsplit + sp) * (ATT_D * 4) : row * (ATT_D * 2);  // bytes
+        uint8_t* const dst = (partial ? reinterpret_cast<uint8_t*>(p.part_o) : reinterpret_cast<uint8_t*>(p.out)) + (lane & 15) * 16;
+        auto put = [&](int c, uint4 w) { *reinterpret_cast<uint4*>(stage + lane * 256 + ((c ^ (lane & 7)) << 4)) = w; };
+        auto flush = [&](int off) {
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int src = 2 * i + (lane >> 4);
+            const int64_t to = __shfl_sync(0xffffffffu, at, src);
+            const bool live = __shfl_sync(0xffffffffu, (int)valid, src) != 0;
+            const uint4 w = *reinterpret_cast<const uint4*>(stage + src * 256 + (((lane & 15) ^ (src & 7)) << 4));
+            if (live) *reinterpret_cast<uint4*>(dst + to + off) = w;
+          }
+          __syncwarp();
+        };
 #pragma unroll
         for (int cc = 0; cc < 4; ++cc) {
-          __syncwarp();  // reconverge after the predicated stores of the previous chunk
           tmem_ld_32x32(tmem_o + 32 * cc, r);
           tmem_ld_wait();
-          if (!valid) continue;
-          if (p.nsplit == 1) {
-            __nv_bfloat16* dst = p.out + row * ATT_D + 32 * cc;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              uint4 w;
-              w.x = pack_bf16x2(__uint_as_float(r[8 * x]) * inv, __uint_as_float(r[8 * x + 1]) * inv);
-              w.y = pack_bf16x2(__uint_as_float(r[8 * x + 2]) * inv, __uint_as_float(r[8 * x + 3]) * inv);
-              w.z = pack_bf16x2(__uint_as_float(r[8 * x + 4]) * inv, __uint_as_float(r[8 * x + 5]) * inv);
-              w.w = pack_bf16x2(__uint_as_float(r[8 * x + 6]) * inv, __uint_as_float(r[8 * x + 7]) * inv);
-              *reinterpret_cast<uint4*>(dst + 8 * x) = w;
-            }
+          for (int x = 0; x < 32; ++x) r[x] = __float_as_uint(__uint_as_float(r[x]) * inv);
+          if (partial) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) put((cc & 1) * 8 + x, make_uint4(r[4 * x], r[4 * x + 1], r[4 * x + 2], r[4 * x + 3]));
+            if (cc & 1) flush((cc >> 1) * 256);
           } else {
-            float* dst = p.part_o + (row * p.nsplit + sp) * ATT_D + 32 * cc;
+            auto two = [&](int k) { return pack_bf16x2(__uint_as_float(r[k]), __uint_as_float(r[k + 1])); };
 #pragma unroll
-            for (int x = 0; x < 8; ++x)
-              *reinterpret_cast<float4*>(dst + 4 * x) =
-                  make_float4(__uint_as_float(r[4 * x]) * inv, __uint_as_float(r[4 * x + 1]) * inv,
-                              __uint_as_float(r[4 * x + 2]) * inv, __uint_as_float(r[4 * x + 3]) * inv);
+            for (int x = 0; x < 4; ++x) put(cc * 4 + x, make_uint4(two(8 * x), two(8 * x + 2), two(8 * x + 4), two(8 * x + 6)));
           }
         }
+        if (!partial) flush(0);
         if (valid && p.nsplit > 1) p.part_lse[row * p.nsplit + sp] = l > 0.f ? m + log2f(l) : (l == 0.f ? -INFINITY : l);
         __syncwarp();
       }
@@ -458,14 +486,7 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
     if (!t4_wait(&bars.drain, 0, &none)) ok = false;
   } else if (lane == 0) {
     // ======== fetch ========
-    const int32_t* table = p.block_tables + (int64_t)seq * p.max_blocks;
     const uint8_t* base = p.records + (int64_t)kvh * p.stride_head;
-    int blk[T4_PAGES];
-    auto ids = [&](int ti) {  // a tile ahead of the copies that need them
-#pragma unroll
-      for (int pg = 0; pg < T4_PAGES; ++pg) blk[pg] = __ldg(table + min(page_begin + ti * T4_PAGES + pg, p.max_blocks - 1));
-    };
-    ids(0);
     int issued = 0;
     for (; issued < n_tiles; ++issued) {
       const int s = issued % T4_STAGES;
