@@ -541,11 +541,12 @@ attn4_kernel(const Attn4Params p) {
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-      if (s_m[w][r] == -INFINITY) continue;  // saw no key: its part may not even be there
-      const float f = ex2f(s_m[w][r] - ref);
-      const float4 v = *reinterpret_cast<const float4*>(a4_smem + s_part[w] + (r * A4_OPITCH + 4 * lane) * 4);
+      // a warp that saw no key: its part may not even be there.  No branch, so that the loads of all warps' parts go out together.
+      const bool there = s_m[w][r] != -INFINITY;
+      const float f = there ? ex2f(s_m[w][r] - ref) : 0.f;
+      const float4 v = *reinterpret_cast<const float4*>(a4_smem + max(s_part[w], 0) + (r * A4_OPITCH + 4 * lane) * 4);
       lt += f * s_l[w][r];
-      acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+      acc.x += there ? f * v.x : 0.f; acc.y += there ? f * v.y : 0.f; acc.z += there ? f * v.z : 0.f; acc.w += there ? f * v.w : 0.f;
     }
     const float inv = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);  // no key: zeros; NaN stays
     if (whole) {
@@ -727,7 +728,7 @@ static int fill_attn4(Attn4Params& p, const void* q, void* out, float* part_o, f
   const int Hkv = pool->heads_per_rank;
   if (Hq <= 0 || Hq % Hkv || num_seqs < 0 || total_q < 0 || max_q_len < 0 || max_blocks <= 0) return DASER_ERR_BAD_ARG;
   if (parts < 0 || (parts > 1 && (!part_o || !part_lse))) return DASER_ERR_BAD_ARG;
-  if (parts > MERGE_MAX || max_blocks > 0x7fffffff / DASER_KV4_TOKENS || total_q > 0x7fffffff / Hq) return DASER_ERR_TOO_LARGE;
+  if (parts > MERGE_MAX || max_blocks > (1 << 29) / DASER_KV4_TOKENS || total_q > 0x7fffffff / Hq) return DASER_ERR_TOO_LARGE;
   if (Hq / Hkv > 16) return DASER_ERR_UNSUPPORTED;
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)part_o) % 16) return DASER_ERR_UNSUPPORTED;
   p.q = (const __nv_bfloat16*)q;

@@ -294,7 +294,7 @@ DASER_API int daser_select_pages_kv4(const void* q, const int8_t* codes, const i
   if (!q || !codes || !exps || !block_tables || !q_start || !ctx_lens || !scores || !pages) return DASER_ERR_BAD_ARG;
   if (Hq / Hkv > 16 || (uintptr_t)codes % 16) return DASER_ERR_UNSUPPORTED;
   const int64_t rows = (int64_t)num_seqs * max_q_len;
-  if (rows > 65535 || Hkv > 65535 || max_blocks > 0x7fffffff / DASER_KV4_TOKENS) return DASER_ERR_TOO_LARGE;
+  if (rows > 65535 || Hkv > 65535 || max_blocks > (1 << 29) / DASER_KV4_TOKENS) return DASER_ERR_TOO_LARGE;
   Select4Params p;
   p.q = (const __nv_bfloat16*)q;
   p.codes = codes + (int64_t)layer * num_blocks * Hkv * 2 * ATT_D;
