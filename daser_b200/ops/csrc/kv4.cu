@@ -9,7 +9,7 @@ namespace daser {
 
 #define KV4_ERR_BLOCK_RANGE 2u
 #define KV4_ERR_DELTA_RANGE 3u
-#define KV4_ERR_NULL_SLOT 4u
+#define KV4_ERR_NULL_SLOT 4u  // or an image off the 16-byte grid
 
 __device__ __forceinline__ void kv4_report(uint32_t* status, uint32_t code, uint32_t slot) {
   if (status != nullptr && atomicCAS(status, 0u, code) == 0u) status[1] = slot;
@@ -237,7 +237,7 @@ kv4_restore_kernel(const DaserKVJob job, const DaserKV4Pool pool) {
   const int64_t adelta = delta < 0 ? -(int64_t)delta : delta;
   uint32_t bad = 0;
   if (block < 0 || block >= pool.num_blocks) bad = KV4_ERR_BLOCK_RANGE;
-  else if (img == 0) bad = KV4_ERR_NULL_SLOT;
+  else if (img == 0 || img % 16 != 0) bad = KV4_ERR_NULL_SLOT;
   else if (delta != 0 && adelta >= job.max_pos) bad = KV4_ERR_DELTA_RANGE;
   if (bad) {
     if (threadIdx.x == 0) kv4_report(job.status, bad, slot);
@@ -341,8 +341,8 @@ kv4_save_kernel(const DaserKVJob job, const DaserKV4Pool pool) {
   const int slot = blockIdx.x / job.num_layers, layer = blockIdx.x % job.num_layers;
   const int block = job.block_id[slot];
   const uint64_t img = job.slot_ptr[slot];
-  if (block < 0 || block >= pool.num_blocks || img == 0) {
-    if (threadIdx.x == 0) kv4_report(job.status, img == 0 && block >= 0 && block < pool.num_blocks ? KV4_ERR_NULL_SLOT : KV4_ERR_BLOCK_RANGE, slot);
+  if (block < 0 || block >= pool.num_blocks || img == 0 || img % 16 != 0) {
+    if (threadIdx.x == 0) kv4_report(job.status, block >= 0 && block < pool.num_blocks ? KV4_ERR_NULL_SLOT : KV4_ERR_BLOCK_RANGE, slot);
     return;
   }
   int first, owned;  // heads of this rank inside the all-head image
@@ -643,6 +643,8 @@ DASER_API int daser_kv4_bounds_read(const int8_t* codes, const int8_t* exps, int
 DASER_API int daser_quant_fp4b16(const void* x, void* codes, void* scales, int64_t n_elems, cudaStream_t stream) {
   if (n_elems < 0 || n_elems % 16) return DASER_ERR_BAD_ARG;
   if (n_elems == 0) return 0;
+  if (!x || !codes || !scales) return DASER_ERR_BAD_ARG;
+  if ((uintptr_t)x % 16 || (uintptr_t)codes % 8) return DASER_ERR_UNSUPPORTED;
   const int64_t g = n_elems / 16, blocks = (g + 255) / 256;
   daser::quant_fp4b16_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, stream>>>((const __nv_bfloat16*)x, (uint8_t*)codes,
                                                                                             (uint8_t*)scales, g);
@@ -652,6 +654,8 @@ DASER_API int daser_quant_fp4b16(const void* x, void* codes, void* scales, int64
 DASER_API int daser_dequant_fp4b16(const void* codes, const void* scales, void* y, int64_t n_elems, cudaStream_t stream) {
   if (n_elems < 0 || n_elems % 16) return DASER_ERR_BAD_ARG;
   if (n_elems == 0) return 0;
+  if (!codes || !scales || !y) return DASER_ERR_BAD_ARG;
+  if ((uintptr_t)codes % 8 || (uintptr_t)y % 16) return DASER_ERR_UNSUPPORTED;
   const int64_t g = n_elems / 16, blocks = (g + 255) / 256;
   daser::dequant_fp4b16_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales,
                                                                                               (__nv_bfloat16*)y, g);

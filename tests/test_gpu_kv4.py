@@ -225,6 +225,23 @@ def test_restore_and_save_report_bad_slots_instead_of_faulting():
         kv_ops.kv_restore(work, KVGeometry(2, 2, D, B, 2, "fp8b16"), pool, table, status)   # more layers than the pool
 
 
+@pytest.mark.parametrize("img", ["fp8b16", "raw"])
+def test_an_image_off_the_16_byte_grid_is_reported(img):
+    _, _, kv_ops = _ops()
+    geo = KVGeometry(1, 2, D, B, 2, img)
+    image = torch.zeros(geo.slot_size + 16, dtype=torch.uint8, device="cuda")
+    records, pool = _pools(kv_ops, geo, 4, 1)
+    before = [r.clone() for r in records]
+    for off in (1, 4, 8):
+        work = kv_ops.KVWorkList(torch.tensor([image.data_ptr() + off], dtype=torch.int64, device="cuda"),
+                                 torch.tensor([2], dtype=torch.int32, device="cuda"))
+        for call in (lambda s: kv_ops.kv_restore(work, geo, pool, None, s), lambda s: kv_ops.kv_save(work, geo, pool, 0, s)):
+            status = torch.zeros(2, dtype=torch.int32, device="cuda")
+            call(status)
+            assert status.tolist() == [4, 0]
+    assert all(torch.equal(a, b) for a, b in zip(records, before)) and not image.any()
+
+
 # -- attention ---------------------------------------------------------------------------
 
 

@@ -220,6 +220,20 @@ def test_c_entry_points_refuse_bad_arguments():
     assert att(a, a, None, None, None, p, 0, 0, a, 4, a, a, 0, 0, 0, 8, 0, 0, 1.0, None) == 0
 
 
+@pytest.mark.parametrize("off,code", [((2, 0, 0), -2), ((8, 0, 0), -2), ((0, 4, 0), -2), ((0, 1, 0), -2)])
+def test_the_codec_refuses_addresses_off_its_vectors(off, code):
+    """bf16 values are read 16 bytes at a time, codes 8: a view that starts elsewhere is refused before a launch."""
+    from daser_b200.ops import _lib
+
+    a = 1 << 21
+    x, codes, scales = a + off[0], a + off[1], a + off[2]
+    assert _lib.kv4_fn("daser_quant_fp4b16")(x, codes, scales, 64, None) == code
+    assert _lib.kv4_fn("daser_dequant_fp4b16")(codes, scales, x, 64, None) == code
+    for args in ((None, a, a), (a, None, a), (a, a, None)):
+        assert _lib.kv4_fn("daser_quant_fp4b16")(*args, 64, None) == -1
+        assert _lib.kv4_fn("daser_dequant_fp4b16")(*args, 64, None) == -1
+
+
 def test_plans_cover_the_context():
     from daser_b200.ops import attention
 
