@@ -581,7 +581,7 @@ DASER_API int daser_kv4_restore(const DaserKVJob* job, const DaserKV4Pool* pool,
   if (int e = kv4_check_job(*job, *pool)) return e;
   if (job->n_slots == 0) return 0;
   if (!job->slot_ptr || !job->block_id || (job->delta && (!job->cos_sin || job->max_pos <= 0))) return DASER_ERR_BAD_ARG;
-  if (job->layer_begin < 0 || job->layer_count < 0 || job->layer_begin + job->layer_count > job->num_layers) return DASER_ERR_BAD_ARG;
+  if (job->layer_begin < 0 || job->layer_count < 0 || (int64_t)job->layer_begin + job->layer_count > job->num_layers) return DASER_ERR_BAD_ARG;
   DaserKVJob j = *job;
   j.layer_count = job->layer_count > 0 ? job->layer_count : job->num_layers - job->layer_begin;
   if (j.layer_count <= 0) return 0;

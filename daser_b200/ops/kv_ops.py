@@ -203,6 +203,10 @@ class PagedKV4Pool:
     def zeros(cls, num_layers: int, num_blocks: int, num_heads: int, device) -> "PagedKV4Pool":
         return cls.from_tensors([torch.zeros(num_layers, num_blocks, num_heads, KV4_RECORD, dtype=torch.uint8, device=device)])
 
+    def c_struct(self):
+        """What the operators of a :class:`PagedKVPool` alone ask for."""
+        raise ValueError("this operator takes a PagedKVPool, not a 4-bit pool")
+
     def check(self, layer: int, rank: int) -> None:
         if self.index < 0:
             raise ValueError("the pool's kernels need a CUDA device")
@@ -314,6 +318,19 @@ def _job(work, geo, image_is_fp8, cos_sin, status, rank=0) -> KVJob:
     return j
 
 
+def _check_work4(work: KVWorkList, geo, pool: PagedKV4Pool, cos_sin, status) -> None:
+    """The tensors of a restore or save of a 4-bit pool: the kernels read them as they are described here."""
+    for t, name, dtype in ((work.slot_ptrs, "slot_ptrs", torch.int64), (work.block_ids, "block_ids", torch.int32),
+                           (work.deltas, "deltas", torch.int32), (cos_sin, "cos_sin", torch.float32), (status, "status", torch.int32)):
+        if t is not None:
+            _lib.check_tensor(t, name, dtype, pool.index)
+    n = work.n_slots
+    _lib.require(work.slot_ptrs.numel() == n and (work.deltas is None or work.deltas.numel() == n), "one entry per slot in slot_ptrs and deltas")
+    _lib.require(cos_sin is None or (cos_sin.dim() == 2 and cos_sin.shape[1] == KV4_DIM), "cos_sin: [positions, 128]")
+    _lib.require(status is None or status.numel() >= 2, "status: two words")
+    _lib.require(geo.codec == "fp8b16" or geo.dtype_bytes == 2, "images of a 4-bit pool are fp8b16 or bf16")
+
+
 def kv_restore(work: KVWorkList, geo, pool: PagedKVPool | PagedKV4Pool, cos_sin: Optional[torch.Tensor],
                status: Optional[torch.Tensor] = None, stream=None, layer_begin: int = 0,
                layer_count: int = 0) -> None:
@@ -328,6 +345,7 @@ def kv_restore(work: KVWorkList, geo, pool: PagedKVPool | PagedKV4Pool, cos_sin:
     job.layer_begin, job.layer_count = int(layer_begin), int(layer_count)
     if isinstance(pool, PagedKV4Pool):
         pool.check(0, 0)
+        _check_work4(work, geo, pool, cos_sin, status)
         _lib.call_on(pool.index, _lib.kv4_fn("daser_kv4_restore"), "kv4_restore", C.addressof(job), pool.c_ptr, stream=stream)
         return
     pool_c = pool.c_struct()
@@ -343,6 +361,7 @@ def kv_save(work: KVWorkList, geo, pool: PagedKVPool | PagedKV4Pool, rank: int =
     job = _job(work, geo, geo.codec == "fp8b16", None, status, rank)
     if isinstance(pool, PagedKV4Pool):
         pool.check(0, rank)
+        _check_work4(work, geo, pool, None, status)
         _lib.call_on(pool.index, _lib.kv4_fn("daser_kv4_save"), "kv4_save", C.addressof(job), pool.c_ptr, stream=stream)
         return
     pool_c = pool.c_struct()

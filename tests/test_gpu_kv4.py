@@ -787,3 +787,31 @@ def test_refusals_on_the_gpu():
                    dict(qk_norm=(x[0, :128], x[0, :128], 1e-6))):
         with pytest.raises(ValueError):
             ew.rope_kv_write(**{**one, **change})
+
+
+def test_work_lists_that_do_not_fit_are_refused():
+    _, _, kv_ops = _ops()
+    geo = KVGeometry(1, 2, D, B, 2, "fp8b16")
+    _, pool = _pools(kv_ops, geo, 4, 1)
+    image = torch.zeros(geo.slot_size, dtype=torch.uint8, device="cuda")
+    ptr, blk, dlt = (torch.tensor([v], dtype=t, device="cuda") for v, t in ((image.data_ptr(), torch.int64), (0, torch.int32), (1, torch.int32)))
+    table = kv_ops.rope_table(32, inv_freq_table(D, 10000.0), "cuda")
+    status = torch.zeros(2, dtype=torch.int32, device="cuda")
+    W = kv_ops.KVWorkList
+    kv_ops.kv_restore(W(ptr, blk, dlt), geo, pool, table, status)
+    for work in (W(ptr.int(), blk), W(ptr, blk.long()), W(ptr, blk, dlt.long()), W(ptr, blk.repeat(2)), W(ptr, blk, dlt[:0]), W(ptr.cpu(), blk),
+                 W(ptr.repeat(2), blk.repeat(4)[::2], None)):
+        with pytest.raises(ValueError):
+            kv_ops.kv_restore(work, geo, pool, table, status)
+        with pytest.raises(ValueError):
+            kv_ops.kv_save(work, geo, pool, 0, status)
+    for bad in (table[:, :64], table.double(), table.cpu()):
+        with pytest.raises(ValueError):
+            kv_ops.kv_restore(W(ptr, blk, dlt), geo, pool, bad, status)
+    for bad in (status[:1], status.long()):
+        with pytest.raises(ValueError):
+            kv_ops.kv_restore(W(ptr, blk, dlt), geo, pool, table, bad)
+    with pytest.raises(ValueError):
+        kv_ops.kv_restore(W(ptr, blk), KVGeometry(1, 2, D, B, 4, "raw"), pool, None, status)  # four bytes a value
+    with pytest.raises(ValueError):
+        pool.c_struct()  # operators of the fp8 pool
