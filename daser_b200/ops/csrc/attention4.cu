@@ -91,7 +91,7 @@ __device__ __forceinline__ SeqInfo seq_info(const Attn4Params& p, int seq) {
   s.q0 = p.q_start[seq];
   const int q1 = p.q_start[seq + 1];
   s.q_all = q1 - s.q0;
-  s.q_len = s.q0 < 0 ? 0 : max(0, min(q1, p.total_q) - s.q0);
+  s.q_len = s.q0 < 0 ? 0 : min(max(0, min(q1, p.total_q) - s.q0), p.max_q_len);
   s.ctx = p.ctx_lens[seq];
   return s;
 }
@@ -604,7 +604,8 @@ attn4_merge_kernel(const Attn4Params p) {
   }
   const int2 s = p.shared[id];
   n = s.y;
-  if (n == 1) return;  // one CTA had it all and wrote the result
+  // 1: one CTA had it all and wrote the result.  (The rest: a row that no sequence has, in a list that is not one of prefix sums.)
+  if (n < 2 || s.x < 0 || n > p.workers - s.x) return;
   at0 = ((int64_t)s.x * 2 + 1) * ROWS + r;
   at1 = (int64_t)(s.x + 1) * 2 * ROWS + r;
   step = 2 * ROWS;
@@ -664,8 +665,9 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32)
 attn4_merge_rows_kernel(const Attn4Params p) {
   const int lane = threadIdx.x & 31;
   pdl_enter();
-  const int64_t row = (int64_t)blockIdx.x * MERGE_WARPS + (threadIdx.x >> 5);
-  if (row >= (int64_t)min(p.q_start[p.num_seqs], p.total_q) * p.Hq) return;  // behind the last sequence: nobody wrote its partials
+  const int q0 = p.q_start[blockIdx.y], q_len = min(min(p.q_start[blockIdx.y + 1], p.total_q) - q0, p.max_q_len);
+  const int64_t in_seq = (int64_t)blockIdx.x * MERGE_WARPS + (threadIdx.x >> 5), row = (int64_t)q0 * p.Hq + in_seq;
+  if (q0 < 0 || q_len <= 0 || in_seq >= (int64_t)q_len * p.Hq) return;  // a row of no sequence: nobody wrote its partials
   const int n = p.nsplit;
   const float* lse = p.part_lse + row * n;
   const float* part = p.part_o + row * n * ATT_D + 4 * lane;
@@ -714,6 +716,7 @@ static int launch_attn4(Attn4Params& p, int max_q_len, cudaStream_t stream) {
     cudaError_t e = cudaFuncSetAttribute(attn4_kernel<NT, SPARSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;
   }
+  p.max_q_len = SPARSE ? p.total_q : max_q_len;  // (`shared` is by token in the sparse form)
   p.tiles = SPARSE ? max_q_len : (max_q_len * p.G + C::ROWS - 1) / C::ROWS;
   if (p.tiles > 65535 || p.num_seqs > 65535 || (SPARSE && p.total_q > 65535)) return DASER_ERR_TOO_LARGE;
   const dim3 grid = p.workers ? dim3((unsigned)p.workers) : dim3((unsigned)p.Hkv, (unsigned)p.num_seqs, (unsigned)p.tiles);
@@ -785,11 +788,12 @@ DASER_API int daser_paged_attention_kv4(const void* q, void* out, float* part_o,
   if (!q || !out || !block_tables || !q_start || !ctx_lens) return DASER_ERR_BAD_ARG;
   if (rows >= A4_TC_MIN_ROWS) {
     p.nsplit = parts;
+    p.max_q_len = max_q_len;
     p.split_pages = split_pages;
     const int rc = daser_launch_attention4_tc(p, max_q_len, stream);
     if (rc || parts == 1) return rc;
-    const unsigned ctas = (unsigned)(((int64_t)total_q * Hq + MERGE_WARPS - 1) / MERGE_WARPS);
-    return (int)launch_pdl(attn4_merge_rows_kernel, dim3(ctas), dim3(MERGE_WARPS * 32), 0, stream, p);
+    const int64_t ctas = ((int64_t)max_q_len * Hq + MERGE_WARPS - 1) / MERGE_WARPS;  // (max_q_len: bounded by the launch in front)
+    return (int)launch_pdl(attn4_merge_rows_kernel, dim3((unsigned)ctas, (unsigned)num_seqs), dim3(MERGE_WARPS * 32), 0, stream, p);
   }
   p.workers = parts;
   if (parts && !shared) return DASER_ERR_BAD_ARG;

@@ -25,6 +25,7 @@ struct Attn4Params {
   int nsplit, split_pages;      // prefill: splits of a context, of split_pages pages each
   float scale_log2;             // softmax scale * log2(e)
   int total_q;
+  int max_q_len;                // query tokens of a sequence beyond it are left alone (decode: `shared` has no place for them)
 };
 
 __device__ __forceinline__ float ex2f(float x) {

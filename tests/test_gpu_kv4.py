@@ -815,3 +815,51 @@ def test_work_lists_that_do_not_fit_are_refused():
         kv_ops.kv_restore(W(ptr, blk), KVGeometry(1, 2, D, B, 4, "raw"), pool, None, status)  # four bytes a value
     with pytest.raises(ValueError):
         pool.c_struct()  # operators of the fp8 pool
+
+
+@pytest.mark.parametrize("split", [0, 5])
+def test_query_tokens_beyond_max_q_len_are_left_alone(split):
+    """A caller's max_q_len that is too small: rows below it are right, and nothing is written outside the call's own memory."""
+    attention, _, kv_ops = _ops()
+    q_lens, ctx_lens = [3, 9, 2], [300, 900, 500]
+    pool, rec, tables, q, start = _setup(q_lens, ctx_lens, 8, 2, seed=71)
+    ws = attention.AttentionWorkspace(torch.device("cuda"))
+    ws.ensure(16, 148, D)
+    places = ws.ensure_shared(200)
+    places.fill_(77)
+    out = _attend(pool, 0, tables, q, start, ctx_lens, 2, 2, split, ws)
+    want, tol = _oracle(rec[0], tables, q, q_lens, ctx_lens, D**-0.5)
+    at = 0
+    for n in q_lens:
+        assert ((out - want).abs() <= tol)[at : at + 2].all()
+        assert (out[at + 2 : at + n] == 7.0).all()
+        at += n
+    assert (places[2 * 3 * 2 :] == 77).all()  # 3 sequences x one tile x 2 KV heads, two words each
+
+
+def test_rows_in_front_of_the_first_sequence_are_left_alone():
+    attention, _, kv_ops = _ops()
+    pool, rec, tables, q, start = _setup([1, 1], [700, 900], 8, 2, seed=72, extra_rows=3)
+    start = start + 2  # rows 0, 1 belong to nobody; the places of their items are whatever the workspace holds
+    q = torch.cat([q[2:4], q])[: 2 + 2 + 1]
+    pages = torch.arange(12, dtype=torch.int32).expand(5, 2, 12).contiguous().cuda()
+    c = torch.tensor([700, 900], dtype=torch.int32, device="cuda")
+    for junk in (0, 1, 3, 2**30, -5):
+        ws = attention.AttentionWorkspace(torch.device("cuda"))
+        ws.ensure(16, 148, D)
+        ws.ensure_shared(64).fill_(junk)
+        out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device="cuda")
+        attention._attention_kv4(q.cuda(), out, pool, 0, tables.cuda(), start.cuda(), c, 1, 0, D**-0.5, ws, 0, pages, 3)
+        torch.cuda.synchronize()
+        want, tol = _oracle(rec[0], tables, q[2:4], [1, 1], [700, 900], D**-0.5, pages=pages[2:4].cpu())
+        assert ((out[2:4].double().cpu() - want).abs() <= tol).all()
+        assert (out[4:] == 7.0).all()
+
+
+def test_prefill_tokens_beyond_max_q_len_are_left_alone():
+    q_lens, ctx_lens = [100, 3], [300, 900]
+    pool, rec, tables, q, start = _setup(q_lens, ctx_lens, 8, 2, seed=73)
+    out = _attend(pool, 0, tables, q, start, ctx_lens, 64, 2, 3)  # a CTA has 64 tokens
+    want, tol = _oracle(rec[0], tables, q, q_lens, ctx_lens, D**-0.5, prefill=True)
+    assert ((out - want).abs() <= tol)[list(range(64)) + [100, 101, 102]].all()
+    assert (out[64:100] == 7.0).all()
