@@ -111,7 +111,7 @@ class AttentionWorkspace:
     """Scratch for split-KV partials, grown on demand and reused.
 
     Calls that use one workspace have to be ordered (one stream, or events between streams), graph replays included.  When it
-    grows it keeps the smaller buffers, whose addresses captured graphs may hold."""
+    grows, to twice the size at least, it keeps the smaller buffers, whose addresses captured graphs may hold."""
 
     def __init__(self, device) -> None:
         self.device = device
@@ -124,19 +124,26 @@ class AttentionWorkspace:
     def ensure(self, rows: int, nsplit: int, head_dim: int) -> None:
         need = rows * nsplit
         if self.part_lse is None or self.part_lse.numel() < need:
-            self._outgrown += [self.part_o, self.part_lse]
+            if self.part_lse is not None:
+                self._outgrown += [self.part_o, self.part_lse]
+                need = max(need, 2 * self.part_lse.numel())
             self.part_o = torch.empty(need * head_dim, dtype=torch.float32, device=self.device)
             self.part_lse = torch.empty(need, dtype=torch.float32, device=self.device)
 
     def ensure_shared(self, items: int) -> torch.Tensor:
         if self.shared is None or self.shared.numel() < 2 * items:
-            self._outgrown.append(self.shared)
-            self.shared = torch.empty(2 * items, dtype=torch.int32, device=self.device)
+            need = 2 * items
+            if self.shared is not None:
+                self._outgrown.append(self.shared)
+                need = max(need, 2 * self.shared.numel())
+            self.shared = torch.empty(need, dtype=torch.int32, device=self.device)
         return self.shared
 
     def ensure_scores(self, need: int) -> torch.Tensor:
         if self.scores is None or self.scores.numel() < need:
-            self._outgrown.append(self.scores)
+            if self.scores is not None:
+                self._outgrown.append(self.scores)
+                need = max(need, 2 * self.scores.numel())
             self.scores = torch.empty(need, dtype=torch.float32, device=self.device)
         return self.scores
 
@@ -165,7 +172,7 @@ def paged_attention(
     keys ``0 .. ctx_len - q_len + t`` (a row with none gets zeros); rows behind the last sequence are left as they were.
 
     Over a :class:`~daser_b200.ops.kv_ops.PagedKV4Pool` any group of up to 16 query heads per KV head is taken,
-    ``max_ctx`` has to be at least the longest context, and ``workspace`` may be ``None`` (scratch of the call's own).
+    ``max_ctx`` has to be at least the longest context, ``max_q_len`` at least the most query tokens of a sequence, and ``workspace`` may be ``None`` (scratch of the call's own).
     ``nsplit`` then is the first value of :func:`plan_kv4`.
     """
     if isinstance(pool, PagedKV4Pool):

@@ -259,3 +259,18 @@ def test_outgrown_workspace_buffers_stay_alive():
     ws.ensure(40, 2, 128)
     assert ws.part_o is not first and any(t is first for t in ws._outgrown)
     assert ws.ensure_scores(10).numel() == 10 and ws.ensure_scores(5).numel() == 10
+
+
+def test_a_workspace_keeps_what_it_outgrew_and_not_more_than_that():
+    """Captured graphs may hold the smaller buffers' addresses; growing in small steps must not pile them up."""
+    from daser_b200.ops import attention
+
+    ws = attention.AttentionWorkspace(torch.device("cpu"))
+    for rows in range(1, 2000, 3):
+        ws.ensure(rows, 2, 4)
+        ws.ensure_shared(rows)
+        assert ws.ensure_scores(rows).numel() >= rows
+        assert ws.part_lse.numel() >= 2 * rows and ws.part_o.numel() == 4 * ws.part_lse.numel() and ws.shared.numel() >= 2 * rows
+    held = sum(t.numel() for t in ws._outgrown)
+    assert held <= ws.part_o.numel() + ws.part_lse.numel() + ws.shared.numel() + ws.scores.numel()
+    assert all(t is not None for t in ws._outgrown)
