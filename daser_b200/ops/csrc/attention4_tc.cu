@@ -10,6 +10,10 @@
 //                one conversion yields the two neighbours of a V^T row.  A row of ones in V^T sums the rows of the P that was multiplied;
 //   * 12         issues the MMAs, S0(i), O0 += P0(i-1) V(i-1), S1(i), O1 += P1(i-1) V(i-1): M 128, N 64, K 128 and M 128, N 144, K 64;
 //   * 13         fetches: a tile is four bulk copies of 2304 bytes, three tiles ahead.
+// Measured: 2048 tokens over 8192 keys, 32 / 8 heads, 241 GFLOP: 285 us, 845 TFLOP/s.  256 CTAs on 148 SMs are 1.73 waves: of the
+// cycles that an SM is at work the tensor pipe is active in 45 %, the ALU in 44 and the exponential's unit in 43: the three share the
+// time, none is free of the others.  64 tokens over 3328 keys, 64 / 8 heads (9 splits of 6 tiles): 20 us + merge, half of it before
+// the first MMA and behind the last.
 // Every mbarrier wait is bounded; on expiry the CTA records it in a status word, frees its TMEM and returns.
 #include "attention4_params.cuh"
 
