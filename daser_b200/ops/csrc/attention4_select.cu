@@ -324,9 +324,10 @@ DASER_API int daser_select_pages_kv4(const void* q, const int8_t* codes, const i
     if (e != cudaSuccess) return (int)e;
   }
   if (stride > n_pages) {
-    // one batch a CTA while that fills the GPU no more than twice (4 resident an SM), four beyond
+    // One batch a CTA while that fills the GPU no more than twice (3 resident an SM), four beyond: 16 sequences of 16k - 64k tokens 65 us
+    // for the whole step with one, 59 to 63 with two to eight; 64 chunks (131072 tokens, 8 heads) fill it once.
     const int64_t chunks = (stride + SCORE_PAGES - 1) / SCORE_PAGES;
-    p.batches = chunks * Hkv * rows > 2 * 148 * 4 ? 4 : 1;
+    p.batches = chunks * Hkv * rows > 2 * 148 * 3 ? 4 : 1;
     cudaError_t e = launch_pdl(attn4_score_kernel, dim3((unsigned)((chunks + p.batches - 1) / p.batches), (unsigned)Hkv, (unsigned)rows),
                                dim3(256), 0, stream, p);
     if (e != cudaSuccess) return (int)e;

@@ -220,7 +220,8 @@ def kv_read(pool: PagedKV4Pool, layer: int, slot_mapping: torch.Tensor, rank: in
     pool.check(layer, rank)
     _lib.check_tensor(slot_mapping, "slot_mapping", torch.int64, pool.index)
     T = slot_mapping.numel()
-    k, v = torch.empty((2, T, pool.heads_per_rank, KV4_DIM), dtype=torch.bfloat16, device=pool.device).unbind(0)
+    k = torch.empty((T, pool.heads_per_rank, KV4_DIM), dtype=torch.bfloat16, device=pool.device)
+    v = torch.empty_like(k)
     _lib.call_on(pool.index, _lib.kv4_fn("daser_kv4_read"), "kv4_read", pool.c_ptr, layer, rank, slot_mapping.data_ptr(),
                  k.data_ptr(), v.data_ptr(), T)
     return k, v
