@@ -18,6 +18,7 @@ NUM_SMS = 148
 MAX_ROW_SPLITS = 262144  # (query rows x KV splits) the split-KV scratch is sized for (135 MB)
 
 
+SELECT_ON_CHIP = 16384  # pages of a context up to which select_pages needs no scratch
 TC_MIN_ROWS = 64  # query rows per KV head from which chunked prefill runs on the tcgen05 kernel
 TC_KEY_TILE = 64
 _tc_enabled = os.environ.get("DASER_ATTN_TC", "1") != "0"
@@ -294,16 +295,15 @@ def select_pages(
     pages = torch.empty((Tq, Hkv, num_pages), dtype=torch.int32, device=q.device)
     stride = max(1, -(-max_ctx // KV4_TOKENS))
     scores = None
-    if stride > num_pages:
+    if stride > SELECT_ON_CHIP:
         need = Tq * Hkv * stride
         scores = workspace.ensure_scores(need) if workspace is not None else torch.empty(need, dtype=torch.float32, device=q.device)
         _lib.require(scores.get_device() == dev, "the workspace is on another device")
+        scores = scores.data_ptr()
     _lib.call_on(dev, _lib.kv4_fn("daser_select_pages_kv4"), "select_pages_kv4", q.data_ptr(), bounds.codes.data_ptr(),
                  bounds.exps.data_ptr(), layer, nb, block_tables.data_ptr(), block_tables.shape[1], q_start.data_ptr(),
-                 ctx_lens.data_ptr(), n, Tq, max_q_len, Hq, Hkv, scores.data_ptr() if scores is not None else pages.data_ptr(), stride,
+                 ctx_lens.data_ptr(), n, Tq, max_q_len, Hq, Hkv, scores, stride,
                  pages.data_ptr(), num_pages, sink_pages, recent_pages)
-    if stride > num_pages:
-        _lib.launch_count += 1  # the score kernel
     return pages
 
 

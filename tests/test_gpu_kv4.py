@@ -578,7 +578,7 @@ def test_selection_matches_whole_number_arithmetic(q_lens, ctx_lens, hq, hkv, n_
 def test_selection_of_hard_scores(kind):
     attention, _, kv_ops = _ops()
     torch.manual_seed(12)
-    pages = 45000 if kind == "long" else 1500  # more keys than the select kernel keeps on chip
+    pages = 45000 if kind == "long" else 1500
     codes = torch.randint(-127, 128, (1, pages, 1, 2, D), dtype=torch.int8)
     exps = torch.randint(-9, 3, (1, pages, 1), dtype=torch.int8)
     if kind == "ties":  # 1500 pages with three different contents
@@ -863,3 +863,25 @@ def test_prefill_tokens_beyond_max_q_len_are_left_alone():
     want, tol = _oracle(rec[0], tables, q, q_lens, ctx_lens, D**-0.5, prefill=True)
     assert ((out - want).abs() <= tol)[list(range(64)) + [100, 101, 102]].all()
     assert (out[64:100] == 7.0).all()
+
+
+@pytest.mark.parametrize("seqs,hkv", [(40, 4), (20, 4), (9, 4), (3, 4), (1, 1)])
+def test_selection_with_any_number_of_lists(seqs, hkv):
+    """The more lists, the fewer CTAs work on one: 160 lists to 1, of 200 to 560 pages."""
+    attention, _, kv_ops = _ops()
+    g = torch.Generator().manual_seed(13)
+    ctx = torch.randint(200 * B, 560 * B, (seqs,), generator=g).tolist()
+    ctx[0] = 560 * B - 1
+    pages, width = 700, 560
+    codes = torch.randint(-127, 128, (1, pages, hkv, 2, D), dtype=torch.int8, generator=g)
+    exps = torch.randint(-6, -2, (1, pages, hkv), dtype=torch.int8, generator=g)
+    tables = torch.stack([torch.randperm(pages, generator=g)[:width] for _ in range(seqs)]).to(torch.int32)
+    q = torch.randn(seqs, 2 * hkv, D, generator=g).to(torch.bfloat16)
+    bounds = kv_ops.PageBounds(codes.cuda(), exps.cuda())
+    start, lens = torch.arange(seqs + 1, dtype=torch.int32, device="cuda"), torch.tensor(ctx, dtype=torch.int32, device="cuda")
+    want = _select_oracle(q, codes[0], exps[0], tables, [1] * seqs, ctx, 40, 1, 4)
+    for max_ctx in (max(ctx), 300_000, 2_300_000):  # scores on chip, scratch at hand, scratch in use by a list of 8 CTAs
+        if max_ctx > 10**6 and seqs > 3:
+            continue
+        got = attention.select_pages(q.cuda(), bounds, 0, tables.cuda(), start, lens, 1, max_ctx, 40)
+        assert torch.equal(got.cpu(), want), max_ctx
