@@ -285,7 +285,7 @@ def select_pages(
 
     Always the first ``sink_pages`` and the last ``recent_pages`` (at least one: the page of the newest key, whose bounds need not be
     up to date) of the pages a row sees; the other places go to the highest bounds on the sum of the group's scores, the lower
-    page first among equals.  A row that sees at most ``num_pages`` pages gets them all.  ``bounds`` have to cover the context
+    page first among equals.  A row that sees at most ``num_pages`` pages gets them all.  Rows of no sequence are not set.  ``bounds`` have to cover the context
     (:func:`~daser_b200.ops.kv_ops.update_page_bounds`); other arguments as in :func:`paged_attention`.
     """
     (layers, nb, Hkv), dev = bounds.shape, bounds.index
