@@ -15,7 +15,9 @@
 // * An item is (sequence, tile of query rows, KV head).  With many pages a fixed number of CTAs shares the pages of ALL
 //   items evenly: CTA c takes [c T / W, (c + 1) T / W) of the T pages in item order, whatever the lengths are, so that
 //   all finish together (splits of a fixed length left the last wave a third empty).  An item that lies in several CTAs is put
-//   together by attn4_merge_kernel from their partial results.
+//   together by attn4_merge_kernel from their partial results.  W is the number of CTAs, or T if that is less (CTAs are planned for the
+//   longest context there can be, T comes from the lengths there are): each of the W has a page then, so that
+//   every CTA between the first and the last of an item leaves a part of it.
 // * The cache is the A operand of mma.sync m16n8k16, the queries the B operand: S^T = K Q^T (16 tokens x 8 rows) and
 //   O^T = V^T P^T (16 dims x 8 rows).  With at most 8 query heads per KV head that is half the MMAs (16 a page) of the form that puts
 //   queries in the 16 rows of A.  The contraction index may be permuted as long as A and B agree, so a lane (g = lane / 4,
@@ -115,7 +117,9 @@ __device__ __forceinline__ int64_t warp_sum_i64(int64_t v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-// The CTA that owns page x of T when W share them: CTA c owns [floor(c T / W), floor((c + 1) T / W)).
+// The CTAs that have pages, of `workers` launched ones: no more than there are pages.
+__device__ __forceinline__ int sharers(int64_t T, int workers) { return (int)min(T, (int64_t)workers); }
+// The CTA that owns page x of T when W <= T share them: CTA c owns [floor(c T / W), floor((c + 1) T / W)).
 __device__ __forceinline__ int owner_of(int64_t x, int64_t T, int W) { return (int)(((x + 1) * W - 1) / T); }
 
 // The items of a CTA, one after the other; its warps walk them on their own.
@@ -164,9 +168,10 @@ struct Walk {
     int64_t mine = lane < p.num_seqs ? seq_pages<ROWS, SPARSE>(p, lane) : 0;  // of sequence base + lane
     T = warp_sum_i64(mine);
     for (int s = 32 + lane; s - lane < p.num_seqs; s += 32) T += warp_sum_i64(s < p.num_seqs ? seq_pages<ROWS, SPARSE>(p, s) : 0);
-    at = (int64_t)blockIdx.x * T / p.workers;
-    todo = (int64_t)(blockIdx.x + 1) * T / p.workers - at;
-    if (todo == 0) return false;
+    const int W = sharers(T, p.workers);
+    if ((int)blockIdx.x >= W) return false;
+    at = (int64_t)blockIdx.x * T / W;
+    todo = (int64_t)(blockIdx.x + 1) * T / W - at;
     int64_t x = at;  // relative to the sequence, the tile, the item
     for (int base = 0;; base += 32) {
       if (base > 0) mine = base + lane < p.num_seqs ? seq_pages<ROWS, SPARSE>(p, base + lane) : 0;
@@ -522,7 +527,7 @@ attn4_kernel(const Attn4Params p) {
   if (p.workers && begins && threadIdx.x == 0) {
     // who has the rest of the item: the owner of its last page is the last
     const int64_t id = SPARSE ? (int64_t)(q0 + tok0) * p.Hkv + kvh : ((int64_t)it.seq * p.tiles + it.tile) * p.Hkv + kvh;
-    const int n = whole ? 1 : owner_of(it.at + it.n_item - 1, it.T, p.workers) - (int)blockIdx.x + 1;
+    const int n = whole ? 1 : owner_of(it.at + it.n_item - 1, it.T, sharers(it.T, p.workers)) - (int)blockIdx.x + 1;
     p.shared[id] = make_int2((int)blockIdx.x, n);
   }
   // ---- the next item: its first pages, but for the stage that holds this warp's part ----

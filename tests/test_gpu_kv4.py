@@ -885,3 +885,67 @@ def test_selection_with_any_number_of_lists(seqs, hkv):
             continue
         got = attention.select_pages(q.cuda(), bounds, 0, tables.cuda(), start, lens, 1, max_ctx, 40)
         assert torch.equal(got.cpu(), want), max_ctx
+
+
+def _junk_workspace(attention):
+    """A workspace whose partials hold large finite numbers with weights to match: what an earlier call may have left."""
+    ws = attention.AttentionWorkspace(torch.device("cuda"))
+    ws.ensure(32, 256, D)
+    ws.part_o.fill_(1e4)
+    ws.part_lse.fill_(60.0)
+    return ws
+
+
+@pytest.mark.parametrize("q_lens,ctx_lens,hq,hkv,max_ctx,split", [
+    ([1], [500], 8, 1, 131072, None),                                  # planned for a capacity: 112 units, 148 CTAs
+    ([1], [100], 8, 1, 131072, None),
+    ([1], [500], 8, 1, 65536, None),
+    ([1], [0], 8, 1, 131072, None),                                    # no key at all
+    ([0, 0, 1, 0, 0, 0, 0, 0], [40, 40, 320, 40, 40, 40, 40, 40], 8, 1, 16384, None),  # one of eight has a query
+    ([1] + [0] * 63, [77] * 64, 8, 1, 32768, None),
+    ([0, 0], [40, 300], 8, 1, 131072, None),                           # nobody has one
+    ([1], [40], 8, 1, None, 200),                                      # more CTAs asked for than there are units
+    ([1], [300], 16, 1, 131072, None),                                 # two column tiles
+    ([3, 1], [90, 20], 8, 1, 131072, 250),
+])
+def test_more_ctas_than_there_is_work_to_share(q_lens, ctx_lens, hq, hkv, max_ctx, split):
+    """CTAs are planned from max_ctx, the work comes from the lengths: what no CTA wrote must not be merged."""
+    attention, _, _ = _ops()
+    pool, rec, tables, q, start = _setup(q_lens, ctx_lens, hq, hkv, seed=81, extra_rows=1)
+    got = _attend(pool, 0, tables, q, start, ctx_lens, max(max(q_lens), 1), hkv, split, _junk_workspace(attention), max_ctx)
+    rows = sum(q_lens)
+    want, tol = _oracle(rec[0], tables, q[:rows], q_lens, ctx_lens, D**-0.5)
+    assert ((got[:rows] - want).abs() <= tol).all(), (got[:rows] - want).abs().max()
+    assert (got[rows:] == 7.0).all()
+
+
+def test_a_captured_decode_step_planned_for_its_capacity():
+    """One graph for contexts of 17 to 2000 keys: with few keys there are fewer units than CTAs."""
+    attention, _, _ = _ops()
+    pool, rec, tables, q, start = _setup([1], [2000], 8, 1, seed=82)
+    ctx = torch.tensor([2000], dtype=torch.int32, device="cuda")
+    ws = _junk_workspace(attention)
+    args = (q.cuda(), torch.zeros(q.shape, dtype=torch.bfloat16, device="cuda"), pool, 0, tables.cuda(), start.cuda(), ctx, 1, 131072, 1, D**-0.5, ws)
+    attention.paged_attention(*args)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attention.paged_attention(*args)
+    for n in (2000, 1100, 300, 17, 1, 1500):
+        ctx.fill_(n)
+        ws.part_o.fill_(1e4)
+        graph.replay()
+        want, tol = _oracle(rec[0], tables, q, [1], [n], D**-0.5)
+        assert ((args[1].double().cpu() - want).abs() <= tol).all(), n
+
+
+def test_sparse_rows_of_no_sequence_leave_fewer_units_than_ctas():
+    attention, _, _ = _ops()
+    pool, rec, tables, q, start = _setup([1], [400], 8, 1, seed=83, extra_rows=30)
+    pages = torch.arange(20, dtype=torch.int32).expand(31, 1, 20).contiguous()
+    out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device="cuda")
+    attention._attention_kv4(q.cuda(), out, pool, 0, tables.cuda(), start.cuda(), torch.tensor([400], dtype=torch.int32, device="cuda"), 1, 0,
+                             D**-0.5, _junk_workspace(attention), 0, pages.cuda(), 148)
+    want, tol = _oracle(rec[0], tables, q[:1], [1], [400], D**-0.5, pages=pages)
+    assert ((out[:1].double().cpu() - want).abs() <= tol).all()
+    assert (out[1:] == 7.0).all()
