@@ -125,7 +125,7 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
   pdl_wait();  // launched ahead of its predecessor's end: nothing is read before this returns
   const int q0 = p.q_start[seq];
   const int q_all = p.q_start[seq + 1] - q0;
-  const int q_len = min(p.q_start[seq + 1], p.total_q) - q0;
+  const int q_len = min(min(p.q_start[seq + 1], p.total_q) - q0, p.max_q_len);
   const int G = p.G;
   const int toks = 128 / G;  // of a row tile
   const int tok0 = grp * 2 * toks;

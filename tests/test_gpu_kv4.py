@@ -949,3 +949,14 @@ def test_sparse_rows_of_no_sequence_leave_fewer_units_than_ctas():
     want, tol = _oracle(rec[0], tables, q[:1], [1], [400], D**-0.5, pages=pages)
     assert ((out[:1].double().cpu() - want).abs() <= tol).all()
     assert (out[1:] == 7.0).all()
+
+
+@pytest.mark.parametrize("max_q,split", [(70, 1), (70, 2), (65, None), (64, 1)])
+def test_prefill_rows_beyond_max_q_len_inside_a_tile_are_left_alone(max_q, split):
+    """A CTA has 64 tokens here: max_q_len ends inside its second tile."""
+    q_lens, ctx_lens = [100, 3], [300, 900]
+    pool, rec, tables, q, start = _setup(q_lens, ctx_lens, 8, 2, seed=74)
+    out = _attend(pool, 0, tables, q, start, ctx_lens, max_q, 2, split)
+    want, tol = _oracle(rec[0], tables, q, q_lens, ctx_lens, D**-0.5, prefill=True)
+    assert ((out - want).abs() <= tol)[list(range(max_q)) + [100, 101, 102]].all()
+    assert (out[max_q:100] == 7.0).all()
