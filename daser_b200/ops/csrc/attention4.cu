@@ -601,7 +601,18 @@ attn4_merge_kernel(const Attn4Params p) {
   if (SPARSE) {
     const int tok = blockIdx.y;
     r = blockIdx.z;
-    if (tok >= p.q_start[p.num_seqs]) return;  // behind the last sequence
+    // a row that no CTA worked on has no entry in `shared`: in front of, between or behind the sequences, beyond max_q_len
+    bool found = false;
+    for (int base = 0; base < p.num_seqs && !found; base += 32) {
+      const int seq = base + lane;
+      bool mine = false;
+      if (seq < p.num_seqs) {
+        const int q0 = p.q_start[seq], q1 = p.q_start[seq + 1];
+        mine = q0 >= 0 && tok >= q0 && tok < q1 && tok - q0 < p.max_q_len;
+      }
+      found = __any_sync(0xffffffffu, mine);
+    }
+    if (!found) return;  // (every warp of the CTA alike)
     id = (int64_t)tok * p.Hkv + kvh;
     row = (int64_t)tok * p.Hq + kvh * p.G + r;
   } else {
@@ -727,7 +738,7 @@ static int launch_attn4(Attn4Params& p, int max_q_len, cudaStream_t stream) {
     cudaError_t e = cudaFuncSetAttribute(attn4_kernel<NT, SPARSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;
   }
-  p.max_q_len = SPARSE ? p.total_q : max_q_len;  // (`shared` is by token in the sparse form)
+  p.max_q_len = max_q_len;
   p.tiles = SPARSE ? max_q_len : (max_q_len * p.G + C::ROWS - 1) / C::ROWS;
   if (p.tiles > 65535 || p.num_seqs > 65535 || (SPARSE && p.total_q > 65535)) return DASER_ERR_TOO_LARGE;
   const dim3 grid = p.workers ? dim3((unsigned)p.workers) : dim3((unsigned)p.Hkv, (unsigned)p.num_seqs, (unsigned)p.tiles);

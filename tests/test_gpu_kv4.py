@@ -960,3 +960,34 @@ def test_prefill_rows_beyond_max_q_len_inside_a_tile_are_left_alone(max_q, split
     want, tol = _oracle(rec[0], tables, q, q_lens, ctx_lens, D**-0.5, prefill=True)
     assert ((out - want).abs() <= tol)[list(range(max_q)) + [100, 101, 102]].all()
     assert (out[max_q:100] == 7.0).all()
+
+
+@pytest.mark.parametrize("parts", [0, 3])
+@pytest.mark.parametrize("front", [0, 2])
+def test_sparse_rows_outside_the_call_are_left_alone(parts, front):
+    """Rows in front of the first sequence, tokens beyond max_q_len (select_pages leaves their lists unset) and rows behind the last
+    sequence, with places in the workspace that an earlier call may have left."""
+    attention, _, _ = _ops()
+    q_lens, ctx_lens = [3, 1, 2] + [0] * 40 + [2], [300, 90, 150] + [5] * 40 + [200]  # more sequences than a warp has lanes
+    pool, rec, tables, q, start = _setup(q_lens, ctx_lens, 8, 2, seed=75, extra_rows=front + 2)
+    start, rows = start + front, q.shape[0]
+    pages = torch.arange(12, dtype=torch.int32).expand(rows, 2, 12).contiguous()
+    c = torch.tensor(ctx_lens, dtype=torch.int32, device="cuda")
+    live, at = [], front
+    for n in q_lens:
+        live += list(range(at, at + min(n, 1)))
+        at += n
+    want, tol = _oracle(rec[0], tables, q[front : front + sum(q_lens)], q_lens, ctx_lens, D**-0.5, pages=pages[front:])
+    for junk in ((0, 2), (1, 2), (0, 3), (0, 1)):
+        ws = attention.AttentionWorkspace(torch.device("cuda"))
+        ws.ensure(16, 148, D)
+        ws.part_o.fill_(1e4)
+        ws.part_lse.fill_(3.0)
+        ws.ensure_shared(256).copy_(torch.tensor(junk, dtype=torch.int32).repeat(256))
+        out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device="cuda")
+        attention._attention_kv4(q.cuda(), out, pool, 0, tables.cuda(), start.cuda(), c, 1, 0, D**-0.5, ws, 0, pages.cuda(), parts)
+        got = out.double().cpu()
+        rest = [r for r in range(rows) if r not in live]
+        assert (got[rest] == 7.0).all(), junk
+        of = [r - front for r in live]
+        assert ((got[live] - want[of]).abs() <= tol[of]).all()
