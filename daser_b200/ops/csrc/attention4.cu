@@ -224,7 +224,8 @@ struct Walk {
   }
 };
 
-template <int NT, bool SPARSE>
+// ONE: the rows of an item are heads of one token and see the same keys (sparse, and dense with at most one query token per sequence).
+template <int NT, bool SPARSE, bool ONE>
 __global__ void __launch_bounds__(A4<NT>::WARPS * 32, 1)
 attn4_kernel(const Attn4Params p) {
   using C = A4<NT>;
@@ -405,6 +406,32 @@ attn4_kernel(const Attn4Params p) {
             if (key0[x] + g > pos[nt][e]) s[x][nt][e] = -INFINITY;
             if (key0[x] + g + 8 > pos[nt][e]) s[x][nt][2 + e] = -INFINITY;
           }
+      if (!ONE && limit - 1 > first_pos) {
+        // A key that only the later rows see must not reach the others as 0 * NaN: a group of its value that is not finite leaves the
+        // product (its scale becomes 0), and NaN goes into the rows that see it.
+        int bad = 1 << 30;  // the first such key of group g
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int x = i >> 2, tok = 2 * t + (i & 1) + 4 * (i & 2);
+          uint8_t* const at = const_cast<uint8_t*>(st[x]) + kv4_scale_at(1, tok, g);
+          if (key0[x] + tok < limit && *at >= 0xf8u) {
+            *at = 0;
+            bad = min(bad, key0[x] + tok);
+          }
+        }
+        if (__any_sync(0xffffffffu, bad < 1 << 30)) {
+          bad = min(bad, __shfl_xor_sync(0xffffffffu, bad, 1));
+          bad = min(bad, __shfl_xor_sync(0xffffffffu, bad, 2));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (bad <= pos[nt][e]) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o[nt][j][e] = o[nt][j][2 + e] = NAN;
+              }
+        }
+      }
     }
     // ---- raise the base where a score is more than 2^8 above it; P ----
     float top = -INFINITY;
@@ -729,20 +756,20 @@ static int launch_merge(const Attn4Params& p, int max_q_len, cudaStream_t stream
   return (int)launch_pdl(attn4_merge_kernel<ROWS, SPARSE>, grid, dim3(MERGE_WARPS * 32), 0, stream, p);
 }
 
-template <int NT, bool SPARSE>
+template <int NT, bool SPARSE, bool ONE>
 static int launch_attn4(Attn4Params& p, int max_q_len, cudaStream_t stream) {
   using C = A4<NT>;
   static bool configured[DASER_MAX_DEVICES] = {false};  // per device: the attribute is the device's
   constexpr int smem = C::SMEM;
   if (daser_first_use_on_device(configured)) {
-    cudaError_t e = cudaFuncSetAttribute(attn4_kernel<NT, SPARSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = cudaFuncSetAttribute(attn4_kernel<NT, SPARSE, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;
   }
   p.max_q_len = max_q_len;
   p.tiles = SPARSE ? max_q_len : (max_q_len * p.G + C::ROWS - 1) / C::ROWS;
   if (p.tiles > 65535 || p.num_seqs > 65535 || (SPARSE && p.total_q > 65535)) return DASER_ERR_TOO_LARGE;
   const dim3 grid = p.workers ? dim3((unsigned)p.workers) : dim3((unsigned)p.Hkv, (unsigned)p.num_seqs, (unsigned)p.tiles);
-  const int rc = (int)launch_pdl(attn4_kernel<NT, SPARSE>, grid, dim3(C::WARPS * 32), smem, stream, p);
+  const int rc = (int)launch_pdl(attn4_kernel<NT, SPARSE, ONE>, grid, dim3(C::WARPS * 32), smem, stream, p);
   return rc || p.workers == 0 ? rc : launch_merge<C::ROWS, SPARSE>(p, max_q_len, stream);
 }
 
@@ -819,7 +846,9 @@ DASER_API int daser_paged_attention_kv4(const void* q, void* out, float* part_o,
   }
   p.workers = parts;
   if (parts && !shared) return DASER_ERR_BAD_ARG;
-  return rows <= 8 ? launch_attn4<1, false>(p, max_q_len, stream) : launch_attn4<2, false>(p, max_q_len, stream);
+  // a single token's rows need no look at values that some of them do not see: 146 us against 150 for 32 sequences of 4k - 32k tokens
+  if (max_q_len == 1) return rows <= 8 ? launch_attn4<1, false, true>(p, max_q_len, stream) : launch_attn4<2, false, true>(p, max_q_len, stream);
+  return rows <= 8 ? launch_attn4<1, false, false>(p, max_q_len, stream) : launch_attn4<2, false, false>(p, max_q_len, stream);
 }
 
 // The same over the pages listed for every (query row, KV head): pages int32 [total_q][Hkv][n_pages], ascending, -1 behind the last.
@@ -840,5 +869,5 @@ DASER_API int daser_sparse_attention_kv4(const void* q, void* out, float* part_o
   p.n_pages = n_pages;
   p.workers = workers;
   if (workers && !shared) return DASER_ERR_BAD_ARG;
-  return p.G <= 8 ? launch_attn4<1, true>(p, max_q_len, stream) : launch_attn4<2, true>(p, max_q_len, stream);
+  return p.G <= 8 ? launch_attn4<1, true, true>(p, max_q_len, stream) : launch_attn4<2, true, true>(p, max_q_len, stream);
 }

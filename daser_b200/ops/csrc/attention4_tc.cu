@@ -106,7 +106,24 @@ struct T4Bars {
   uint64_t s_ready[2], s_free[2], p_ready[2], o_done[2];  // by row tile
   uint64_t q_ready, drain;
   uint32_t tmem, abort;
+  int bad_v[8];  // of every group of 16 dims: the first key whose value is not finite and that some row of the CTA does not see
 };
+
+// A key that only the later rows of a CTA see must not reach the others as 0 * NaN: a group of its value that is not finite leaves the product
+// (its scale becomes 0), and the rows that see it get their NaN when they are written.  Called where the causal edge runs through
+// a tile; a warp looks at the two groups of which it makes V^T.  (In line it cost every tile: 292 us against 291, 25.3 against 24.9.)
+__device__ __noinline__ void t4_leave_out_bad_values(uint8_t* raw, int* bad_v, int key0, int key_end) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int rep = 0; rep < 4; ++rep) {
+    const int kt = lane + 32 * (rep & 1), g = 2 * (warp - 8) + (rep >> 1);
+    uint8_t* const at = raw + (kt >> 4) * T4_PITCH + kv4_scale_at(1, kt & 15, g);
+    if (key0 + kt < key_end && *at >= 0xf8u) {
+      *at = 0;
+      atomicMin(bad_v + g, key0 + kt);
+    }
+  }
+  __syncwarp();
+}
 
 __global__ void __launch_bounds__(T4_THREADS, 1)
 attn4_tc_kernel(const Attn4Params p, int groups) {
@@ -138,6 +155,7 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
   const int page_end = min(page_begin + p.split_pages, n_all);
   const int n_tiles = page_begin < page_end ? (page_end - page_begin + T4_PAGES - 1) / T4_PAGES : 0;
   const int key_end = min(page_end * DASER_KV4_TOKENS, limit);
+  const int seen_by_all = p.ctx_lens[seq] - q_all + tok0;  // the last key that the CTA's first row sees
 
   // softmax threads: this thread's row
   const int tile = warp >> 2, rt = tid & 127;
@@ -205,6 +223,7 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
     bars.abort = 0u;
     mbar_init_fence();
   }
+  if (warp == 11 && lane < 8) bars.bad_v[lane] = 0x7fffffff;
   if (warp == 12) {
     tmem_alloc(&bars.tmem, T4_TMEM_COLS);
     tmem_relinquish();
@@ -297,6 +316,7 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
         if (lane == 0) mbar_arrive(&bars.p_ready[tile]);
       }
       if (ok) ok = t4_wait(&bars.o_done[tile], (n_tiles - 1) & 1, abort_flag);
+      if (ok) ok = t4_wait(&bars.v_ready[(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, abort_flag);  // (long past: orders bad_v)
       tc_fence_after();
       if (ok) {
         // ---- O / l from TMEM (column 128 holds l).  The TMEM loads are warp-wide (.sync.aligned): every thread
@@ -304,6 +324,7 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
         uint32_t r[32];
         tmem_ld_32x32(tmem_o + ATT_D, r);
         tmem_ld_wait();
+        const bool hurt = __any_sync(0xffffffffu, bars.bad_v[lane & 7] != 0x7fffffff);
         const float l = __uint_as_float(r[0]);
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays
         // Through shared memory, so that half a warp writes 256 bytes of a row (a row per thread: 11000 cycles for the partials).  The Q
@@ -331,6 +352,12 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
           tmem_ld_wait();
 #pragma unroll
           for (int x = 0; x < 32; ++x) r[x] = __float_as_uint(__uint_as_float(r[x]) * inv);
+          if (hurt) {
+            const bool bad0 = bars.bad_v[2 * cc] <= pos, bad1 = bars.bad_v[2 * cc + 1] <= pos;
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (x < 16 ? bad0 : bad1) r[x] = 0x7fc00000u;
+          }
           if (partial) {
 #pragma unroll
             for (int x = 0; x < 8; ++x) put((cc & 1) * 8 + x, make_uint4(r[4 * x], r[4 * x + 1], r[4 * x + 2], r[4 * x + 3]));
@@ -393,6 +420,7 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
       t4_fence_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.k_ready[b]);
+      if (key0 + T4_NK - 1 > seen_by_all) t4_leave_out_bad_values(raw_s + (ti % T4_STAGES) * T4_RAW, bars.bad_v, key0, key_end);
       if (ti >= 2 && !(ok = t4_wait(&bars.v_free[b], (ti / 2 - 1) & 1, abort_flag))) break;
       // ---- V^T: 8 keys x 8 dims per thread ----
       {

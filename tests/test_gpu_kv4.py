@@ -991,3 +991,35 @@ def test_sparse_rows_outside_the_call_are_left_alone(parts, front):
         assert (got[rest] == 7.0).all(), junk
         of = [r - front for r in live]
         assert ((got[live] - want[of]).abs() <= tol[of]).all()
+
+
+@pytest.mark.parametrize("q_lens,ctx_lens,hq,hkv,split,bad", [
+    ([3], [40], 8, 1, None, 38),            # few rows: the second of three new tokens
+    ([3], [40], 8, 1, 0, 39),
+    ([5, 2], [700, 90], 16, 2, 7, 698),     # pages of the items shared by seven CTAs
+    ([9], [333], 14, 2, None, 330),         # 63 rows: four row tiles
+    ([9], [333], 14, 2, 5, 325),
+    ([4], [50], 32, 2, None, 48),           # sixteen heads per KV head
+    ([20], [40], 8, 1, None, 30),           # tensor cores: one row tile
+    ([64], [320], 8, 1, 1, 300),            # two row tiles
+    ([64], [320], 8, 1, 3, 257),            # splits
+    ([100], [100], 16, 2, None, 0),         # every row sees it
+    ([100], [100], 16, 2, None, 50),
+    ([70], [257], 2, 2, 1, 255),
+    ([130], [130], 7, 1, None, 64),
+])
+def test_a_value_that_is_not_finite_stays_in_the_rows_that_see_it(q_lens, ctx_lens, hq, hkv, split, bad):
+    """A NaN in the value of key `bad` of the first sequence, in one group of 16 dims: rows in front of it do not change, rows from it on
+    have NaN in those dims and the formula in the others."""
+    from daser_b200.ops import kv_ops
+
+    _, rec, tables, q, start = _setup(q_lens, ctx_lens, hq, hkv, seed=91)
+    want, tol = _oracle(rec[0], tables, q, q_lens, ctx_lens, D**-0.5, prefill=max(q_lens) * hq // hkv >= 64)
+    dirty, t, head, group = rec.clone(), bad % B, hkv - 1, 5
+    dirty[0, tables[0, bad // B].long(), head, 2176 + (t // 8) * 64 + 8 * group + t % 8] = 0xFF
+    got = _attend(kv_ops.PagedKV4Pool.from_tensors([dirty.cuda()]), 0, tables, q, start, ctx_lens, max(q_lens), hkv, split)
+    sees = torch.zeros(q.shape, dtype=torch.bool)
+    first, G = max(0, bad - (ctx_lens[0] - q_lens[0])), hq // hkv
+    sees[first : q_lens[0], head * G : (head + 1) * G, 16 * group : 16 * group + 16] = True
+    assert torch.isnan(got[sees]).all()
+    assert ((got - want).abs() <= tol)[~sees].all(), (got - want)[~sees].abs().max()
