@@ -289,8 +289,8 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
         const bool raise = mx > m + T4_RAISE_AT || (m == -INFINITY && mx > -INFINITY);
         // the previous P V has completed: its P may be overwritten, and O may be touched
         if (ti > 0 && !(ok = t4_wait(&bars.o_done[tile], (ti - 1) & 1, abort_flag))) break;
+        tc_fence_after();  // the stores below come behind that product's reads of P, whether or not O is touched
         if (ti > 0 && __any_sync(0xffffffffu, raise)) {
-          tc_fence_after();
           const float alpha = raise ? ex2f(m - mx) : 1.f;
 #pragma unroll
           for (int cc = 0; cc < 9; ++cc) {

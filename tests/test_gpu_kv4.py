@@ -1023,3 +1023,23 @@ def test_a_value_that_is_not_finite_stays_in_the_rows_that_see_it(q_lens, ctx_le
     sees[first : q_lens[0], head * G : (head + 1) * G, 16 * group : 16 * group + 16] = True
     assert torch.isnan(got[sees]).all()
     assert ((got - want).abs() <= tol)[~sees].all(), (got - want)[~sees].abs().max()
+
+
+def test_prefill_whose_maximum_is_never_raised():
+    """The largest score comes first, so that P is replaced tile after tile while O is never touched in between: right, and the same each time."""
+    _, _, kv_ops = _ops()
+    ctx, q_len = 2500, 32
+    _, rec, tables, q, start = _setup([q_len], [ctx], 8, 1, seed=76)
+    g = torch.Generator().manual_seed(77)
+    k = torch.randn(rec.shape[1], 1, B, D, generator=g) * 0.3
+    q = (q.abs() + 0.1).to(torch.bfloat16)
+    k[tables[0, 0].long(), 0, 0] = 1.0  # key 0: above all others
+    rec = codec.pack_kv4_records(k, torch.randn(k.shape, generator=g))[None]
+    pool = kv_ops.PagedKV4Pool.from_tensors([rec.cuda()])
+    want, tol = _oracle(rec[0], tables, q, [q_len], [ctx], D**-0.5, prefill=True)
+    first = None
+    for _ in range(20):
+        got = _attend(pool, 0, tables, q, start, [ctx], q_len, 1, 1)
+        assert ((got - want).abs() <= tol).all()
+        first = got if first is None else first
+        assert torch.equal(got, first)
