@@ -194,7 +194,7 @@ class GpuRagEngine(SchedulingMixin):
             table = self.blocks.alloc(n_blocks)
             shapes = [[{"tokens": [1] * t, "start_pos": ctx - t, "block_table": table}]
                       for t in token_counts if t <= self.runner.max_tokens]
-            shapes += [[{"tokens": [1], "start_pos": ctx - 1, "block_table": table}] * b
+            shapes += [[{"tokens": [1], "start_pos": ctx - 1, "block_table": table, "write": i == 0} for i in range(b)]
                        for b in decode_batches if b <= self.runner.max_seqs]
             for seqs in shapes:
                 for _ in range(3):
@@ -471,9 +471,10 @@ class GpuRagEngine(SchedulingMixin):
         seqs = [{"tokens": [r.generated[-1]], "start_pos": r.context_len + len(r.generated) - 1,
                  "block_table": r.block_table, "temperature": r.temperature, "seed": r.step_seed(),
                  "top_k": r.top_k, "top_p": r.top_p} for r in batch]
-        # padding rows repeat the first sequence: they rewrite the same KV entry with the same
-        # value and their samples are dropped
-        seqs += [seqs[0]] * (self.decode_bucket(len(seqs), self.runner.max_seqs) - len(seqs))
+        # Padding rows repeat the first sequence; their samples are dropped and they write no KV.  (Their keys and
+        # values may differ from the first row's in the last bits, projections that are split along K add their parts
+        # in no fixed order, and two rows must not write one slot of the cache.)
+        seqs += [dict(seqs[0], write=False)] * (self.decode_bucket(len(seqs), self.runner.max_seqs) - len(seqs))
         inp = self.runner.stage_inputs(seqs)
         self.h2d_bytes += self.runner.h2d_bytes
         out = self._tokens_out(self.runner.forward(inp), len(batch))

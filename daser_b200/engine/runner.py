@@ -257,7 +257,8 @@ class GpuModelRunner:
     # -- step inputs ---------------------------------------------------------------------------------
     def stage_inputs(self, seqs: list[dict]) -> StepInputs:
         """Write one step's inputs into the runner's fixed buffers (pinned host -> device, one
-        copy each) and describe them.  ``seqs`` = ``[{tokens, start_pos, block_table}]``."""
+        copy each) and describe them.  ``seqs`` = ``[{tokens, start_pos, block_table}]``; a sequence with
+        ``write=False`` (a padding row) leaves the cache alone."""
         bt = self.cfg.block_tokens
         h = self._in_host
         if self._in_event is not None:
@@ -273,7 +274,7 @@ class GpuModelRunner:
             pos = torch.arange(p0, p0 + n, dtype=torch.int64)
             h["positions"][t : t + n] = pos.to(torch.int32)
             tbl = torch.as_tensor(table, dtype=torch.int64)
-            h["slot_mapping"][t : t + n] = tbl[pos // bt] * bt + pos % bt
+            h["slot_mapping"][t : t + n] = tbl[pos // bt] * bt + pos % bt if s.get("write", True) else -1
             h["block_tables"][i, : len(table)] = tbl.to(torch.int32)
             t += n
             h["q_start"][i + 1] = t

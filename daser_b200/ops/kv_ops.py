@@ -158,7 +158,8 @@ class PagedKV4Pool:
     ``sparse_paged_attention`` work on.  16 tokens per block, head_dim 128.  ``record_ptrs[r]`` is rank ``r``'s base
     address as mapped into this process; the pool's kernels run on ``device``.
 
-    Slots written by one call have to be distinct: of two tokens with the same slot, one wins group by group.
+    Slots written by one call have to be distinct, and so do the blocks of one restore: of two tokens with the same slot each store
+    of a few bytes is one's or the other's, so that a group may end up with the codes of one under the scale of the other.
     """
 
     def __init__(self, record_ptrs: Sequence[int], stride_layer: int, stride_block: int, stride_head: int, num_layers: int,

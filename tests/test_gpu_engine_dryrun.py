@@ -221,3 +221,16 @@ def test_decode_batches_run_while_a_starting_request_waits_for_the_drive(engine,
     while engine.has_work():
         engine.step()
     assert engine.blocks.num_free == 32
+
+
+def test_padding_rows_of_a_decode_batch_write_no_cache(engine):
+    """Three running requests are a batch of four: the fourth row repeats the first, and only one of the two writes its slot."""
+    eng = engine
+    reqs = [eng.submit(RagRequest([], [5 + i, 6, 7], 4)) for i in range(3)]
+    while eng.waiting:
+        eng.step()
+    eng._decode_step()
+    rows = eng.runner.calls[-1]
+    assert [r.get("write", True) for r in rows] == [True, True, True, False]
+    assert rows[3]["tokens"] == rows[0]["tokens"] and rows[3]["block_table"] == rows[0]["block_table"]
+    assert all(len(r.generated) == 2 for r in reqs)

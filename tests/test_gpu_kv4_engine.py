@@ -134,3 +134,29 @@ def test_the_runner_refuses_what_the_pool_cannot_hold():
         GpuModelRunner(PRESETS["toy-qk"], w, num_blocks=8, max_tokens=16, kv_format="fp4b16")
     with pytest.raises(ValueError, match="kv_format"):
         GpuModelRunner(PRESETS["toy-qk"], w, num_blocks=8, max_tokens=16, kv_format="int4")
+
+
+@pytest.mark.parametrize("kv_format", ["fp4b16", "fp8b16"])
+def test_a_padding_row_leaves_the_cache_alone(kv_format):
+    """A batch padded with a copy of its first sequence: the copy has no slot, the cache is what the batch without it writes, and the copy
+    attends as the first row does."""
+    from daser_b200.engine.runner import GpuModelRunner
+
+    cfg = PRESETS["tiny-gqa"]
+    w = LlamaWeights.random(cfg, "cuda", torch.bfloat16, seed=7, std=0.05)
+    runner = GpuModelRunner(cfg, w, num_blocks=16, max_tokens=64, max_seqs=4, max_blocks=8, kv_format=kv_format)
+    _step(runner, [{"tokens": list(range(3, 23)), "start_pos": 0, "block_table": [4, 2]}])
+    seq = {"tokens": [9], "start_pos": 20, "block_table": [4, 2]}
+    inp = runner.stage_inputs([seq, dict(seq, write=False)])
+    assert inp.slot_mapping.tolist() == [2 * 16 + 4, -1]
+    pool = (lambda: runner.local_pool.keepalive[0][0]) if kv_format == "fp4b16" else (lambda: runner.kv_payload)
+    before = pool().clone()
+    runner.forward(runner.stage_inputs([dict(seq, write=False)]))
+    assert torch.equal(pool(), before)
+    runner.forward(runner.stage_inputs([seq, dict(seq, write=False)]))  # (a step's inputs live in the runner's buffers)
+    assert not torch.equal(pool(), before)
+    if kv_format == "fp4b16":  # the last layer's queries and outputs are still there
+        rec = runner.local_pool.keepalive[0][0][len(w.layers) - 1].cpu()
+        want, tol = _oracle(rec, torch.tensor([[4, 2]] * 2), runner.q_rot[:2].float().cpu(), [1, 1], [21, 21], D**-0.5)
+        assert ((runner.attn_out[:2].view(2, runner.hq, D).double().cpu() - want).abs() <= tol).all()
+    runner.check_status()
