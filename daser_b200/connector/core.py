@@ -109,9 +109,11 @@ class ConnectorMeta:
 
 class SchedulerHalf:
     def __init__(self, socket_path: str, block_tokens: int = 16, model_id: str = "default",
-                 client: Optional[IPCClientSync] = None) -> None:
+                 client: Optional[IPCClientSync] = None, also_reads: Sequence[str] = ()) -> None:
+        """Chunks are stored as ``model_id``'s; lookups by key fall back to those of ``also_reads``, in order."""
         self.block_tokens = block_tokens
         self.model_id = model_id
+        self.also_reads = tuple(also_reads)
         self._ipc = client or IPCClientSync(socket_path)
         self._pending_loads: dict[str, list[ReqLoadSpec]] = {}
         self._pending_stores: dict[str, ReqStoreSpec] = {}
@@ -181,6 +183,16 @@ class SchedulerHalf:
             else:
                 self._negotiated = True
 
+    def _lookup_keys(self, keys: Sequence[str]) -> list[Optional[dict[str, Any]]]:
+        """The committed chunk of every key: this model's, else that of a model it may read from."""
+        found = list(self._ipc.lookup_chunks(list(keys), self.model_id))
+        for other in self.also_reads:
+            missing = [i for i, meta in enumerate(found) if meta is None]
+            if missing:
+                for i, meta in zip(missing, self._ipc.lookup_chunks([keys[i] for i in missing], other)):
+                    found[i] = meta
+        return found
+
     def plan_chunk_loads(self, req_id: str, placements: Sequence[tuple[str, int]]) -> list[Optional[ReqLoadSpec]]:
         """Resolve ``(chunk_key, token offset)`` pairs; returns one spec (or None) per pair.
 
@@ -194,7 +206,7 @@ class SchedulerHalf:
         self._negotiate_once()
         try:
             with trace.span("rpc.lookup_chunks", "connector", req=req_id, chunks=len(placements)):
-                found = self._ipc.lookup_chunks([k for k, _ in placements], self.model_id)
+                found = self._lookup_keys([k for k, _ in placements])
         except RuntimeError as exc:
             logger.warning("[CONNECTOR] lookup_chunks failed for %s (%s)", req_id, exc)
             metrics.inc("connector.rpc_errors")
@@ -243,7 +255,7 @@ class SchedulerHalf:
             return chunks
         keys = self.composition_keys(chunks)
         try:
-            found = self._ipc.lookup_chunks(keys[1:], self.model_id)
+            found = self._lookup_keys(keys[1:])
         except RuntimeError:
             return chunks
         for k in range(len(chunks), 1, -1):

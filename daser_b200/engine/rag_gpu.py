@@ -107,7 +107,10 @@ class GpuRagEngine(SchedulingMixin):
         self.hbm = HBMStore(self.geo.slot_size, hbm_slots, self.device) if hbm_slots > 0 else None
         self.host = HBMStore(self.geo.slot_size, host_slots, torch.device("cpu")) if host_slots > 0 else None
         self.is_lead = self.rank == 0 and (pp_link is None or pp_link.first)  # plans, reserves, finishes
-        self.sched = SchedulerHalf(socket_path, cfg.block_tokens, model_id) if self.is_lead else None
+        # What an engine with a 4-bit pool stores was computed over and read out of 4 bits: it goes under a model id of its own, so
+        # that no engine with an fp8 pool restores it as its own.  The other way round nothing is lost.
+        ids = (model_id, ()) if kv_format == "fp8b16" else (f"{model_id}+{kv_format}", (model_id,))
+        self.sched = SchedulerHalf(socket_path, cfg.block_tokens, ids[0], also_reads=ids[1]) if self.is_lead else None
         if self.tp > 1 and self.rank != 0:
             tp_ctx.wait_for_path(store_path)  # rank 0 creates the store file
         self.worker = WorkerHalf(socket_path, store_path, self.geo, self.kv_backend, io_backend=io_backend, tp=self.tp,

@@ -160,3 +160,27 @@ def test_a_padding_row_leaves_the_cache_alone(kv_format):
         want, tol = _oracle(rec, torch.tensor([[4, 2]] * 2), runner.q_rot[:2].float().cpu(), [1, 1], [21, 21], D**-0.5)
         assert ((runner.attn_out[:2].view(2, runner.hq, D).double().cpu() - want).abs() <= tol).all()
     runner.check_status()
+
+
+def test_engines_of_both_formats_on_one_store(tmp_path):
+    """The 4-bit engine restores what the fp8 engine stored; the fp8 engine computes what only the 4-bit engine has."""
+    from daser_b200.engine.rag_gpu import GpuRagEngine
+
+    cfg = PRESETS["tiny-gqa"]
+    lp = LiveControlPlane(tmp_path, total_slots=256, slot_size=cfg.num_layers * 2 * 16 * cfg.num_kv_heads * cfg.head_dim * 5 // 4).start()
+    make = lambda fmt: GpuRagEngine(cfg, lp.socket_path, lp.cfg.store_path, num_blocks=64, max_tokens=64, model_id="m", kv_format=fmt)  # noqa: E731
+    fp8, kv4 = make("fp8b16"), make("fp4b16")
+    try:
+        rng = random.Random(2)
+        a, b = ([rng.randrange(cfg.vocab_size) for _ in range(32)] for _ in range(2))
+        kv4.store_chunk(a)
+        fp8.store_chunk(b)
+        query = [rng.randrange(cfg.vocab_size) for _ in range(9)]
+        assert fp8.generate([a, b], query, max_new_tokens=2).restored_chunks == 1
+        assert kv4.generate([a, b], query, max_new_tokens=2).restored_chunks == 2
+        for eng in (fp8, kv4):
+            eng.runner.check_status()
+    finally:
+        fp8.close()
+        kv4.close()
+        lp.stop()

@@ -274,3 +274,30 @@ def test_a_workspace_keeps_what_it_outgrew_and_not_more_than_that():
     held = sum(t.numel() for t in ws._outgrown)
     assert held <= ws.part_o.numel() + ws.part_lse.numel() + ws.shared.numel() + ws.scores.numel()
     assert all(t is not None for t in ws._outgrown)
+
+
+def test_chunks_of_a_4_bit_engine_are_found_by_engines_of_its_kind_alone(live_plane):
+    """Two schedulers on one store, as GpuRagEngine makes them for the two formats."""
+    from daser_b200.connector.core import SchedulerHalf
+    from daser_b200.hashing import hash_tokens
+
+    fp8 = SchedulerHalf(live_plane.socket_path, 16, "m")
+    kv4 = SchedulerHalf(live_plane.socket_path, 16, "m+fp4b16", also_reads=("m",))
+    try:
+        mine, theirs = list(range(32)), list(range(100, 148))
+        for half, tokens in ((kv4, mine), (fp8, theirs)):
+            spec = half.reserve_chunk_store("s", tokens, list(range(3)))
+            half._ipc.commit_chunk(spec.chunk_key)
+            half.request_finished("s")
+        places = [(hash_tokens(mine), 0), (hash_tokens(theirs), 32), (hash_tokens([7] * 16), 80)]
+        got8, got4 = fp8.plan_chunk_loads("a", places), kv4.plan_chunk_loads("b", places)
+        assert [s is not None for s in got8] == [False, True, False]
+        assert [s is not None for s in got4] == [True, True, False]
+        assert got4[0].num_slots == 2 and got4[1].num_slots == 3 and got4[1].start_slot == got8[1].start_slot
+        combo = [mine, list(range(200, 216))]
+        spec = fp8.reserve_chunk_store("c", [t for c in combo for t in c], [0, 1, 2])
+        fp8._ipc.commit_chunk(spec.chunk_key)
+        assert len(kv4.merge_composed(combo)) == len(fp8.merge_composed(combo)) == 1
+    finally:
+        fp8.close()
+        kv4.close()
