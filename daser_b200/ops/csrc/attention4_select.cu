@@ -36,14 +36,31 @@ struct Select4Params {
   const int32_t* ctx_lens;
   float* scores;             // [Tq, Hkv, stride], used when a share exceeds SELECT_KEYS
   int32_t* pages;            // [Tq, Hkv, n_pages]
-  int max_blocks, num_blocks, Hq, Hkv, G, max_q_len, total_q;
+  int max_blocks, num_blocks, num_seqs, Hq, Hkv, G, max_q_len, total_q;
+  int by_row;                // a CTA's row comes from its index in all rows, not in num_seqs * max_q_len of them
   int stride, n_pages, sink, recent;
   int cluster;               // CTAs per list
   int keys;                  // places for scores in a CTA's shared memory; 0: they are in `scores`
 };
 
-// The query row of (sequence, offset) and the pages it sees; false if there is no such row.
-__device__ __forceinline__ bool select_row(const Select4Params& p, int seq, int off, int& row, int& count) {
+// The i-th query row, its sequence and the pages it sees; false if there is no such row.  Whole warps call it.
+__device__ __forceinline__ bool select_row(const Select4Params& p, int i, int& seq, int& row, int& count) {
+  int off = 0;
+  if (p.by_row) {
+    const int lane = threadIdx.x & 31;
+    uint32_t mine = 0;
+    for (int base = 0; base < p.num_seqs && mine == 0; base += 32) {
+      seq = min(base + lane, p.num_seqs - 1);
+      off = i - p.q_start[seq];
+      mine = __ballot_sync(0xffffffffu, base + lane < p.num_seqs && off >= 0 && i < p.q_start[seq + 1] && off < p.max_q_len);
+    }
+    if (mine == 0) return false;
+    seq = __shfl_sync(0xffffffffu, seq, __ffs(mine) - 1);
+    off = __shfl_sync(0xffffffffu, off, __ffs(mine) - 1);
+  } else {
+    seq = i / p.max_q_len;
+    off = i - seq * p.max_q_len;
+  }
   const int q0 = p.q_start[seq], q1 = p.q_start[seq + 1];
   row = q0 + off;
   if (q0 < 0 || row >= min(q1, p.total_q)) return false;
@@ -111,10 +128,9 @@ attn4_select_kernel(const Select4Params p) {
   __shared__ uint32_t s_bin, s_above, s_in;
   pdl_launch_dependents();  // (launched the plain way: its predecessor has ended)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int C = p.cluster, rank = blockIdx.x % C, kvh = blockIdx.x / C;
-  const int seq = blockIdx.y / p.max_q_len, off = blockIdx.y % p.max_q_len;
-  int row, count;
-  if (!select_row(p, seq, off, row, count)) return;  // (this and the next two returns: all CTAs of the cluster alike)
+  const int C = p.cluster, rank = blockIdx.x % C, kvh = blockIdx.x / C % p.Hkv;
+  int seq, row, count;
+  if (!select_row(p, blockIdx.x / C / p.Hkv, seq, row, count)) return;  // (this and the next two returns: all CTAs of the cluster alike)
   int32_t* list = p.pages + ((int64_t)row * p.Hkv + kvh) * p.n_pages;
   if (count <= p.n_pages) {
     if (rank == 0)
@@ -329,8 +345,10 @@ DASER_API int daser_select_pages_kv4(const void* q, const int8_t* codes, const i
   if (num_seqs == 0 || total_q == 0 || max_q_len == 0) return 0;
   if (!q || !codes || !exps || !block_tables || !q_start || !ctx_lens || !pages) return DASER_ERR_BAD_ARG;
   if (Hq / Hkv > 16 || (uintptr_t)codes % 16) return DASER_ERR_UNSUPPORTED;
-  const int64_t rows = (int64_t)num_seqs * max_q_len;
-  if (rows > 65535 || Hkv > 65535 || max_blocks > (1 << 29) / DASER_KV4_TOKENS) return DASER_ERR_TOO_LARGE;
+  // Rows by (sequence, offset) while that many exist, as in a decode step, else by a search in q_start (one more dependent load): 32
+  // sequences of one token beside a chunk of 2048 are 2080 rows, not 33 * 2048.
+  const int64_t all = (int64_t)num_seqs * max_q_len, rows = all < total_q ? all : total_q;
+  if (max_q_len > 65535 || max_blocks > (1 << 29) / DASER_KV4_TOKENS) return DASER_ERR_TOO_LARGE;
   Select4Params p;
   p.q = (const __nv_bfloat16*)q;
   p.codes = codes + (int64_t)layer * num_blocks * Hkv * 2 * ATT_D;
@@ -342,6 +360,8 @@ DASER_API int daser_select_pages_kv4(const void* q, const int8_t* codes, const i
   p.pages = pages;
   p.max_blocks = max_blocks;
   p.num_blocks = num_blocks;
+  p.num_seqs = num_seqs;
+  p.by_row = all > total_q;
   p.Hq = Hq;
   p.Hkv = Hkv;
   p.G = Hq / Hkv;
@@ -358,14 +378,14 @@ DASER_API int daser_select_pages_kv4(const void* q, const int8_t* codes, const i
   const int share = (stride + cluster - 1) / cluster;
   p.keys = share <= SELECT_KEYS ? share : 0;
   if (p.keys == 0 && !scores) return DASER_ERR_BAD_ARG;
-  if ((int64_t)Hkv * cluster > 0x7fffffff) return DASER_ERR_TOO_LARGE;
+  if (rows * Hkv > 0x7fffffff / cluster) return DASER_ERR_TOO_LARGE;
   static bool configured[DASER_MAX_DEVICES] = {false};  // per device: the attribute is the device's
   if (daser_first_use_on_device(configured)) {
     cudaError_t e = cudaFuncSetAttribute(attn4_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SELECT_KEYS * 4);
     if (e != cudaSuccess) return (int)e;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(Hkv * cluster), (unsigned)rows);
+  cfg.gridDim = dim3((unsigned)(rows * Hkv * cluster));
   cfg.blockDim = dim3(SELECT_THREADS);
   cfg.dynamicSmemBytes = (size_t)p.keys * 4;
   cfg.stream = stream;

@@ -1043,3 +1043,23 @@ def test_prefill_whose_maximum_is_never_raised():
         assert ((got - want).abs() <= tol).all()
         first = got if first is None else first
         assert torch.equal(got, first)
+
+
+@pytest.mark.parametrize("q_lens,front,behind", [([1] * 32 + [2048], 0, 0), ([3] + [0] * 40 + [1, 7], 2, 3), ([2, 2, 2], 0, 2)])
+def test_selection_in_a_step_of_unequal_sequences(q_lens, front, behind):
+    """Decode steps beside a chunk of a prompt: the lists are those of the rows there are, not of sequences times the longest."""
+    attention, _, _ = _ops()
+    from daser_b200.ops import kv_ops
+
+    g = torch.Generator().manual_seed(14)
+    pages, width, n_pages, T = 300, 160, 8, sum(q_lens)
+    ctx = [n + int(torch.randint(B, width * B - n, (1,), generator=g)) for n in q_lens]
+    codes = torch.randint(-127, 128, (1, pages, 1, 2, D), dtype=torch.int8, generator=g)
+    exps = torch.randint(-6, -2, (1, pages, 1), dtype=torch.int8, generator=g)
+    tables = torch.stack([torch.randperm(pages, generator=g)[:width] for _ in q_lens]).to(torch.int32)
+    q = torch.randn(front + T + behind, 4, D, generator=g).to(torch.bfloat16)
+    start = torch.tensor([0] + torch.tensor(q_lens).cumsum(0).tolist(), dtype=torch.int32) + front
+    got = attention.select_pages(q.cuda(), kv_ops.PageBounds(codes.cuda(), exps.cuda()), 0, tables.cuda(), start.cuda(),
+                                 torch.tensor(ctx, dtype=torch.int32, device="cuda"), max(q_lens), max(ctx), n_pages).cpu()
+    want = _select_oracle(q[front : front + T], codes[0], exps[0], tables, q_lens, ctx, n_pages, 1, 4)
+    assert torch.equal(got[front : front + T], want)
