@@ -25,7 +25,10 @@
 //   (+ 8): the record stores V by groups so that these 16 bytes are contiguous too, and both reads hit all banks once.
 //   P^T in the layout of B is the transpose of S^T as it comes out: one movmatrix per 8 tokens.
 // * The running maximum is raised only when a page exceeds it by 2^8 (P is f16, sums are fp32): one vote a page instead of six
-//   shuffles.  Scores, sums and O are fp32; K, V are exact in f16; Q and P are rounded to f16 (2^-11, finer than bf16's 2^-8).
+//   shuffles.  Scores, sums and O are fp32; K, V are exact in f16; Q and P are rounded to f16, because the MMA takes no fp32 operand that
+//   keeps up with the memory: 2^-11 of their size, finer than bf16's 2^-8.  P of the maximum is 2^7 to 2^15, so that weights have those 11
+//   bits down to 2^-21 of the largest and an absolute error of at most 2^-32 of it below (with P of 1 to 2^8 a long tail 2^-20 below one
+//   loud key was off by 2 %).
 //
 // Measured (L2 flushed in front of each call): 32 sequences of 4k - 32k tokens, 64 / 8 heads, 681 MB: 130 us, 5.2 TB/s (a copy: 6.5);
 // the ALU is 57 % busy (conversions, byte selection), the tensor pipe 29 %.  4 sequences of 50k - 120k tokens on one KV head, 49 MB: 22 us +
@@ -50,7 +53,7 @@ template <int NT> struct A4 {
   static constexpr bool IN_RING = PART <= A4_PAIR;
   static constexpr int SMEM = RING + (IN_RING ? 0 : WARPS * PART);
 };
-constexpr float A4_RAISE_AT = 8.f;
+constexpr float A4_TOP = 7.f, A4_RAISE_AT = 15.f;  // P of a new maximum is 2^7, raised when a score would make it more than 2^15
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -127,7 +130,7 @@ template <int NT, bool SPARSE>
 struct Walk {
   int seq, tile, kvh;  // the item
   int p0;              // its first page that is this CTA's
-  int64_t at, todo, T; // p0 in the order of all pages, pages left to this CTA from there on, pages of all items
+  int64_t todo;        // pages left to this CTA from there on
   SeqInfo si;
   // of the item:
   int row0, tok0, n_rows;  // rows: dense, ROWS consecutive ones (query token major, then head of the group); sparse, the heads of one token
@@ -150,12 +153,12 @@ struct Walk {
     p1 = (int)min((int64_t)n_item, p0 + todo);
     page_end = min(p1, real);
   }
-  // The first item; false if there is none.
-  __device__ __forceinline__ bool start(const Attn4Params& p) {
+  // The first item; false if there is none.  at: p0 in the order of all pages, T: pages of all items.
+  __device__ __forceinline__ bool start(const Attn4Params& p, int64_t& at, int64_t& T) {
     constexpr int ROWS = A4<NT>::ROWS;
     const int lane = threadIdx.x & 31;
     p0 = 0;
-    at = 0;
+    at = T = 0;
     if (p.workers == 0) {
       kvh = blockIdx.x;
       seq = blockIdx.y;
@@ -204,9 +207,7 @@ struct Walk {
     return true;
   }
   __device__ __forceinline__ bool next(const Attn4Params& p) {
-    const int done = p1 - p0;
-    at += done;
-    todo -= done;
+    todo -= p1 - p0;
     if (todo <= 0) return false;
     p0 = 0;
     if (++kvh == p.Hkv) {
@@ -233,12 +234,17 @@ attn4_kernel(const Attn4Params p) {
   extern __shared__ __align__(128) uint8_t a4_smem[];  // ring [warp][stage][2 records], parts [warp][row][A4_OPITCH]
   __shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS];
   __shared__ int s_part[WARPS];
+  __shared__ int64_t s_at, s_T;  // where this CTA is in the order of all pages, and how many there are: thread 0's, out of its registers
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int G = p.G;
   pdl_enter();
   Walk<NT, SPARSE> it;
-  if (!it.start(p)) return;  // uniform over the CTA
+  {
+    int64_t at, T;
+    if (!it.start(p, at, T)) return;  // uniform over the CTA
+    if (threadIdx.x == 0) { s_at = at; s_T = T; }
+  }
 
   const uint8_t* ring = a4_smem + warp * STAGES * A4_PAIR;
   const uint32_t ring_u32 = smem_u32(ring);
@@ -309,7 +315,8 @@ attn4_kernel(const Attn4Params p) {
 
   bool more;
   do {
-  const int row0 = it.row0, tok0 = it.tok0, n_rows = it.n_rows, first_pos = it.first_pos, limit = it.limit, kvh = it.kvh, q0 = it.si.q0;
+  const int row0 = it.row0, tok0 = it.tok0, n_rows = it.n_rows, first_pos = it.first_pos, kvh = it.kvh, q0 = it.si.q0;
+  const int limit = ONE ? first_pos + 1 : it.limit;
   int use_cur = log_cur, use_nxt = log_nxt;  // windows of the uses, which run behind those of the fetches
   // ---- queries: B fragments, scaled, f16.  Column g of n-tile nt is row row0 + 8 nt + g ----
   uint32_t qf[NT][16];
@@ -326,9 +333,9 @@ attn4_kernel(const Attn4Params p) {
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) pos[nt][e] = SPARSE ? first_pos : first_pos + (row0 + 8 * nt + 2 * t + e) / G - tok0;
+    for (int e = 0; e < 2; ++e) pos[nt][e] = ONE ? first_pos : first_pos + (row0 + 8 * nt + 2 * t + e) / G - tok0;
 
-  // base: what the exponents are relative to: the running maximum, up to 2^8 behind it; 0 until the row has seen a key
+  // base: what the exponents are relative to: 7 less than the running maximum, which may be up to 8 behind; 0 until the row has seen a key
   float o[NT][8][4], base[NT][2], l[NT][2];
   bool seen[NT][2];
 #pragma unroll
@@ -451,8 +458,8 @@ attn4_kernel(const Attn4Params p) {
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          // relative to the old base: to the first maximum wherever it lies, then upwards only
-          const float up = mx == -INFINITY ? 0.f : (seen[nt][e] ? fmaxf(mx, 0.f) : mx);
+          // relative to the old base: to 7 below the first maximum wherever that lies, then upwards only
+          const float up = mx == -INFINITY ? 0.f : fmaxf(mx - A4_TOP, seen[nt][e] ? 0.f : -INFINITY);
           seen[nt][e] |= mx > -INFINITY;
           none |= !seen[nt][e];
           const float al = ex2f(-up);
@@ -551,11 +558,14 @@ attn4_kernel(const Attn4Params p) {
   if (lane == 0) s_part[warp] = part;
   const bool begins = it.p0 == 0, whole = begins && it.p1 == it.n_item;
   const int64_t slot = ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * ROWS;  // of a partial: 0 continues an item, 1 begins one
-  if (p.workers && begins && threadIdx.x == 0) {
-    // who has the rest of the item: the owner of its last page is the last
-    const int64_t id = SPARSE ? (int64_t)(q0 + tok0) * p.Hkv + kvh : ((int64_t)it.seq * p.tiles + it.tile) * p.Hkv + kvh;
-    const int n = whole ? 1 : owner_of(it.at + it.n_item - 1, it.T, sharers(it.T, p.workers)) - (int)blockIdx.x + 1;
-    p.shared[id] = make_int2((int)blockIdx.x, n);
+  if (p.workers && threadIdx.x == 0) {
+    if (begins) {
+      // who has the rest of the item: the owner of its last page is the last
+      const int64_t id = SPARSE ? (int64_t)(q0 + tok0) * p.Hkv + kvh : ((int64_t)it.seq * p.tiles + it.tile) * p.Hkv + kvh;
+      const int n = whole ? 1 : owner_of(s_at + it.n_item - 1, s_T, sharers(s_T, p.workers)) - (int)blockIdx.x + 1;
+      p.shared[id] = make_int2((int)blockIdx.x, n);
+    }
+   s_at += it.p1 - it.p0;
   }
   // ---- the next item: its first pages, but for the stage that holds this warp's part ----
   cp_async_wait<0>();  // (groups that were empty)

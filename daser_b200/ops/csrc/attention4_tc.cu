@@ -3,8 +3,8 @@
 // One CTA per SM works on two tiles of 128 query rows (128 / G query tokens x the G heads of one KV head, each) against tiles of 64 keys, so
 // that a tile of keys is dequantised once for 256 rows and one row tile's softmax runs under the other's MMAs.  14 warps:
 //   * 0-3, 4-7   softmax of row tile 0, 1: a thread owns a row of S (tcgen05.ld 32x32b), takes it into registers and frees it at once,
-//                so that the next S is under way while P = 2^(S - m) is made: f16, back into TMEM, as the MMA operand.  The running
-//                maximum m is raised only when a tile exceeds it by 2^8, and only then is O rescaled (tcgen05.ld / st);
+//                so that the next S is under way while P = 2^(S - m) is made: f16, back into TMEM, as the MMA operand.  m is 7 less than
+//                the running maximum and raised only when a tile exceeds that by 2^8, and only then is O rescaled (tcgen05.ld / st);
 //   * 8-11       dequantise: K as [key][dim], V transposed to [dim][key], f16 (exact), in the 128-byte-swizzled K-major layout of the
 //                MMA descriptors, two buffers each.  V's codes of two neighbouring tokens are interleaved nibble by nibble, so that
 //                one conversion yields the two neighbours of a V^T row.  A row of ones in V^T sums the rows of the P that was multiplied;
@@ -16,6 +16,9 @@
 // some 2000 that it takes; the warp that issues the MMAs waits for operands in a quarter of them only.  (Exponents before the wait
 // for the last P V: 293 us; their maximum in packed f16: 302.)  64 tokens over 3328 keys, 64 / 8 heads (9 splits of 6 tiles): 20 us + merge, half of it before
 // the first MMA and behind the last.
+// Rounded to f16: Q and P, 2^-11 of their size, P below 2^-21 of a row's maximum to 2^-32 of that.  Exponents are fp32: an f16 exponential
+// of rounded exponents took 288 us instead of 292, but was off by up to 2^-8 where the maximum lags, and P of 1 to 2^8 lost what
+// lies 2^-20 below the maximum, 2 % of a long flat tail.
 // Every mbarrier wait is bounded; on expiry the CTA records it in a status word, frees its TMEM and returns.
 #include "attention4_params.cuh"
 
@@ -38,7 +41,7 @@ constexpr uint32_t T4_TMEM_COLS = 512;
 __device__ __forceinline__ uint32_t t4_s_col(int t) { return 64u * t; }
 __device__ __forceinline__ uint32_t t4_o_col(int t) { return 128u + 192u * t; }
 __device__ __forceinline__ uint32_t t4_p_col(int t) { return 288u + 192u * t; }
-constexpr float T4_RAISE_AT = 8.f;
+constexpr float T4_TOP = 7.f, T4_RAISE_AT = 15.f;  // P of a new maximum is 2^7, raised when a score would make it more than 2^15
 
 __device__ uint32_t g_attn4_tc_status = 0;  // bit 0: a bounded wait ran out
 
@@ -81,14 +84,6 @@ __device__ __forceinline__ void t4_umma_ts(uint32_t tmem_d, uint32_t tmem_a, uin
       : "memory");
 }
 __device__ __forceinline__ void t4_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ uint32_t t4_ex2_f16x2(float lo, float hi) {  // {2^lo, 2^hi}
-  uint32_t r;
-  asm("{\n\t.reg .b32 t;\n\t"
-      "cvt.rn.f16x2.f32 t, %2, %1;\n\t"
-      "ex2.approx.f16x2 %0, t;\n\t}\n"
-      : "=r"(r) : "f"(lo), "f"(hi));
-  return r;
-}
 __device__ __forceinline__ void t4_bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
                "r"(bytes), "r"(smem_u32(bar))
@@ -258,7 +253,7 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.q_ready);
 
-      float m = -INFINITY;  // the maximum the accumulated P are relative to
+      float m = -INFINITY;  // what the accumulated P are relative to
       for (int ti = 0; ti < n_tiles; ++ti) {
         const int key0 = (page_begin + ti * T4_PAGES) * DASER_KV4_TOKENS;
         if (!(ok = t4_wait(&bars.s_ready[tile], ti & 1, abort_flag))) break;
@@ -285,13 +280,14 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
           mx1 = fmaxf(mx1, __uint_as_float(sr[1][j]));
         }
         const float mx = fmaxf(mx0, mx1);
-        // raise m only when this tile is far above it: P then stays below 2^8, well inside f16
+        // raise m only when this tile is far above it: P then stays below 2^15, inside f16
         const bool raise = mx > m + T4_RAISE_AT || (m == -INFINITY && mx > -INFINITY);
+        const float to = mx - T4_TOP;
         // the previous P V has completed: its P may be overwritten, and O may be touched
         if (ti > 0 && !(ok = t4_wait(&bars.o_done[tile], (ti - 1) & 1, abort_flag))) break;
         tc_fence_after();  // the stores below come behind that product's reads of P, whether or not O is touched
         if (ti > 0 && __any_sync(0xffffffffu, raise)) {
-          const float alpha = raise ? ex2f(m - mx) : 1.f;
+          const float alpha = raise ? ex2f(m - to) : 1.f;
 #pragma unroll
           for (int cc = 0; cc < 9; ++cc) {
             uint32_t r[16];
@@ -303,12 +299,12 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
           }
           t4_tmem_st_wait();
         }
-        if (raise) m = mx;
+        if (raise) m = to;
         const float base = m == -INFINITY ? 0.f : m;
         // P, two keys a register, over the first half of the scores' registers
 #pragma unroll
         for (int j = 0; j < T4_NK; j += 2)
-          sr[0][j >> 1] = t4_ex2_f16x2(__uint_as_float(sr[j >> 5][j & 31]) - base, __uint_as_float(sr[(j + 1) >> 5][(j + 1) & 31]) - base);
+          sr[0][j >> 1] = pack_half2(ex2f(__uint_as_float(sr[j >> 5][j & 31]) - base), ex2f(__uint_as_float(sr[(j + 1) >> 5][(j + 1) & 31]) - base));
         t4_tmem_st32(tmem_p, sr[0]);
         t4_tmem_st_wait();
         tc_fence_before();

@@ -1063,3 +1063,37 @@ def test_selection_in_a_step_of_unequal_sequences(q_lens, front, behind):
                                  torch.tensor(ctx, dtype=torch.int32, device="cuda"), max(q_lens), max(ctx), n_pages).cpu()
     want = _select_oracle(q[front : front + T], codes[0], exps[0], tables, q_lens, ctx, n_pages, 1, 4)
     assert torch.equal(got[front : front + T], want)
+
+
+@pytest.mark.parametrize("scale_byte_of_16ths", [11, 13, 15])
+@pytest.mark.parametrize("q_len,ctx", [(1, 32768), (16, 32768), (2, 9000)])
+def test_a_long_flat_tail_far_below_the_maximum_keeps_its_mass(scale_byte_of_16ths, q_len, ctx):
+    """One loud key in every second page of the first 32 (each warp of a CTA meets one at once), the other keys 16.5, 19.5 or 22.5 below them in
+    log2, all equal.  The loud keys' values are 0, the others' 1, so an output is the tail's share.
+
+    P of the tail is 2^(7 - gap) in f16: off by 2^-11 of itself or, below 2^-14, by 2^-25; scores, whole multiples of 2^-7 here, are exact up to
+    their fp32 sum (2^-18 of them); ex2 and the sums in fp32 2^-14 in all; then one rounding to bf16."""
+    import math
+
+    from daser_b200.ops import attention, kv_ops
+
+    n = -(-ctx // B)
+    k, v = torch.zeros(n, 1, B, D), torch.ones(n, 1, B, D)
+    loud = 6 * scale_byte_of_16ths / 64  # absmax 6 s with s = m / 64, four bits: exact in the format
+    k[0:32:2, 0, 0], v[0:32:2, 0, 0] = loud, 0.0
+    rec = codec.pack_kv4_records(k, v)[None]
+    kk, vv = codec.unpack_kv4_records(rec[0])
+    assert kk.max() == loud and (kk.unique().numel(), vv.unique().numel()) == (2, 2)
+    q = torch.ones(q_len, 8, D).to(torch.bfloat16)
+    tables = torch.arange(n, dtype=torch.int32)[None].cuda()
+    out = torch.zeros(q.shape, dtype=torch.bfloat16, device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    attention.paged_attention(q.cuda(), out, kv_ops.PagedKV4Pool.from_tensors([rec.cuda()]), 0, tables, torch.tensor([0, q_len], **i32),
+                              torch.tensor([ctx], **i32), q_len, ctx, 1, 0.125 / math.log2(math.e), None, nsplit=0 if q_len < 8 else 1)
+    gap = 0.125 * D * loud
+    one = float(vv.max())
+    for t in range(q_len):
+        tail = ctx - q_len + t + 1 - 16
+        share = tail * 2.0**-gap / (16 + tail * 2.0**-gap)
+        rel = max(2.0**-11, 2.0**-25 * 2.0 ** (gap - 7)) + gap * 2.0**-18 + 2.0**-14 + BF16_HALF
+        assert ((out[t].double().cpu() - one * share).abs() <= rel * one * share).all(), (gap, t, out[t, 0, 0].item() / (one * share))
