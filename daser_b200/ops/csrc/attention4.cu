@@ -26,7 +26,8 @@
 //   P^T in the layout of B is the transpose of S^T as it comes out: one movmatrix per 8 tokens.
 // * The running maximum is raised only when a page exceeds it by 2^8 (P is f16, sums are fp32): one vote a page instead of six
 //   shuffles.  Scores, sums and O are fp32; K, V are exact in f16; Q and P are rounded to f16, because the MMA takes no fp32 operand that
-//   keeps up with the memory: 2^-11 of their size, finer than bf16's 2^-8.  P of the maximum is 2^7 to 2^15, so that weights have those 11
+//   keeps up with the memory: 2^-11 of their size, finer than bf16's 2^-8 (a query at least 2^-25, which is 2^-11 of its row's largest;
+//   rows that f16 does not hold: plain_row).  P of the maximum is 2^7 to 2^15, so that weights have those 11
 //   bits down to 2^-21 of the largest and an absolute error of at most 2^-32 of it below (with P of 1 to 2^8 a long tail 2^-20 below one
 //   loud key was off by 2 %).
 //
@@ -226,6 +227,51 @@ struct Walk {
 };
 
 // ONE: the rows of an item are heads of one token and see the same keys (sparse, and dense with at most one query token per sequence).
+// One query row over pages [p0, page_end) of an item in plain fp32 products: for queries that f16 does not hold (scaled and rounded to f16 the
+// largest of a row is outside [2^-14, 2^15), where it would be infinite or few bits would be left).  The row is looked at when it is put
+// together, so that the warps that work on its pages have nothing to do with it.  With an infinite query the sum is NaN.
+// A warp; a lane has 4 dims.
+struct PlainItem {
+  const uint8_t* records;  // of the layer and KV head
+  int64_t stride_block;
+  const int32_t* table;
+  const int32_t* list;     // sparse
+  int p0, page_end, max_blocks, num_blocks;
+  float scale_log2;
+};
+struct PlainRow {
+  float4 acc;
+  float m, l;
+};
+__device__ __noinline__ void plain_row(const PlainItem* item, uint2 w, int pos, PlainRow* out) {
+  const PlainItem it = *item;
+  const int lane = threadIdx.x & 31;
+  const float qs[4] = {bf16_lo(w.x) * it.scale_log2, bf16_hi(w.x) * it.scale_log2, bf16_lo(w.y) * it.scale_log2, bf16_hi(w.y) * it.scale_log2};
+  const float top = warp_max(fmaxf(fmaxf(fabsf(qs[0]), fabsf(qs[1])), fmaxf(fabsf(qs[2]), fabsf(qs[3]))));
+  PlainRow r = {make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f};
+  for (int at = it.p0; at < it.page_end; ++at) {
+    const int page = it.list ? it.list[at] : at;
+    if (page < 0 || page >= it.max_blocks) continue;
+    const int blk = it.table[page];
+    const uint8_t* rec = it.records + (int64_t)(blk < 0 ? 0 : (blk >= it.num_blocks ? it.num_blocks - 1 : blk)) * it.stride_block;
+    for (int tok = 0; tok < DASER_KV4_TOKENS && page * DASER_KV4_TOKENS + tok <= pos; ++tok) {
+      float k[8], v[8];
+      fp4_decode8(*reinterpret_cast<const uint32_t*>(rec + kv4_code_at(0, tok, lane >> 1)), rec[kv4_scale_at(0, tok, lane >> 2)], k);
+      fp4_decode8(*reinterpret_cast<const uint32_t*>(rec + kv4_code_at(1, tok, lane >> 1)), rec[kv4_scale_at(1, tok, lane >> 2)], v);
+      const bool h = lane & 1;  // which half of the 8 dims
+      const float s = warp_sum(qs[0] * (h ? k[4] : k[0]) + qs[1] * (h ? k[5] : k[1]) + qs[2] * (h ? k[6] : k[2]) + qs[3] * (h ? k[7] : k[3]));
+      const float m = fmaxf(r.m, s), al = r.m == m ? 1.f : ex2f(r.m - m), e = top < INFINITY ? ex2f(s - m) : NAN;
+      r.m = m;
+      r.l = r.l * al + e;
+      r.acc.x = r.acc.x * al + e * (h ? v[4] : v[0]);
+      r.acc.y = r.acc.y * al + e * (h ? v[5] : v[1]);
+      r.acc.z = r.acc.z * al + e * (h ? v[6] : v[2]);
+      r.acc.w = r.acc.w * al + e * (h ? v[7] : v[3]);
+    }
+  }
+  *out = r;
+}
+
 template <int NT, bool SPARSE, bool ONE>
 __global__ void __launch_bounds__(A4<NT>::WARPS * 32, 1)
 attn4_kernel(const Attn4Params p) {
@@ -234,6 +280,7 @@ attn4_kernel(const Attn4Params p) {
   extern __shared__ __align__(128) uint8_t a4_smem[];  // ring [warp][stage][2 records], parts [warp][row][A4_OPITCH]
   __shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS];
   __shared__ int s_part[WARPS];
+  __shared__ PlainItem s_item;
   __shared__ int64_t s_at, s_T;  // where this CTA is in the order of all pages, and how many there are: thread 0's, out of its registers
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -556,6 +603,9 @@ attn4_kernel(const Attn4Params p) {
         if (part >= 0) *reinterpret_cast<float4*>(dst + 2 * j) = make_float4(o[nt][j][e], o[nt][j][2 + e], o[nt][j + 1][e], o[nt][j + 1][2 + e]);
     }
   if (lane == 0) s_part[warp] = part;
+  if (threadIdx.x == 32)
+    s_item = {p.records + (int64_t)kvh * p.stride_head, p.stride_block, p.block_tables + (int64_t)it.seq * p.max_blocks, it.list, it.p0, it.page_end,
+              p.max_blocks, p.num_blocks, p.scale_log2};
   const bool begins = it.p0 == 0, whole = begins && it.p1 == it.n_item;
   const int64_t slot = ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * ROWS;  // of a partial: 0 continues an item, 1 begins one
   if (p.workers && threadIdx.x == 0) {
@@ -596,13 +646,22 @@ attn4_kernel(const Attn4Params p) {
       lt += f * s_l[w][r];
       acc.x += there ? f * v.x : 0.f; acc.y += there ? f * v.y : 0.f; acc.z += there ? f * v.z : 0.f; acc.w += there ? f * v.w : 0.f;
     }
+    const int tq = SPARSE ? tok0 : row / G, h = SPARSE ? row : row % G;
+    const int64_t at = ((int64_t)(q0 + tq) * p.Hq + kvh * G + h) * ATT_D;  // in q and out
+    const uint2 qw = *reinterpret_cast<const uint2*>(p.q + at + 4 * lane);
+    if (odd_row(__reduce_max_sync(0xffffffffu, top_half(top_bf16(0u, make_uint4(qw.x, qw.y, 0u, 0u)))), p.q_lo, p.q_hi)) {
+      PlainRow pr;
+      plain_row(&s_item, qw, first_pos + tq - tok0, &pr);
+      acc = pr.acc;
+      mx = pr.m;
+      lt = pr.l;
+    }
     const float inv = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);  // no key: zeros; NaN stays
     if (whole) {
-      const int tq = SPARSE ? tok0 : row / G, h = SPARSE ? row : row % G;
       uint2 w2;
       w2.x = pack_bf16x2(acc.x * inv, acc.y * inv);
       w2.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-      *reinterpret_cast<uint2*>(p.out + ((int64_t)(q0 + tq) * p.Hq + kvh * G + h) * ATT_D + 4 * lane) = w2;
+      *reinterpret_cast<uint2*>(p.out + at + 4 * lane) = w2;
     } else {
       *reinterpret_cast<float4*>(p.part_o + (slot + r) * ATT_D + 4 * lane) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
       if (lane == 0) p.part_lse[slot + r] = lt > 0.f ? mx + log2f(lt) : (lt == 0.f ? -INFINITY : lt);
@@ -817,6 +876,12 @@ static int fill_attn4(Attn4Params& p, const void* q, void* out, float* part_o, f
   p.nsplit = 1;
   p.split_pages = 0;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  // with the scale's exponent e, |q| in [2^(-14 - e), 2^(14 - e)) keeps |q scale| in [2^-14, 2^15)
+  int e = 0;
+  if (p.scale_log2 != 0.f && isfinite(p.scale_log2)) frexpf(p.scale_log2, &e), --e;
+  const int lo = 127 - 14 - e, hi = 127 + 14 - e;
+  p.q_lo = (uint32_t)(lo < 0 ? 0 : lo > 255 ? 255 : lo) << 7;
+  p.q_hi = (uint32_t)(hi < 0 ? 0 : hi > 255 ? 255 : hi) << 7;
   p.total_q = total_q;
   return 0;
 }

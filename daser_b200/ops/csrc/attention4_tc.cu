@@ -120,6 +120,14 @@ __device__ __noinline__ void t4_leave_out_bad_values(uint8_t* raw, int* bad_v, i
   __syncwarp();
 }
 
+// The scale of a query row (null: none).
+__device__ __noinline__ RowScale t4_row_scale(const __nv_bfloat16* q, float scale_log2, uint32_t q_lo, uint32_t q_hi) {
+  uint32_t top = 0u;
+  if (q != nullptr)
+    for (int i = 0; i < ATT_D / 8; ++i) top = top_bf16(top, *reinterpret_cast<const uint4*>(q + 8 * i));
+  return row_scale(top_half(top), scale_log2, q_lo, q_hi);
+}
+
 __global__ void __launch_bounds__(T4_THREADS, 1)
 attn4_tc_kernel(const Attn4Params p, int groups) {
   extern __shared__ uint8_t t4_smem_raw[];
@@ -237,16 +245,22 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
       const uint32_t tmem_o = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t4_o_col(tile);
       const uint32_t tmem_p = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t4_p_col(tile);
       uint8_t* my_q = q_s + tile * T4_Q_BYTES;
-      // Q -> f16, times scale * log2(e), into the swizzled A tile
+      // Q -> f16, times scale * log2(e), into the swizzled A tile.  Rows with a scale of their own (row_scale) are looked for by 8 dims: if all
+      // of the warp's are in the range, or zero, so are the rows.
+      RowScale rs = {p.scale_log2, 1.f};
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) odd |= odd_row(top_half(top_bf16(0u, qw[i])), p.q_lo, p.q_hi);
+      odd = __any_sync(0xffffffffu, odd);
+      if (odd) rs = t4_row_scale(valid ? p.q + row * ATT_D : nullptr, p.scale_log2, p.q_lo, p.q_hi);
+      const bool plain = valid && rs.factor == 1.f;  // keys in front of the causal edge count as they are
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int r = (warp & 3) * 32 + 2 * i + (lane >> 4), ck = lane & 15;
         const uint4 w = qw[i];
-        uint4 h;
-        h.x = pack_half2(bf16_lo(w.x) * p.scale_log2, bf16_hi(w.x) * p.scale_log2);
-        h.y = pack_half2(bf16_lo(w.y) * p.scale_log2, bf16_hi(w.y) * p.scale_log2);
-        h.z = pack_half2(bf16_lo(w.z) * p.scale_log2, bf16_hi(w.z) * p.scale_log2);
-        h.w = pack_half2(bf16_lo(w.w) * p.scale_log2, bf16_hi(w.w) * p.scale_log2);
+        const float sc = odd ? __shfl_sync(0xffffffffu, rs.scale, 2 * i + (lane >> 4)) : p.scale_log2;
+        auto two = [&](uint32_t x) { return pack_half2(bf16_lo(x) * sc, bf16_hi(x) * sc); };
+        const uint4 h = make_uint4(two(w.x), two(w.y), two(w.z), two(w.w));
         *reinterpret_cast<uint4*>(my_q + (ck >> 3) * 16384 + r * 128 + (((ck & 7) ^ (r & 7)) << 4)) = h;
       }
       t4_fence_async();
@@ -265,12 +279,12 @@ attn4_tc_kernel(const Attn4Params p, int groups) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.s_free[tile]);
-        if (!(valid && key0 + T4_NK - 1 <= pos && key0 + T4_NK <= key_end)) {
-          // the causal edge or the end of the range runs through this tile
+        if (!(plain && key0 + T4_NK - 1 <= pos && key0 + T4_NK <= key_end)) {
+          // the causal edge or the end of the range runs through this tile, or the row has a scale of its own
 #pragma unroll
           for (int j = 0; j < T4_NK; ++j) {
             const int key = key0 + j;
-            if (!(valid && key < key_end && key <= pos)) sr[j >> 5][j & 31] = 0xff800000u;  // -inf
+            sr[j >> 5][j & 31] = valid && key < key_end && key <= pos ? __float_as_uint(__uint_as_float(sr[j >> 5][j & 31]) * rs.factor) : 0xff800000u;  // -inf
           }
         }
         float mx0 = -INFINITY, mx1 = -INFINITY;

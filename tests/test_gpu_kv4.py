@@ -1097,3 +1097,92 @@ def test_a_long_flat_tail_far_below_the_maximum_keeps_its_mass(scale_byte_of_16t
         share = tail * 2.0**-gap / (16 + tail * 2.0**-gap)
         rel = max(2.0**-11, 2.0**-25 * 2.0 ** (gap - 7)) + gap * 2.0**-18 + 2.0**-14 + BF16_HALF
         assert ((out[t].double().cpu() - one * share).abs() <= rel * one * share).all(), (gap, t, out[t, 0, 0].item() / (one * share))
+
+
+@pytest.mark.parametrize("size,key,scale", [(2e5, 2e-5, 1.0), (1e30, 4e-6, 1e-25), (1.0, 3e4, 1e-6), (1e-30, 5.0, 1e29), (5e37, 4e-6, 1e-33)])
+@pytest.mark.parametrize("q_len,split", [(1, None), (1, 5), (5, 0), (16, None), (40, 2)])
+def test_queries_beyond_the_range_of_f16(q_len, split, size, key, scale):
+    """Scaled queries far above 65504 and far below 2^-14 (where f16 has fewer bits): each row as the formula has it.  One row of ordinary
+    size, one of zeros among them."""
+    from daser_b200.ops import attention, kv_ops
+
+    ctx = 300
+    _, rec, tables, q, start = _setup([q_len], [ctx], 8, 1, seed=95)
+    g = torch.Generator().manual_seed(96)
+    k, v = torch.randn(rec.shape[1], 1, B, D, generator=g) * key, torch.randn(rec.shape[1], 1, B, D, generator=g)
+    rec = codec.pack_kv4_records(k, v)[None]
+    q = (q.float() * size / 2).to(torch.bfloat16)
+    q[0, 3] = 0
+    q[-1, 5] = torch.randn(D, generator=g).to(torch.bfloat16)
+    assert torch.isfinite(q.float()).all()
+    out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    attention.paged_attention(q.cuda(), out, kv_ops.PagedKV4Pool.from_tensors([rec.cuda()]), 0, tables.cuda(), start.cuda(), torch.tensor([ctx], **i32),
+                              q_len, ctx, 1, scale, None, nsplit=split)
+    want, tol = _oracle(rec[0], tables, q, [q_len], [ctx], scale, prefill=q_len > 7)
+    got = out.double().cpu()
+    assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
+
+
+@pytest.mark.parametrize("q_len,split", [(1, None), (3, 4), (16, None)])
+def test_small_queries_against_large_keys(q_len, split):
+    """A scaled query of 2.5 * 2^-24 is 2 * 2^-24 in f16, a fifth less: values that have the sign of their key's score show it."""
+    import math
+
+    from daser_b200.ops import attention, kv_ops
+
+    ctx, scale = 300, 2.5 * 2.0**-24 / math.log2(math.e)
+    _, rec, tables, q, start = _setup([q_len], [ctx], 8, 1, seed=97)
+    g = torch.Generator().manual_seed(98)
+    sign = torch.where(torch.randn(D, generator=g) > 0, 1.0, -1.0)
+    q = sign.expand(q.shape).to(torch.bfloat16).contiguous()
+    k = torch.randn(rec.shape[1], 1, B, D, generator=g) * 1e4 + sign * 4e3 * torch.randn(rec.shape[1], 1, B, 1, generator=g)
+    v = torch.sign((k * sign).sum(-1, keepdim=True)).expand(k.shape)
+    rec = codec.pack_kv4_records(k, v)[None]
+    out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    attention.paged_attention(q.cuda(), out, kv_ops.PagedKV4Pool.from_tensors([rec.cuda()]), 0, tables.cuda(), start.cuda(), torch.tensor([ctx], **i32),
+                              q_len, ctx, 1, scale, None, nsplit=split)
+    want, tol = _oracle(rec[0], tables, q, [q_len], [ctx], scale, prefill=q_len > 7)
+    got = out.double().cpu()
+    assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
+
+
+@pytest.mark.parametrize("q_len,split", [(1, None), (1, 5), (2, 0), (16, None), (40, 2)])
+def test_a_query_that_is_not_finite_is_nan_in_its_row_alone(q_len, split):
+    """Also where every score is minus infinity, which is not the same as no key."""
+    from daser_b200.ops import kv_ops
+
+    ctx = 300
+    _, rec, tables, q, start = _setup([q_len], [ctx], 8, 1, seed=99)
+    k, v = codec.unpack_kv4_records(rec[0])
+    rec = codec.pack_kv4_records(-k.abs() - 0.5, v)[None]  # no key of 0
+    want, tol = _oracle(rec[0], tables, q, [q_len], [ctx], D**-0.5, prefill=q_len > 7)
+    q[0, 3, 77], q[-1, 6, 5] = float("inf"), float("nan")
+    q[0, 1, 0] = float("-inf")
+    got = _attend(kv_ops.PagedKV4Pool.from_tensors([rec.cuda()]), 0, tables, q, start, [ctx], q_len, 1, split)
+    bad = torch.zeros(q_len, 8, dtype=torch.bool)
+    bad[0, 1] = bad[0, 3] = bad[-1, 6] = True
+    assert torch.isnan(got[bad]).all() and ((got - want).abs() <= tol)[~bad].all()
+
+
+@pytest.mark.parametrize("parts", [0, 7])
+def test_sparse_queries_beyond_the_range_of_f16(parts):
+    attention, _, _ = _ops()
+    from daser_b200.ops import kv_ops
+
+    q_lens, ctx_lens = [1, 2], [500, 230]
+    _, rec, tables, q, start = _setup(q_lens, ctx_lens, 32, 2, seed=100)
+    g = torch.Generator().manual_seed(101)
+    k, v = torch.randn(rec.shape[1], 2, B, D, generator=g) * 2e-5, torch.randn(rec.shape[1], 2, B, D, generator=g)
+    rec = codec.pack_kv4_records(k, v)[None]
+    q = (q.float() * 1e6).to(torch.bfloat16)
+    q[1, 17:30] *= 1e-6
+    pages = torch.full((3, 2, 12), -1, dtype=torch.int32)
+    pages[:, 0, :9] = torch.tensor([0, 2, 3, 5, 7, 8, 11, 13, 14])
+    pages[:, 1, :5] = torch.tensor([1, 4, 6, 10, 12])
+    out = torch.zeros(q.shape, dtype=torch.bfloat16, device="cuda")
+    attention._attention_kv4(q.cuda(), out, kv_ops.PagedKV4Pool.from_tensors([rec.cuda()]), 0, tables.cuda(), start.cuda(),
+                             torch.tensor(ctx_lens, dtype=torch.int32, device="cuda"), 2, 0, D**-0.5, None, 0, pages.cuda(), parts)
+    want, tol = _oracle(rec[0], tables, q, q_lens, ctx_lens, D**-0.5, pages=pages)
+    assert ((out.double().cpu() - want).abs() <= tol).all()
