@@ -595,6 +595,7 @@ DASER_API int daser_paged_attention_fp8(const void* q, void* out, float* part_o,
     if (e != cudaSuccess) return (int)e;
     e = cudaFuncSetAttribute(paged_attn_fp8_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PF_SMEM);
     if (e != cudaSuccess) return (int)e;
+    daser_used_on_device(configured);
   }
   if (attention_tc_enabled() && max_q_len * G >= 64 && 128 % G == 0) {
     // at least half of a 128-row MMA tile per KV head: the tcgen05 kernel

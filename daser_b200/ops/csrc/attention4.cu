@@ -833,6 +833,7 @@ static int launch_attn4(Attn4Params& p, int max_q_len, cudaStream_t stream) {
   if (daser_first_use_on_device(configured)) {
     cudaError_t e = cudaFuncSetAttribute(attn4_kernel<NT, SPARSE, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;
+    daser_used_on_device(configured);
   }
   p.max_q_len = max_q_len;
   p.tiles = SPARSE ? max_q_len : (max_q_len * p.G + C::ROWS - 1) / C::ROWS;

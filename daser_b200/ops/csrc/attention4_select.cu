@@ -383,6 +383,7 @@ DASER_API int daser_select_pages_kv4(const void* q, const int8_t* codes, const i
   if (daser_first_use_on_device(configured)) {
     cudaError_t e = cudaFuncSetAttribute(attn4_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SELECT_KEYS * 4);
     if (e != cudaSuccess) return (int)e;
+    daser_used_on_device(configured);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * Hkv * cluster));

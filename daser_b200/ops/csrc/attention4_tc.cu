@@ -568,6 +568,7 @@ int daser_launch_attention4_tc(const daser::Attn4Params& p, int max_q_len, cudaS
   if (daser_first_use_on_device(configured)) {
     cudaError_t e = cudaFuncSetAttribute(attn4_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T4_SMEM);
     if (e != cudaSuccess) return (int)e;
+    daser_used_on_device(configured);
   }
   const int toks = 2 * (128 / p.G);
   const int groups = (max_q_len + toks - 1) / toks;

@@ -450,6 +450,7 @@ int daser_launch_attention_tc(const daser::AttnParams& p, int max_q_len, cudaStr
   if (daser_first_use_on_device(configured)) {
     cudaError_t e = cudaFuncSetAttribute(paged_attn_fp8_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TC_SMEM);
     if (e != cudaSuccess) return (int)e;
+    daser_used_on_device(configured);
   }
   const int groups = (max_q_len * p.G + 127) / 128;
   const dim3 grid(p.Hkv, p.num_seqs, groups * p.nsplit);

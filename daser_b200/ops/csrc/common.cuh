@@ -11,16 +11,19 @@
 
 #include "kv_paged.h"  // DASER_ERR_* return codes and the host-visible parameter blocks
 
-// True the first time it is called for the current device with this `flags` array: attributes
-// set with cudaFuncSetAttribute belong to a device, so a process that drives several GPUs has to
-// set them once on each.
+// True until daser_used_on_device has been called for the current device with this `flags` array: attributes set with
+// cudaFuncSetAttribute belong to a device, so a process that drives several GPUs has to set them once on each.  The
+// caller marks the device when they are set, not before: a second thread that arrives meanwhile sets them too (which
+// is harmless) instead of launching without them.
 #define DASER_MAX_DEVICES 64
-static inline bool daser_first_use_on_device(bool (&flags)[DASER_MAX_DEVICES]) {
+static inline bool daser_first_use_on_device(const bool (&flags)[DASER_MAX_DEVICES]) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= DASER_MAX_DEVICES) return true;
-  if (flags[dev]) return false;
-  flags[dev] = true;
-  return true;
+  return !__atomic_load_n(&flags[dev], __ATOMIC_ACQUIRE);
+}
+static inline void daser_used_on_device(bool (&flags)[DASER_MAX_DEVICES]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < DASER_MAX_DEVICES) __atomic_store_n(&flags[dev], true, __ATOMIC_RELEASE);
 }
 
 // Status words written by kernels whose waits ran out (see signals.cuh).

@@ -543,6 +543,7 @@ static int launch(const CUtensorMap& ta, const CUtensorMap& tb, const GemmParams
     cudaError_t e = cudaFuncSetAttribute(gemm_tcgen05_kernel<BN, STAGES, FUSED>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, S::DYNAMIC);
     if (e != cudaSuccess) return (int)e;
+    daser_used_on_device(configured);
   }
   const dim3 grid((p.N + BN - 1) / BN, (p.M + GEMM_BM - 1) / GEMM_BM, p.k_splits);
   // Programmatic dependent launch: CTAs of this grid may be scheduled while the previous

@@ -1186,3 +1186,14 @@ def test_sparse_queries_beyond_the_range_of_f16(parts):
                              torch.tensor(ctx_lens, dtype=torch.int32, device="cuda"), 2, 0, D**-0.5, None, 0, pages.cuda(), parts)
     want, tol = _oracle(rec[0], tables, q, q_lens, ctx_lens, D**-0.5, pages=pages)
     assert ((out.double().cpu() - want).abs() <= tol).all()
+
+
+def test_first_calls_of_a_process_from_several_threads():
+    """A kernel's shared memory has to be asked for once per device before its first launch: by whichever thread is first."""
+    import os
+    import subprocess
+    import sys
+
+    worker = os.path.join(os.path.dirname(os.path.abspath(__file__)), "kv4_threads_worker.py")
+    done = subprocess.run([sys.executable, worker], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stdout + done.stderr
