@@ -188,6 +188,9 @@ def _rope_kv4_write(qkv, positions, slot_mapping, cos_sin, q_out, hq, hkv, head_
     T, cols = qkv.shape
     step, unit = qkv.stride()
     need(cols >= (hq + 2 * hkv) * head_dim and unit == 1, "qkv: too few columns, or columns with a stride")
+    if T <= 1:
+        step = 0  # (of a single row it is anything)
+    need(not zero_after or T <= 1 or abs(step) >= (hq + 2 * hkv) * head_dim, "qkv: rows that overlap cannot be zeroed")
     _lib.check_tensor(positions, "positions", torch.int32, dev)
     _lib.check_tensor(slot_mapping, "slot_mapping", torch.int64, dev)
     _lib.check_tensor(cos_sin, "cos_sin", torch.float32, dev)

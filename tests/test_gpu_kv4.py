@@ -1197,3 +1197,31 @@ def test_first_calls_of_a_process_from_several_threads():
     worker = os.path.join(os.path.dirname(os.path.abspath(__file__)), "kv4_threads_worker.py")
     done = subprocess.run([sys.executable, worker], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stdout + done.stderr
+
+
+def test_row_strides_of_the_projections():
+    """One row of a tensor whose rows are off the vector grid is taken; rows that are one row repeated are read, but not zeroed under one another."""
+    _, ew, kv_ops = _ops()
+    hq, hkv = 8, 2
+    cols = (hq + 2 * hkv) * D
+    pool = kv_ops.PagedKV4Pool.zeros(1, 2, hkv, "cuda")
+    cos_sin = kv_ops.rope_table(32, inv_freq_table(D, 10000.0), "cuda")
+    q_out = torch.zeros(3, hq, D, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator().manual_seed(102)
+    wide = torch.randn(3, cols + 3, generator=g).cuda()
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    ew.rope_kv_write(wide[:1, :cols], i(3), i(5).long(), cos_sin, q_out, hq, hkv, D, B, pool, 0)
+    want = _rope_ref(wide[:1, : hq * D].float().reshape(1, hq, D).cpu(), cos_sin.cpu()[3:4]).to(torch.bfloat16)
+    assert torch.equal(q_out[:1].cpu(), want)
+    k, v = kv_ops.kv_read(pool, 0, i(5).long())
+    assert torch.equal(v.float().cpu()[0], codec.dequantize_fp4b16(*codec.quantize_fp4b16(wide[0, (hq + hkv) * D : cols].reshape(hkv, D).to(torch.bfloat16).float().cpu())))
+    with pytest.raises(Exception):
+        ew.rope_kv_write(wide[:3, :cols], i(3, 3, 3), i(5, 6, 7).long(), cos_sin, q_out, hq, hkv, D, B, pool, 0)  # three such rows
+    same = torch.randn(1, cols, generator=g).cuda()
+    rep = same.expand(3, cols)
+    ew.rope_kv_write(rep, i(3, 3, 3), i(5, 6, 7).long(), cos_sin, q_out, hq, hkv, D, B, pool, 0)
+    assert torch.equal(q_out[0], q_out[2])
+    before = same.clone()
+    with pytest.raises(ValueError):
+        ew.rope_kv_write(rep, i(3, 3, 3), i(5, 6, 7).long(), cos_sin, q_out, hq, hkv, D, B, pool, 0, zero_after=True)
+    assert torch.equal(same, before)
