@@ -615,7 +615,7 @@ attn4_kernel(const Attn4Params p) {
       const int n = whole ? 1 : owner_of(s_at + it.n_item - 1, s_T, sharers(s_T, p.workers)) - (int)blockIdx.x + 1;
       p.shared[id] = make_int2((int)blockIdx.x, n);
     }
-   s_at += it.p1 - it.p0;
+    s_at += it.p1 - it.p0;
   }
   // ---- the next item: its first pages, but for the stage that holds this warp's part ----
   cp_async_wait<0>();  // (groups that were empty)

@@ -281,7 +281,8 @@ def update_page_bounds(pool: PagedKV4Pool, bounds: PageBounds, layer: int, block
                        ctx_lens: torch.Tensor, max_q_len: int, rank: int = 0) -> None:
     """Recompute the bounds of every page that holds one of a sequence's last ``q_start[s+1] - q_start[s]`` tokens (the step's
     new ones; after a restore, the restored ones).  Arguments as ``paged_attention`` takes them; call it behind the step's
-    ``rope_kv_write``."""
+    ``rope_kv_write``.  ``max_q_len`` has to be at least the most tokens of a sequence: pages beyond it are not looked at.  Of a page the
+    tokens below ``ctx_len`` count; where sequences share a page that the call recomputes, they have to see the same tokens of it."""
     pool.check(layer, rank)
     _lib.require(bounds.shape == (pool.num_layers, pool.num_blocks, pool.heads_per_rank) and bounds.index == pool.index,
                  "the bounds belong to a pool of another shape or device")
