@@ -170,10 +170,12 @@ def paged_attention(
     """``q, out``: bf16 ``[Tq, Hq, D]``; sequences given by ``q_start`` (prefix sums) and ``ctx_lens``.
 
     The K/V of the new tokens must already be in the pool; row ``t`` of a sequence attends
-    keys ``0 .. ctx_len - q_len + t`` (a row with none gets zeros); rows behind the last sequence are left as they were.
+    keys ``0 .. ctx_len - q_len + t`` (a row with none gets zeros); rows of no sequence are left as they were.
 
     Over a :class:`~daser_b200.ops.kv_ops.PagedKV4Pool` any group of up to 16 query heads per KV head is taken,
-    ``max_ctx`` has to be at least the longest context, ``max_q_len`` at least the most query tokens of a sequence, and ``workspace`` may be ``None`` (scratch of the call's own).
+    ``max_ctx`` has to be at least the longest context (it may be a capacity), ``max_q_len`` at least the most query tokens of a sequence (those
+    beyond it are left alone), and ``workspace`` may be ``None`` (scratch of the call's own).  A value that is not finite shows in the rows that see
+    it.  Queries are rounded to f16 once they are scaled; a row that f16 does not hold takes a slower way (scores have to fit fp32).
     ``nsplit`` then is the first value of :func:`plan_kv4`.
     """
     if isinstance(pool, PagedKV4Pool):
@@ -284,8 +286,10 @@ def select_pages(
     behind the last.
 
     Always the first ``sink_pages`` and the last ``recent_pages`` (at least one: the page of the newest key, whose bounds need not be
-    up to date) of the pages a row sees; the other places go to the highest bounds on the sum of the group's scores, the lower
-    page first among equals.  A row that sees at most ``num_pages`` pages gets them all.  Rows of no sequence are not set.  ``bounds`` have to cover the context
+    up to date) of the pages a row sees; the other places go to the highest estimates of the largest sum of the group's scores, the lower
+    page first among equals.  The estimate is what the bounds give for the query rounded to int8 under one power of two: in whole numbers, and
+    up to half a step per dim on either side of the bound itself.  A row that sees at most ``num_pages`` pages gets them all.  Rows of no
+    sequence, and query tokens beyond ``max_q_len`` (at most 65535), are not set.  ``bounds`` have to cover the context
     (:func:`~daser_b200.ops.kv_ops.update_page_bounds`); other arguments as in :func:`paged_attention`.
     """
     (layers, nb, Hkv), dev = bounds.shape, bounds.index
@@ -323,8 +327,8 @@ def sparse_paged_attention(
 ) -> torch.Tensor:
     """:func:`paged_attention` over the pages of ``pages`` (int32 ``[Tq, Hkv, n]``, as :func:`select_pages` gives them): row ``t``
     of a sequence attends the keys of its listed pages up to ``ctx_len - q_len + t``.  Every query row reads its own list: a
-    decode operator, for one or a few query tokens per sequence.  Pages have to be distinct within a list (one listed
-    twice counts twice); entries outside the context are skipped."""
+    decode operator, for one or a few query tokens per sequence, at most 65535 rows.  Pages have to be distinct within a list (one listed
+    twice counts twice); entries outside the context are skipped.  Rows of no sequence, and query tokens beyond ``max_q_len``, are left alone."""
     _lib.require(isinstance(pool, PagedKV4Pool), "sparse attention works on a PagedKV4Pool")
     _lib.require(pages.dim() == 3 and pages.shape[2] >= 1 and tuple(pages.shape[:2]) == (q.shape[0], pool.heads_per_rank),
                  "pages: int32 [rows, KV heads, pages]")

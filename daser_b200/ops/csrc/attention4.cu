@@ -31,11 +31,15 @@
 //   bits down to 2^-21 of the largest and an absolute error of at most 2^-32 of it below (with P of 1 to 2^8 a long tail 2^-20 below one
 //   loud key was off by 2 %).
 //
-// Measured (L2 flushed in front of each call): 32 sequences of 4k - 32k tokens, 64 / 8 heads, 681 MB: 130 us, 5.2 TB/s (a copy: 6.5);
-// the ALU is 57 % busy (conversions, byte selection), the tensor pipe 29 %.  4 sequences of 50k - 120k tokens on one KV head, 49 MB: 22 us +
+// Measured (L2 flushed in front of each call): 32 sequences of 4k - 32k tokens, 64 / 8 heads, 681 MB: 132 us, 5.2 TB/s (a copy: 6.5);
+// the ALU is 56 % busy (conversions, byte selection), the tensor pipe 28 %.  4 sequences of 50k - 120k tokens on one KV head, 49 MB: 22 us +
 // merge, of which 3 go by before the first page is asked for (lengths, table: dependent misses), 6 until the first pair of all
-// warps is there, and 3 for putting warps and CTAs together.  One sequence of 327 keys: 7 us, latency alone.  16 lists of 128
-// pages, 64 / 8 heads, 38 MB: 19 us.
+// warps is there, and 3 for putting warps and CTAs together.  One sequence of 327 keys: 6 us, latency alone.  16 lists of 128
+// pages, 64 / 8 heads, 38 MB: 17 us.  More query rows take more passes over the pages, 16 rows each, with 8 warps a CTA (240 registers): 16
+// sequences of 8k - 16k tokens and 64 / 8 heads, 229 MB, take 144 us for 4 new tokens each and 232 for 7, 180 TFLOP/s either
+// way; 16 heads per KV head, 32 sequences of 4k - 32k tokens, 170 MB: 61 us.
+// Registers bind the form for 8 rows: at 128 a thread the dense kernel spills 24 bytes, and code added to the loop over pages costs some
+// 2 % whether it runs or not.
 #include "attention4_params.cuh"
 
 namespace daser {
@@ -230,7 +234,7 @@ struct Walk {
 // One query row over pages [p0, page_end) of an item in plain fp32 products: for queries that f16 does not hold (scaled and rounded to f16 the
 // largest of a row is outside [2^-14, 2^15), where it would be infinite or few bits would be left).  The row is looked at when it is put
 // together, so that the warps that work on its pages have nothing to do with it.  With an infinite query the sum is NaN.
-// A warp; a lane has 4 dims.
+// A warp; a lane has 4 dims.  One sequence of 4096 keys, 64 / 8 heads: 246 us for such queries, 13 for others.
 struct PlainItem {
   const uint8_t* records;  // of the layer and KV head
   int64_t stride_block;

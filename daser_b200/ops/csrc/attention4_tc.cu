@@ -10,15 +10,15 @@
 //                one conversion yields the two neighbours of a V^T row.  A row of ones in V^T sums the rows of the P that was multiplied;
 //   * 12         issues the MMAs, S0(i), O0 += P0(i-1) V(i-1), S1(i), O1 += P1(i-1) V(i-1): M 128, N 64, K 128 and M 128, N 144, K 64;
 //   * 13         fetches: a tile is four bulk copies of 2304 bytes, three tiles ahead.
-// Measured: 2048 tokens over 8192 keys, 32 / 8 heads, 241 GFLOP: 285 us, 845 TFLOP/s.  256 CTAs on 148 SMs are 1.73 waves: of the
-// cycles that an SM is at work the tensor pipe is active in 45 %, the ALU in 44 and the exponential's unit in 43.  What binds is shared
+// Measured: 2048 tokens over 8192 keys, 32 / 8 heads, 241 GFLOP: 283 us, 850 TFLOP/s.  256 CTAs on 148 SMs are 1.73 waves: of the
+// cycles that an SM is at work the tensor pipe is active in 46 %, the ALU in 39 and the exponential's unit in 43.  What binds is shared
 // memory: a tile moves 174 KB (Q and K into the scores 96, V^T 37, dequantised tiles 32, records 9), 1360 cycles at 128 bytes, of the
 // some 2000 that it takes; the warp that issues the MMAs waits for operands in a quarter of them only.  (Exponents before the wait
-// for the last P V: 293 us; their maximum in packed f16: 302.)  64 tokens over 3328 keys, 64 / 8 heads (9 splits of 6 tiles): 20 us + merge, half of it before
-// the first MMA and behind the last.
+// for the last P V were 3 % slower, their maximum in packed f16 6 %.)  64 tokens over 3328 keys, 64 / 8 heads (9 splits of 6 tiles): 25 us with
+// the merge, half of it before the first MMA and behind the last.
 // Rounded to f16: Q and P, 2^-11 of their size, P below 2^-21 of a row's maximum to 2^-32 of that.  Exponents are fp32: an f16 exponential
-// of rounded exponents took 288 us instead of 292, but was off by up to 2^-8 where the maximum lags, and P of 1 to 2^8 lost what
-// lies 2^-20 below the maximum, 2 % of a long flat tail.
+// of rounded exponents was 1.4 % faster, but off by up to 2^-8 where the maximum lags, and P of 1 to 2^8 lost what
+// lies 2^-20 below the maximum, 2 % of a long flat tail.  Rows whose queries f16 does not hold have a scale of their own (row_scale).
 // Every mbarrier wait is bounded; on expiry the CTA records it in a status word, frees its TMEM and returns.
 #include "attention4_params.cuh"
 

@@ -63,8 +63,8 @@ __device__ __forceinline__ void load_pairs4(const float* p, uint64_t (&x)[4]) {
 // Bound by bytes: the projections in, the queries out, 72 B a row into the pool.  A thread takes 8 dims and their rotary
 // partners, so that a warp's access is four runs of 128 contiguous bytes and the two halves of a scale group sit
 // on neighbouring lanes (one shuffle joins their maxima); it keeps the token's cosines in registers for all its heads.
-// 4096 tokens of 32 / 8 heads, bf16, 88 MB: 17.2 us, 5.1 TB/s (18.4 with every trip's values read in the trip itself); 64 tokens of
-// 64 / 8 heads, fp32: 4 us, a launch and three dependent misses.
+// 4096 tokens of 32 / 8 heads, bf16, 88 MB: 17.2 us, 5.1 TB/s (18.4 with every trip's values read in the trip itself), 19 with the
+// per-head norm (72 registers, 4 bytes spilled); 64 tokens of 64 / 8 heads, fp32: 4 us, a launch and three dependent misses.
 template <typename TIn, bool QKNORM>
 __global__ void __launch_bounds__(128)
 kv4_write_kernel(TIn* __restrict__ qkv, int64_t qkv_stride, const int32_t* __restrict__ positions,
@@ -175,8 +175,8 @@ kv4_write_kernel(TIn* __restrict__ qkv, int64_t qkv_stride, const int32_t* __res
 // ---- read by slot ------------------------------------------------------------------------------------------------
 //
 // k, v [T][H][128] bf16 of the tokens that slot_mapping names, exact (e2m1 * scale has six significant bits); a slot below zero,
-// or beyond the pool, reads as zeros.  A thread takes 8 dims: 4 bytes in, 16 out, 16 lanes a row.  Bound by the 256 bytes written a
-// row; 4096 tokens of 8 heads, 21 MB: 8 us, mostly latency.
+// or beyond the pool, reads as zeros.  A thread takes 8 dims: 4 bytes in, 16 out, 16 lanes a row.  Its floor is the 256 bytes written a
+// row; 4096 tokens of 8 heads, 21 MB, take 7 us against 3.2: one item in flight a thread, behind the load of its slot.
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(const uint8_t* __restrict__ pool, int64_t stride_block, int64_t stride_head, int num_blocks,
                 const int64_t* __restrict__ slot_mapping, __nv_bfloat16* __restrict__ k, __nv_bfloat16* __restrict__ v,
@@ -205,9 +205,11 @@ kv4_read_kernel(const uint8_t* __restrict__ pool, int64_t stride_block, int64_t 
 // One CTA per (slot, layer, up to KV4_HEADS heads).  An item is one scale group of a row and its rotary partner: dequantised,
 // rotated by the slot's delta (keys), quantised, and put into the record's place in shared memory; whole records
 // then leave as 16-byte stores.  Stored directly, the 8-byte pieces of V would each be a quarter of a 32-byte sector.
-// Bound by instructions: 208 slots of 10 layers and 8 heads (85 MB in, 38 out) take 42 us where a copy of the bytes takes 19: ALU 41 %,
-// FMA 30 % busy with dequantisation, rotation, maxima and rounding.  (57 us with a division per group in place of the table of
-// reciprocals and without reading an item ahead.)
+// 208 slots of 10 layers and 8 heads (85 MB in, 38 out) take 41 us from fp8 images, 47 from bf16 ones (136 MB in), where a copy of the
+// bytes takes 19 and 27.  No unit is full (ALU 40 %, FMA 42, memory 45): a CTA makes its table, loads, computes and stores one after the
+// other, three of them an SM (80 registers), and waits longest for its loads.  (57 us with a division per group in place of the table of
+// reciprocals and without reading an item ahead.)  The pool's bases are indexed by rank, so each thread has the parameter in local
+// memory (104 bytes), here and in the save.
 constexpr int KV4_HEADS = 8;
 constexpr int KV4_PITCH = DASER_KV4_RECORD + 32;  // of a record in shared memory: the rows of eight heads start in different banks
 
@@ -337,8 +339,9 @@ kv4_restore_kernel(const DaserKVJob job, const DaserKV4Pool pool) {
 // ---- pages -> chunk images ---------------------------------------------------------------------------------------
 //
 // The mirror image: records in as 16-byte loads, rows out.  A raw image gets the values as they stand (exact in bf16), an fp8b16
-// image is quantised again (group maximum 448: relative error at most 2^-4).  208 slots of 10 layers and 8 heads into raw images (38 MB
-// in, 136 out): 37 us, 4.7 TB/s.
+// image is quantised again (group maximum 448: relative error at most 2^-4).  208 slots of 10 layers and 8 heads: into raw images (38 MB
+// in, 136 out) 36 us, 4.9 TB/s; into fp8b16 ones (85 out), which is what an engine stores, 37 us, 3.3 TB/s.  The phases of a CTA, records in,
+// barrier, rows out, do not overlap; the largest stall is on its loads.
 template <bool IMG_FP8>
 __global__ void __launch_bounds__(256)
 kv4_save_kernel(const DaserKVJob job, const DaserKV4Pool pool) {
@@ -412,7 +415,7 @@ kv4_save_kernel(const DaserKVJob job, const DaserKV4Pool pool) {
 // sum_d max(q_d hi_d, q_d lo_d) bounds every score of the page from above.  One warp per (page, head).
 // Recomputed from the whole page, so that the result depends on the page alone; only tokens below ctx count (what lies behind
 // them in a page is left over from its last owner).  A page with a key that is not finite gets exponent 127.  A decode step touches one
-// page per sequence: 8 us, a launch and four dependent misses.
+// page per sequence: 6 to 8 us, of which a launch is 2 and the chain of lengths, table, record about 3; the rest has not been looked into.
 __device__ __forceinline__ int pow2_exponent(float a) {
   // the smallest e with a <= 127 * 2^e, for a > 0: a = m * 2^x, m in [1/2, 1), gives e = x - 7, one more if m * 128 > 127
   const int x = (int)(__float_as_uint(a) >> 23) - 126;
@@ -500,6 +503,9 @@ kv4_bounds_read_kernel(const int8_t* __restrict__ codes, const int8_t* __restric
 }
 
 // ---- the codec on its own ----------------------------------------------------------------------------------------
+//
+// A thread takes a group.  67 million values: 30 us to codes (172 MB, 5.8 TB/s), 41 us back (4.2 TB/s; a thread's 32 bytes
+// leave as two 16-byte stores).
 __global__ void __launch_bounds__(256)
 quant_fp4b16_kernel(const __nv_bfloat16* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t groups) {
   for (int64_t g = blockIdx.x * (int64_t)256 + threadIdx.x; g < groups; g += (int64_t)gridDim.x * 256) {
