@@ -4,7 +4,7 @@
 //   sum_h sum_d max(q_hd hi_d, q_hd lo_d) = sum_d Q+_d hi_d + Q-_d lo_d,   Q+ = sum_h max(q_h, 0), Q- = sum_h min(q_h, 0)
 // so the heads of a group collapse into two vectors.  Q+ and Q- are rounded to int8 with one power-of-two scale (it is common to
 // all pages and drops out), to nearest, so that the score lies up to half a step per dim on either side of that bound: of 4096 pages and
-// 128 places one or two go to other pages than by the bound itself with normal queries, 2 to 9 % of them with one loud channel.  That is the
+// 128 places one to three go to other pages than by the bound itself with normal queries, up to 9 % of them with one loud channel.  That is the
 // price of whole numbers: the bounds are int8 already, a page costs 256 integer products, |sum| <= 256 * 127^2 < 2^24, and
 // its score, the sum times the page's power of two, is exact in fp32.  The choice therefore depends on no order of summation.
 // (Q+ and Q- are sums of up to 16 bf16 values in fp64, exact while their exponents lie within 41 of one another, and
