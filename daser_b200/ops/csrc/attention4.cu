@@ -513,7 +513,7 @@ attn4_kernel(const Attn4Params p) {
           const float up = mx == -INFINITY ? 0.f : fmaxf(mx - A4_TOP, seen[nt][e] ? 0.f : -INFINITY);
           seen[nt][e] |= mx > -INFINITY;
           none |= !seen[nt][e];
-          const float al = ex2f(-up);
+          const float al = ex2f(fminf(-up, 0.f));  // (a row's first maximum may lie far below 0: there is nothing to scale yet)
           base[nt][e] += up;
           l[nt][e] *= al;
 #pragma unroll

@@ -1225,3 +1225,22 @@ def test_row_strides_of_the_projections():
     with pytest.raises(ValueError):
         ew.rope_kv_write(rep, i(3, 3, 3), i(5, 6, 7).long(), cos_sin, q_out, hq, hkv, D, B, pool, 0, zero_after=True)
     assert torch.equal(same, before)
+
+
+@pytest.mark.parametrize("level", [-1e4, -200.0, -100.0, 100.0, 1e4])
+@pytest.mark.parametrize("q_lens,ctx_lens,hq,hkv,split", [([1], [300], 8, 1, None), ([1, 1], [300, 40], 16, 2, 5), ([1], [900], 16, 1, 0), ([3], [70], 8, 1, None),
+                                                          ([20], [200], 8, 1, 1), ([40], [300], 8, 1, 3)])
+def test_scores_that_all_lie_far_from_zero(q_lens, ctx_lens, hq, hkv, split, level):
+    """Every score of a row is near `level` (in log2): the first maximum a warp meets is far above or below what it starts from."""
+    from daser_b200.ops import kv_ops
+
+    _, rec, tables, q, start = _setup(q_lens, ctx_lens, hq, hkv, seed=110)
+    g = torch.Generator().manual_seed(111)
+    k = torch.randn(rec.shape[1], hkv, B, D, generator=g)
+    k[..., :16] = level / (16 * 0.1275)  # a group of 16 dims carries the level, the others the differences
+    q = (q.float() / 1.3).to(torch.bfloat16)
+    q[..., :16] = 1.0
+    rec = codec.pack_kv4_records(k, torch.randn(k.shape, generator=g))[None]
+    got = _attend(kv_ops.PagedKV4Pool.from_tensors([rec.cuda()]), 0, tables, q, start, ctx_lens, max(q_lens), hkv, split)
+    want, tol = _oracle(rec[0], tables, q, q_lens, ctx_lens, D**-0.5, prefill=max(q_lens) * hq // hkv >= 64)
+    assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
